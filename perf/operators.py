@@ -5,8 +5,8 @@ Four operators of the serving path, over the packed rows and the per-persona KV 
 * ``sample``: one token per row of logits by temperature, top-k, top-p and min-p from one given uniform
   number a row (``sampling.sample``);
 * ``tree``: attention of a tree of drafted tokens over a persona's KV ring (``tree.tree_attention``);
-* ``commit``: the accepted path of a drafted tree, and its keys and values copied into the rings of all layers
-  (``tree.tree_accept``, ``kv_cache.ring_commit``);
+* ``commit``: the accepted path of a drafted tree, and its keys and values copied into the rings of all layers,
+  (2, layers, slots, KV heads, window, head dim) (``tree.tree_accept``, ``kv_cache.ring_commit``);
 * ``fork``: the rings of a persona copied to other slots, all layers at once (``kv_cache.ring_fork``).
 
 ``own`` chooses between the plain forms (elementary torch operations) and the framework's calls.
@@ -169,7 +169,6 @@ def prepare(case, seed):
         return st
     L, slots = c["L"], c["slots"]
     st["rings"] = _bf16(g, 2, L, slots, n_kv, W, hd)
-    st["k_ring"], st["v_ring"] = list(st["rings"][0].unbind(0)), list(st["rings"][1].unbind(0))
     if c["op"] == "commit":
         B, N = c["B"], c["N"]
         st["parents"], st["n_nodes"] = _trees(c, g)
@@ -181,7 +180,6 @@ def prepare(case, seed):
         other = torch.randint(0, 32000, (B, N), device="cuda", generator=g, dtype=torch.int32)
         st["tokens"] = torch.where(torch.rand(B, N, device="cuda", generator=g) < 0.85, hit, other).contiguous()
         st["tree"] = _bf16(g, 2, L, B, n_kv, N, hd)
-        st["k_tree"], st["v_tree"] = list(st["tree"][0].unbind(0)), list(st["tree"][1].unbind(0))
         return st
     order = torch.randperm(slots, device="cuda", generator=g).tolist()
     n_src = c["pairs"] // c["fan"]
@@ -327,10 +325,9 @@ def run(state):
             return {"out": st["out"], "k_tree": st["k_tree"], "v_tree": st["v_tree"]}
         if st["op"] == "commit":
             path, n_path, following = tree.tree_accept(st["tokens"], st["parents"], st["picks"], st["n_nodes"])
-            kv_cache.ring_commit(st["k_ring"], st["v_ring"], st["k_tree"], st["v_tree"], st["pos"], st["slots"],
-                                 path, n_path)
+            kv_cache.ring_commit(st["rings"], st["tree"], st["pos"], st["slots"], path, n_path)
             return {"path": path, "n_path": n_path, "next": following, "rings": st["rings"]}
-        kv_cache.ring_fork(st["k_ring"], st["v_ring"], st["src"], st["dst"], st["end"])
+        kv_cache.ring_fork(st["rings"], st["src"], st["dst"], st["end"])
         return st["rings"]
     if st["op"] == "sample":
         return _plain_sample(st)
