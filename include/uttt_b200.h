@@ -355,6 +355,67 @@ int uttt_attn_prefill(int B, int T, int start_pos, int hist, int n_heads, int n_
 int uttt_kv_ring_fill(int B, int L, int end_pos, int n_kv, int hd, int W, const void* k_buf, const void* v_buf,
                       const int* slot, void* k_ring, void* v_ring, void* stream);
 
+/* ---- drafted tokens -------------------------------------------------------- */
+/*
+ * Attention of a tree of drafted tokens over the KV rings of a packed batch, to
+ * verify all of them in one step (the reference drafts along one line,
+ * model/uttt_model.py:1052-1179).  Row b holds up to N nodes in rows
+ * b * N .. of qkv and out; node i's parent is parents[b * N + i] < i (anything
+ * else: a root), its depth d the number of its ancestors, its absolute position
+ * pos[b] + d.  pos[b] is the number of positions cached so far.  A node sees the
+ * ring's positions in (pos[b] + d - W, pos[b]) and, of the tree, itself and its
+ * ancestors less than W above it: what uttt_attn_decode gives along its path.
+ *   qkv, k_ring, v_ring, rope_cos / rope_sin   as uttt_attn_decode; the rings
+ *           have n_slots slots, the tables n_pos rows (positions past them take
+ *           the last row); any W.  The rings are only read.
+ *   n_nodes nodes of each row (NULL: N); 0 leaves a row out.
+ *   k_tree, v_tree  BF16 (B, n_kv, N, hd): the nodes' RoPE'd keys and values
+ *   out     BF16 rows (B * N, out_ld), heads concatenated
+ * Nothing is written for the nodes behind a row's last, nor for rows with a slot
+ * outside [0, n_slots) or a negative position.  Nothing that a node does not see
+ * reaches it, whatever its bits.  hd in {32, 64, 128}, n_heads / n_kv <= 8,
+ * N <= 64.  No workspace.
+ */
+int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos, const void* qkv,
+                   int qkv_ld, const int* parents, const int* n_nodes, const int* pos, const int* slot,
+                   const void* k_ring, const void* v_ring, const float* rope_cos, const float* rope_sin, void* k_tree,
+                   void* v_tree, void* out, int out_ld, void* stream);
+/*
+ * The accepted path of each row's tree: node 0 (the token that was pending), then
+ * from every node on its lowest later child whose token is the pick after that
+ * node, until there is none (the rule that keeps a drafted reply equal to the
+ * undrafted one).  tokens, parents, picks: (B, N); path (B, N): the nodes, -1
+ * behind the last; n_path (B); next (B): the pick after the path's last node.
+ * A row without nodes gets n_path 0 and next -1.  N <= 64.
+ */
+int uttt_tree_accept(int B, int N, const int* tokens, const int* parents, const int* n_nodes, const int* picks,
+                     int* path, int* n_path, int* next, void* stream);
+
+/* ---- copies of the KV rings of all layers ------------------------------------ */
+/*
+ * Layer l's rings start l * ring_stride elements behind k_ring / v_ring
+ * ((n_slots, n_kv, W, hd) each, as one layer's in uttt_attn_decode; 16-byte
+ * aligned, strides multiples of 8).
+ *
+ * uttt_kv_ring_commit puts node path[b * N + t], t < n_path[b], of the drafted
+ * keys and values (layer l at k_tree / v_tree + l * tree_stride, (B, n_kv, N, hd)
+ * of uttt_attn_tree) at position pos[b] + t of slot[b]'s rings; of a path longer
+ * than W its last W nodes.  The batch's slots must differ.  Rows with a slot
+ * outside [0, n_slots) or a negative position are left out.
+ *
+ * uttt_kv_ring_fork copies, for each pair i (src, dst and end_pos are HOST
+ * arrays), the places of slot src[i] that hold its first end_pos[i] positions
+ * (min(end_pos[i], W) places; NULL: all) to slot dst[i].  Every source is read as
+ * it was before the call (pairs whose destination another pair still reads wait
+ * for it).  Destinations must differ; slots that would swap in a cycle are
+ * refused (UTTT_ERR_INVALID), like slots out of range, before anything is copied.
+ */
+int uttt_kv_ring_commit(int n_layers, int B, int N, int n_kv, int hd, int W, int n_slots, const void* k_tree,
+                        const void* v_tree, long long tree_stride, void* k_ring, void* v_ring, long long ring_stride,
+                        const int* pos, const int* slot, const int* path, const int* n_path, void* stream);
+int uttt_kv_ring_fork(int n_layers, int n_pairs, int n_kv, int hd, int W, int n_slots, void* k_ring, void* v_ring,
+                      long long ring_stride, const int* src, const int* dst, const int* end_pos, void* stream);
+
 /* ---- row-wise ops -------------------------------------------------------- */
 /* RMSNorm (model/uttt_layer.py:881-896): out = x * rsqrt(mean(x^2) + eps) * weight
  * (weight FP32, rounded to BF16 as weight.to(x.dtype) does; NULL for none). */
@@ -371,6 +432,40 @@ int uttt_embed(int rows, int d, int V, const int* ids, const void* table, void* 
  * receives the best and second-best values per row. */
 int uttt_greedy_argmax(int rows, int V, const void* logits, int logits_f32, long long ld, int active_limit,
                        int stop_free, int* ids, float* top2, void* stream);
+
+/*
+ * Sampling of one token per row (_sample_next_token, model/uttt_model.py:1181-1235,
+ * with top-k and min-p) from given uniform numbers, for packed decode batches.
+ * The candidates are those of uttt_greedy_argmax (without its BF16 rounding);
+ * a NaN or -inf logit is none.  With m the largest logit, w_i = exp((s_i - m) / T);
+ * in the order (logit descending, id ascending) top_k keeps the first k, top_p
+ * then those whose mass before them is at most top_p of the mass that is left,
+ * min_p those with w_i >= min_p.  The pick is the lowest id i for which the kept
+ * mass up to and with i exceeds u of the kept mass.  Weights are 64-bit whole
+ * numbers of 2^-45, so the pick does not depend on the batch or the grid.
+ * Settings per row (device arrays of `rows`) or, where NULL, for all rows:
+ * temperature <= 1e-5 picks greedily; top_k <= 0, top_p >= 1 and min_p <= 0 are
+ * off.  Row r's uniform number, in [0, 1) (others are clamped), is
+ * u[r * u_ld + u_index[r]] (u_index NULL: 0; clamped to [0, u_len)).
+ *   logits  rows of V (ld elements apart), FP32 or BF16, any alignment
+ *   ids     the picks; kept (optional) the number of kept ids; prob (optional)
+ *           the pick's share of the kept mass.  A row without candidates gets
+ *           the id that uttt_greedy_argmax gives it, kept 0 and prob 0.
+ * V <= 262144, rows <= 65535.  No workspace.
+ */
+typedef struct UtttSampling {
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all;
+  float min_p_all;
+} UtttSampling;
+int uttt_sample(int rows, int V, const void* logits, int logits_f32, long long ld, int active_limit, int stop_free,
+                const UtttSampling* opt, const float* u, long long u_ld, const int* u_index, int u_len, int* ids,
+                int* kept, float* prob, void* stream);
 
 /* ---- device-side scheduling of a packed decode batch ------------------------ */
 /*

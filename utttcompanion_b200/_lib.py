@@ -73,9 +73,16 @@ SIGNATURES: Dict[str, tuple] = {
     "uttt_attn_decode": (i32, [i32, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp]),
     "uttt_attn_prefill": (i32, [i32, i32, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp]),
     "uttt_kv_ring_fill": (i32, [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
+    "uttt_attn_tree": (i32, [i32, i32, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                             vp, i32, vp]),
+    "uttt_tree_accept": (i32, [i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "uttt_kv_ring_commit": (i32, [i32, i32, i32, i32, i32, i32, i32, vp, vp, C.c_longlong, vp, vp, C.c_longlong, vp,
+                                  vp, vp, vp, vp]),
+    "uttt_kv_ring_fork": (i32, [i32, i32, i32, i32, i32, i32, vp, vp, C.c_longlong, vp, vp, vp, vp]),
     "uttt_rmsnorm": (i32, [i32, i32, vp, C.c_longlong, vp, f32, vp, C.c_longlong, vp]),
     "uttt_embed": (i32, [i32, i32, i32, vp, vp, vp, vp]),
     "uttt_greedy_argmax": (i32, [i32, i32, vp, i32, C.c_longlong, i32, i32, vp, vp, vp]),
+    "uttt_sample": (i32, [i32, i32, vp, i32, C.c_longlong, i32, i32, vp, vp, C.c_longlong, vp, i32, vp, vp, vp, vp]),
     "uttt_engine_step": (i32, [i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp]),
     "uttt_engine_admit": (i32, [i32, vp, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, vp]),
     "uttt_pack_read_copies": (i32, [i32, i32, i32, vp, vp, vp, vp, vp, vp]),
@@ -91,6 +98,13 @@ class Segment(C.Structure):
     _fields_ = [("start", C.c_int), ("len", C.c_int), ("op", C.c_int), ("out_f32", C.c_int),
                 ("out", C.c_void_p), ("out_ld", C.c_longlong), ("aux", C.c_void_p), ("aux_ld", C.c_longlong),
                 ("scale", C.c_float), ("aux2", C.c_void_p)]
+
+
+class Sampling(C.Structure):
+    """``UtttSampling`` of include/uttt_b200.h."""
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("temperature_all", C.c_float), ("top_k_all", C.c_int), ("top_p_all", C.c_float),
+                ("min_p_all", C.c_float)]
 
 
 SEG_STORE, SEG_RESID, SEG_RMSNORM, SEG_SIGMOID, SEG_NORM = 0, 1, 2, 3, 4

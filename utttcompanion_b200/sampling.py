@@ -1,0 +1,104 @@
+"""Sampling of one token per row from given random numbers (``uttt_sample``).
+
+``UtttB200.greedy``'s counterpart at temperature > 0: the rules of
+``uTTTModel._sample_next_token`` (``model/uttt_model.py:1181-1235``) with top-k
+and min-p beside top-p, for every row of a packed batch in one launch, each row
+with its own settings.  The uniform numbers are inputs, so a pick depends on
+its row's logits, settings and number alone.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple, Optional, Union
+
+import torch
+
+from . import _lib
+from .fastweight import _require_cuda
+
+Setting = Union[None, int, float, torch.Tensor]
+
+
+class Sampled(NamedTuple):
+    """``ids`` int32 (rows,); ``kept`` int32 (rows,), the ids that the settings left; ``prob`` FP32 (rows,), the
+    pick's share of their mass."""
+    ids: torch.Tensor
+    kept: torch.Tensor
+    prob: torch.Tensor
+
+
+def check_settings(temperature: float = 1.0, top_k: Optional[int] = None, top_p: Optional[float] = None,
+                   min_p: Optional[float] = None) -> None:
+    """The ``ValueError`` of settings that no call takes (the reference's checks, ``:1190-1197``)."""
+    if not math.isfinite(temperature) or temperature < 0:
+        raise ValueError("temperature must be finite and nonnegative")
+    if top_k is not None and (int(top_k) != top_k or not 0 <= top_k < 2 ** 31):
+        raise ValueError("top_k must be a nonnegative integer")
+    if top_p is not None and (not math.isfinite(top_p) or not 0 < top_p <= 1):
+        raise ValueError("top_p must be finite and in (0, 1]")
+    if min_p is not None and (not math.isfinite(min_p) or not 0 <= min_p <= 1):
+        raise ValueError("min_p must be finite and in [0, 1]")
+
+
+def _per_row(name: str, v: Setting, off, dtype: torch.dtype, rows: int, device: torch.device):
+    """(device pointer or None, value for all rows)."""
+    if isinstance(v, torch.Tensor):
+        if v.dtype != dtype or v.dim() != 1 or v.shape[0] != rows or not v.is_contiguous() or v.device != device:
+            raise ValueError(f"{name} per row must be a contiguous {dtype} tensor of {rows} on {device}")
+        return v.data_ptr(), off
+    return None, off if v is None else v
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, top_k: Setting = None,
+           top_p: Setting = None, min_p: Setting = None, active_limit: Optional[int] = None,
+           stop_free: bool = False, u_index: Optional[torch.Tensor] = None) -> Sampled:
+    """One id per row of FP32 or BF16 ``logits`` (rows, V).
+
+    ``u``: FP32 uniform numbers in [0, 1), (rows,), or (rows, n) with ``u_index`` int32 (rows,) naming each
+    row's column.  ``temperature``, ``top_k``, ``top_p``, ``min_p``: a number for all rows or a device tensor
+    (FP32; ``top_k`` int32) of one per row, whose values the device takes as ``include/uttt_b200.h`` says;
+    a temperature of at most 1e-5 picks greedily, ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 are off.
+    PAD / BOS / UNK and ids from ``active_limit`` on are never picked (nor ids 2, 4 and 5 when
+    ``stop_free``), as by ``UtttB200.greedy``.  Runs on the current stream of the logits' device."""
+    _require_cuda(logits, u, u_index)
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] <= 6:
+        raise ValueError("logits must be FP32 or BF16 (rows, V) with V > 6")
+    dev = logits.device
+    rows, V = logits.shape
+    if rows == 0:
+        return Sampled(torch.empty(0, dtype=torch.int32, device=dev), torch.empty(0, dtype=torch.int32, device=dev),
+                       torch.empty(0, device=dev))
+    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < V):
+        logits = logits.contiguous()
+    if u.dtype != torch.float32 or u.device != dev or u.shape[0] != rows or u.dim() not in (1, 2) \
+            or not u.is_contiguous() or u.numel() == 0:
+        raise ValueError("u must be a contiguous FP32 (rows,) or (rows, n) tensor beside the logits")
+    if u_index is None and u.dim() == 2 and u.shape[1] != 1:
+        raise ValueError("u of several numbers a row needs u_index")
+    if u_index is not None and (u_index.dtype != torch.int32 or u_index.shape != (rows,) or u_index.device != dev
+                                or not u_index.is_contiguous()):
+        raise ValueError("u_index must be a contiguous int32 (rows,) tensor beside the logits")
+    check_settings(*(d if isinstance(v, torch.Tensor) else v
+                     for v, d in ((temperature, 1.0), (top_k, None), (top_p, None), (min_p, None))))
+    limit = V if active_limit is None else int(active_limit)
+    if limit <= 2:
+        raise ValueError("Active vocabulary must include EOS")
+    f = torch.float32
+    opt = _lib.Sampling()
+    opt.temperature, opt.temperature_all = _per_row("temperature", temperature, 1.0, f, rows, dev)
+    opt.top_k, opt.top_k_all = _per_row("top_k", top_k, 0, torch.int32, rows, dev)
+    opt.top_p, opt.top_p_all = _per_row("top_p", top_p, 1.0, f, rows, dev)
+    opt.min_p, opt.min_p_all = _per_row("min_p", min_p, 0.0, f, rows, dev)
+    n_u = u.shape[1] if u.dim() == 2 else 1
+    ids, kept = torch.empty(2, rows, dtype=torch.int32, device=dev).unbind(0)
+    prob = torch.empty(rows, dtype=f, device=dev)
+    with torch.cuda.device(dev):
+        st = _lib.load().uttt_sample(rows, V, logits.data_ptr(), int(logits.dtype == f),
+                                     logits.stride(0) if rows > 1 else V, limit, int(stop_free), C.byref(opt),
+                                     u.data_ptr(), n_u, None if u_index is None else u_index.data_ptr(), n_u,
+                                     ids.data_ptr(), kept.data_ptr(), prob.data_ptr(),
+                                     torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(st, "uttt_sample")
+    return Sampled(ids, kept, prob)

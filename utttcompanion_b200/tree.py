@@ -1,0 +1,118 @@
+"""Drafted tokens as a tree: attention of all its nodes over the KV rings, and the path that the picks accept.
+
+One packed step verifies a tree of drafted tokens per persona (``UtttB200.tree_step``): every node attends to the
+persona's KV ring and to its own path of the tree (``tree_attention``), the model's pick after each node decides
+which path stands (``tree_accept``), and ``kv_cache.ring_commit`` puts that path's keys and values into the rings.
+The reference drafts along one line (``model/uttt_model.py:1052-1179``).
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from . import _lib
+from .fastweight import _require_cuda
+
+MAX_NODES = 64
+
+
+def check_tree(parents: Sequence[int]) -> None:
+    """The ``ValueError`` of a host-side tree that no call takes: node 0 is the root (-1), every other node's
+    parent comes before it, and there are at most ``MAX_NODES``."""
+    if not 1 <= len(parents) <= MAX_NODES:
+        raise ValueError(f"a drafted tree has 1 to {MAX_NODES} nodes")
+    if parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(parents) if i > 0):
+        raise ValueError("node 0 is the root (parent -1) and a node's parent comes before it")
+
+
+def _int_rows(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 {shape} tensor on {device}")
+    return t.data_ptr()
+
+
+def tree_attention(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
+                   k_ring: torch.Tensor, v_ring: torch.Tensor, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
+                   n_heads: int, n_nodes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                   k_tree: Optional[torch.Tensor] = None, v_tree: Optional[torch.Tensor] = None
+                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Attention of B trees of N nodes (``uttt_attn_tree``); returns ``(out, k_tree, v_tree)``.
+
+    ``qkv`` BF16 (B * N, [q | k | v] heads), rows any stride; ``parents`` int32 (B, N); ``pos`` and ``slots``
+    int32 (B,): positions cached so far and ring slot of each row; ``k_ring`` / ``v_ring`` BF16
+    (slots, n_kv, W, hd) of one layer, only read; ``rope_cos`` / ``rope_sin`` FP32 (positions, hd);
+    ``n_nodes`` int32 (B,): nodes of each row (default N).  ``out`` BF16 (B * N, n_heads * hd), rows any stride,
+    ``k_tree`` / ``v_tree`` BF16 (B, n_kv, N, hd): taken if given, else new (zeros); what lies behind a row's last
+    node is left as it was."""
+    _require_cuda(qkv, parents, pos, slots, k_ring, v_ring, rope_cos, rope_sin, n_nodes, out, k_tree, v_tree)
+    dev, bf = qkv.device, torch.bfloat16
+    if parents.dim() != 2 or k_ring.dim() != 4:
+        raise ValueError("parents must be (B, N) and the rings (slots, n_kv, W, hd)")
+    B, N = parents.shape
+    n_slots, n_kv, W, hd = k_ring.shape
+    if k_ring.dtype != bf or v_ring.dtype != bf or v_ring.shape != k_ring.shape or not k_ring.is_contiguous() \
+            or not v_ring.is_contiguous() or k_ring.device != dev or v_ring.device != dev:
+        raise ValueError("the rings must be contiguous BF16 tensors of one shape beside qkv")
+    if not 1 <= N <= MAX_NODES:
+        raise ValueError(f"a drafted tree has 1 to {MAX_NODES} nodes")
+    if n_heads < 1 or n_heads % n_kv or qkv.dtype != bf or qkv.dim() != 2 or qkv.shape[0] != B * N \
+            or qkv.shape[1] < (n_heads + 2 * n_kv) * hd or qkv.stride(1) != 1:
+        raise ValueError("qkv must be BF16 (B * N, (n_heads + 2 * n_kv) * hd) rows")
+    for t in (rope_cos, rope_sin):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or not t.is_contiguous() or t.device != dev \
+                or t.shape[0] != rope_cos.shape[0] or t.shape[0] < 1:
+            raise ValueError("rope_cos and rope_sin must be contiguous FP32 (positions, hd) tables")
+    if out is None:
+        out = torch.zeros(B * N, n_heads * hd, dtype=bf, device=dev)
+    elif out.dtype != bf or out.dim() != 2 or out.shape[0] != B * N or out.shape[1] != n_heads * hd \
+            or out.stride(1) != 1 or out.device != dev:
+        raise ValueError("out must be BF16 (B * N, n_heads * hd) rows")
+    if k_tree is None:
+        k_tree = torch.zeros(B, n_kv, N, hd, dtype=bf, device=dev)
+    if v_tree is None:
+        v_tree = torch.zeros(B, n_kv, N, hd, dtype=bf, device=dev)
+    for t in (k_tree, v_tree):
+        if t.dtype != bf or t.shape != (B, n_kv, N, hd) or not t.is_contiguous() or t.device != dev:
+            raise ValueError("k_tree and v_tree must be contiguous BF16 (B, n_kv, N, hd)")
+    args = (_int_rows("parents", parents, (B, N), dev), _int_rows("n_nodes", n_nodes, (B,), dev),
+            _int_rows("pos", pos, (B,), dev), _int_rows("slots", slots, (B,), dev))
+    if B == 0:
+        return out, k_tree, v_tree
+    many = B * N > 1
+    with torch.cuda.device(dev):
+        st = _lib.load().uttt_attn_tree(B, N, n_heads, n_kv, hd, W, n_slots, rope_cos.shape[0], qkv.data_ptr(),
+                                        qkv.stride(0) if many else qkv.shape[1], *args, k_ring.data_ptr(),
+                                        v_ring.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
+                                        k_tree.data_ptr(), v_tree.data_ptr(), out.data_ptr(),
+                                        out.stride(0) if many else out.shape[1],
+                                        torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(st, "uttt_attn_tree")
+    return out, k_tree, v_tree
+
+
+def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor,
+                n_nodes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The accepted path of each tree (``uttt_tree_accept``): ``(path (B, N), n_path (B,), next (B,))`` int32.
+
+    ``tokens``, ``parents``, ``picks`` int32 (B, N): each node's drafted token and parent, and the model's pick
+    after it.  The path is node 0, then from each node on its lowest later child that holds the pick; -1 behind
+    its last node, whose pick is ``next``."""
+    _require_cuda(tokens, parents, picks, n_nodes)
+    if tokens.dim() != 2 or not 1 <= tokens.shape[1] <= MAX_NODES:
+        raise ValueError(f"tokens must be (B, N) with 1 to {MAX_NODES} nodes")
+    dev, shape = tokens.device, tuple(tokens.shape)
+    B, N = shape
+    ptrs = (_int_rows("tokens", tokens, shape, dev), _int_rows("parents", parents, shape, dev),
+            _int_rows("n_nodes", n_nodes, (B,), dev), _int_rows("picks", picks, shape, dev))
+    path = torch.empty(B, N, dtype=torch.int32, device=dev)
+    n_path, following = torch.empty(2, B, dtype=torch.int32, device=dev).unbind(0)
+    if B:
+        with torch.cuda.device(dev):
+            st = _lib.load().uttt_tree_accept(B, N, *ptrs, path.data_ptr(), n_path.data_ptr(), following.data_ptr(),
+                                              torch.cuda.current_stream(dev).cuda_stream)
+        _lib.check(st, "uttt_tree_accept")
+    return path, n_path, following
