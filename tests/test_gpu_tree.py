@@ -84,11 +84,15 @@ def _check(c, nh, out, kt, vt, rows=None):
     (1, 9, 15, 3, 64, 200, [63], "random", None),                 # five heads a KV head; tiles that end inside
     (1, 17, 18, 3, 32, 63, [62], "star", None),
     (1, 2, 3, 3, 128, 64, [64], "chain", None),
+    # enough rows that nothing splits the keys; ragged trees and lengths
+    (64, 16, 20, 5, 128, 512, [32 + 64 * i for i in range(64)], "random", [1 + i % 16 for i in range(64)]),
+    (40, 64, 12, 4, 64, 300, [1 + 37 * i for i in range(40)], "random", [1 + (i * 7) % 64 for i in range(40)]),
+    (80, 9, 8, 2, 64, 130, [100 + i for i in range(80)], "star", None),
 ])
 def test_tree_attention(B, N, nh, nkv, hd, W, pos, kind, nodes):
     c = _case(B, N, nh, nkv, hd, W, pos, kind, nodes, seed=N * W + hd)
     rings = c["k_ring"].clone(), c["v_ring"].clone()
-    _check(c, nh, *_run(c, nh), rows=None if B < 10 else (0, 13, B - 1))
+    _check(c, nh, *_run(c, nh), rows=None if B < 10 else (0, 2, 13, 14, 15, 31, B - 2, B - 1))
     assert torch.equal(rings[0], c["k_ring"]) and torch.equal(rings[1], c["v_ring"])
 
 

@@ -556,9 +556,483 @@ int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
   return launch_status();
 }
 
+// ---------------------------------------------------------------------------
+// The same on tcgen05, for many rows (head dim 64 or 128).
+//
+// One CTA takes 128 rows (TMEM lanes).  Tile by tile: S = Q K^T into one of two
+// TMEM buffers; the thread that owns a row reads its 64 scores, keeps the running
+// maximum and sum, and writes P_hi and P_lo (BF16, packed in pairs) over the same
+// 64 columns, from where they enter O += P V as the A operand; O stays in TMEM.
+// O is rescaled only when a row's maximum grows by more than 2^8 (weights up to
+// 2^8 lose nothing: P_hi / P_lo and the FP32 sums are relative).  Warp 0 issues the
+// TMA loads, warp 1 the MMAs, warps 2-5 own a row per thread; they also rotate Q
+// and, in one CTA of the cluster, the drafted keys, which are its first tile.
+// Two CTAs of 96 KB and 256 TMEM columns share an SM.
+// ---------------------------------------------------------------------------
+constexpr int TT_THREADS = 192;
+constexpr float TT_GROWTH = 8.f;         // log2 of the growth that a rescaling waits for
+
+template <int HD>
+struct TtLayout {
+  static constexpr int BLK = HD / 64;             // 64-column blocks of a head vector
+  static constexpr int Q_BYTES = 128 * HD * 2;    // per block [128 rows][128 B], K-major SW128
+  static constexpr int TILE = TR_KT * HD * 2;     // per block [64 keys][128 B]
+  static constexpr int K0 = Q_BYTES, V0 = Q_BYTES + 2 * TILE;   // two slots each
+  static constexpr int OLD = HD + 4;              // row stride of the partial outputs (floats)
+  static constexpr int USED = Q_BYTES + 4 * TILE > 128 * OLD * 4 ? Q_BYTES + 4 * TILE : 128 * OLD * 4;
+  static constexpr int SMEM = 1024 + USED;
+};
+
+// D[tmem] (+)= A[tmem] * B[smem]^T (kind::f16): A is 128 lanes of packed BF16 pairs
+__device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// grid (S, n_kv * row blocks, B), cluster (S, 1, 1): CTA z takes tiles [nt * z / S, nt * (z + 1) / S) of the nt
+// tiles: tile 0 holds the drafted keys, tile t > 0 the ring's places 64 (t - 1) ..
+template <int HD>
+__global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __grid_constant__ CUtensorMap tmK,
+                                                                     const __grid_constant__ CUtensorMap tmV,
+                                                                     const TreeArgs a) {
+  using LY = TtLayout<HD>;
+  constexpr int CH = HD / 8;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], ready;
+  __shared__ uint32_t tmem_slot;
+  __shared__ u64 anc_s[2][TR_KT], bad_keys;
+  __shared__ int jump_s[2][TR_KT], depth_s[TR_KT];
+  __shared__ float cml[2][128];
+  __shared__ u64 bad_mask[8];            // tiles with non-finite values: their keys ...
+  __shared__ int bad_tile[8], n_bad;     // ... and numbers
+  uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *sQ = base, *sK = base + LY::K0, *sV = base + LY::V0;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int S = gridDim.x, z = blockIdx.x, b = blockIdx.z;
+  const int g = blockIdx.y % a.n_kv, row0 = blockIdx.y / a.n_kv * 128;
+  const int N = a.N, rep = a.rep, W = a.W;
+  pdl_wait();
+  pdl_trigger();
+  const int n = a.n_nodes ? min(a.n_nodes[b], N) : N;
+  const int p0 = a.pos[b], sl = a.slot[b];
+  const int rows = n * rep;
+  if (row0 >= rows || sl < 0 || sl >= a.n_slots || p0 < 0) return;   // the same in the whole cluster
+  const int nvalid = min(p0, W), nt = (nvalid + TR_KT - 1) / TR_KT + 1;
+  const int t_lo = (int)((long long)nt * z / S), t_hi = (int)((long long)nt * (z + 1) / S), cnt = t_hi - t_lo;
+  const bool has_tree = t_lo == 0 && cnt > 0;
+  const int act = 32 * ((min(128, rows - row0) + 31) / 32);   // threads that own rows; warps of padding rows rest
+  // sequence i of the CTA is tile t_lo + i in slot i & 1; fills of a slot by TMA before it
+  auto tma_fills = [&](int i) { return (i >> 1) - (has_tree && !(i & 1) ? 1 : 0); };
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], act);
+    }
+    mbar_init(&ready, 128);
+    fence_mbarrier_init();
+    n_bad = 0;
+  }
+  if (warp == 1) tmem_alloc(&tmem_slot, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot, tO = tmem + 128;   // S / P: two buffers of 64 columns, O: HD columns
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+      const int head = sl * a.n_kv + g;
+      auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* empty, int i) {
+        if (i >= cnt || (has_tree && i == 0)) return;
+        const int s = i & 1;
+        if (i >= 2) mbar_wait(&empty[s], ((i >> 1) - 1) & 1, nullptr);
+        mbar_arrive_expect_tx(&full[s], LY::TILE);
+#pragma unroll
+        for (int h = 0; h < LY::BLK; ++h)
+          tma_load_3d(ring + s * LY::TILE + h * 8192, tm, &full[s], h * 64, (t_lo + i - 1) * TR_KT, head);
+      };
+      load(&tmK, sK, k_full, k_empty, 0);
+      for (int i = 0; i < cnt; ++i) {
+        load(&tmK, sK, k_full, k_empty, i + 1);
+        load(&tmV, sV, v_full, v_empty, i);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && cnt > 0) {
+      const uint32_t id_s = idesc_bf16(128, 64, false, false);   // A = Q K-major, B = K K-major
+      const uint32_t id_o = idesc_bf16(128, HD, false, true);    // A = P in TMEM, B = V MN-major
+      const uint32_t qa = smem_u32(sQ);
+      mbar_wait(&ready, 0, nullptr);
+      auto issue_s = [&](int i) {
+        const int s = i & 1;
+        if (!(has_tree && i == 0)) mbar_wait(&k_full[s], tma_fills(i) & 1, nullptr);
+        // P of sequence i - 2 has left this buffer
+        if (i >= 2) mbar_wait(&v_empty[s], ((i >> 1) - 1) & 1, nullptr);
+        tc_fence_after();
+        const uint32_t ka = smem_u32(sK + s * LY::TILE);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          mma_bf16(tmem + s * 64, sdesc_sw128(qa + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
+                   sdesc_sw128(ka + (k >> 2) * 8192 + (k & 3) * 32, 16, 1024), id_s, k > 0 ? 1u : 0u);
+        mma_commit(&s_full[s]);
+        mma_commit(&k_empty[s]);
+      };
+      issue_s(0);
+      for (int i = 0; i < cnt; ++i) {
+        if (i + 1 < cnt) issue_s(i + 1);
+        const int s = i & 1;
+        if (!(has_tree && i == 0)) mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
+        mbar_wait(&p_full[s], (i >> 1) & 1, nullptr);
+        tc_fence_after();
+        const uint32_t va = smem_u32(sV + s * LY::TILE), pa = tmem + s * 64;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)      // P_hi V (columns 0 .. 31), then P_lo V (32 .. 63): 8 columns per 16 keys
+          mma_bf16_ts(tO, pa + k * 8, sdesc_sw128(va + (k & 3) * 2048, 8192, 1024), id_o,
+                      (i > 0 || k > 0) ? 1u : 0u);
+        mma_commit(&v_empty[s]);
+      }
+    }
+  } else {
+    const int ti = tid - 64;             // 0 .. 127
+    // ---- every node's path, as in attn_tree_kernel
+    const int par_i = ti < N ? a.parents[(size_t)b * N + ti] : -1;
+    if (ti < TR_KT) {
+      anc_s[0][ti] = 1ull << ti;
+      jump_s[0][ti] = ti < n && par_i >= 0 && par_i < ti ? par_i : -1;
+    }
+    named_bar(1, 128);
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      if (ti < TR_KT) {
+        const int j = jump_s[k & 1][ti];
+        anc_s[(k & 1) ^ 1][ti] = anc_s[k & 1][ti] | (j >= 0 ? anc_s[k & 1][j] : 0ull);
+        jump_s[(k & 1) ^ 1][ti] = j >= 0 ? jump_s[k & 1][j] : -1;
+      }
+      named_bar(1, 128);
+    }
+    if (ti < TR_KT) {
+      u64 m = anc_s[0][ti];
+      const int d = __popcll(m) - 1;
+      depth_s[ti] = d;
+      if (d >= W)
+        for (u64 rest = m; rest; rest &= rest - 1) {
+          const int j = __ffsll((long long)rest) - 1;
+          if (d - (__popcll(anc_s[0][j]) - 1) >= W) m &= ~(1ull << j);
+        }
+      anc_s[1][ti] = m;
+    }
+    named_bar(1, 128);
+    // ---- Q, and the drafted keys and values
+    const __nv_bfloat16* qrows = a.qkv + (size_t)b * N * a.qkv_ld;
+    const int k_col = (a.n_kv * rep + g) * HD, v_col = k_col + a.n_kv * HD;
+    const size_t ring0 = ((size_t)sl * a.n_kv + g) * (size_t)W * HD;
+    auto table_row = [&](int node) {
+      return (size_t)min((long long)p0 + depth_s[node], (long long)a.n_pos - 1) * HD;
+    };
+    auto put = [&](uint8_t* t, int blk, int r, int c, uint4 v) {
+      *reinterpret_cast<uint4*>(t + (c >> 3) * blk + sw128_offset(r, (c & 7) * 16)) = v;
+    };
+    for (int i = ti; i < 128 * CH / 2; i += 128) {
+      const int r = i / (CH / 2), c = i % (CH / 2), row = row0 + r;
+      uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
+      if (row < rows) {
+        const int node = row / rep;
+        const __nv_bfloat16* x = qrows + (size_t)node * a.qkv_ld + (size_t)(g * rep + row % rep) * HD;
+        q0 = load8(x + c * 8, a.vec_in);
+        q1 = load8(x + HD / 2 + c * 8, a.vec_in);
+        const size_t tr = table_row(node);
+        rope8(q0, q1, a.cos_t + tr, a.sin_t + tr, c * 8, HD / 2, a.vec_in);
+      }
+      put(sQ, 16384, r, c, q0);
+      put(sQ, 16384, r, c + CH / 2, q1);
+    }
+    if (has_tree) {
+      for (int i = ti; i < TR_KT * CH / 2; i += 128) {
+        const int r = i / (CH / 2), c = i % (CH / 2);
+        uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0, v0 = k0, v1 = k0;
+        if (r < n) {
+          const __nv_bfloat16* x = qrows + (size_t)r * a.qkv_ld;
+          k0 = load8(x + k_col + c * 8, a.vec_in);
+          k1 = load8(x + k_col + HD / 2 + c * 8, a.vec_in);
+          v0 = load8(x + v_col + c * 8, a.vec_in);
+          v1 = load8(x + v_col + HD / 2 + c * 8, a.vec_in);
+          const size_t tr = table_row(r);
+          rope8(k0, k1, a.cos_t + tr, a.sin_t + tr, c * 8, HD / 2, a.vec_in);
+          if (row0 == 0) {
+            const size_t o = (((size_t)b * a.n_kv + g) * N + r) * HD + c * 8;
+            *reinterpret_cast<uint4*>(a.ktree + o) = k0;
+            *reinterpret_cast<uint4*>(a.ktree + o + HD / 2) = k1;
+            *reinterpret_cast<uint4*>(a.vtree + o) = v0;
+            *reinterpret_cast<uint4*>(a.vtree + o + HD / 2) = v1;
+          }
+        }
+        put(sK, 8192, r, c, k0);
+        put(sK, 8192, r, c + CH / 2, k1);
+        put(sV, 8192, r, c, v0);
+        put(sV, 8192, r, c + CH / 2, v1);
+      }
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(&ready);
+
+    // ---- one row per thread: row i = node i / rep, head i % rep of the group
+    const int quad = warp & 3, i_row = quad * 32 + lane, row = row0 + i_row;
+    const bool valid = row < rows, active = i_row < act;
+    const int node = valid ? row / rep : 0, dep = depth_s[node];
+    const u64 anc = anc_s[1][node];
+    const int next = p0 % W;
+    const uint32_t trow = (uint32_t)(quad * 32) << 16;
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; active && i < cnt; ++i) {
+      const int t = t_lo + i, s = i & 1, j0 = (t - 1) * TR_KT;
+      const bool is_tree = t == 0;
+      const int rel = is_tree ? 0 : (j0 - next + W) % W;
+      const bool edge = is_tree || j0 + TR_KT > nvalid || rel < TR_KT || rel + TR_KT > W;
+      // scores i are issued once values i - 2 have been used: after this wait v_full's phase can be told
+      mbar_wait(&s_full[s], (i >> 1) & 1, nullptr);
+      tc_fence_after();
+      if (edge) {
+        // 0 * NaN would let a key's value reach rows that do not see it: such values leave the product and
+        // are added at the end to the rows that do
+        if (!is_tree) mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
+        if (i_row == 0) bad_keys = 0ull;
+        named_bar(2, act);
+        for (int k = i_row; k < TR_KT * CH; k += act) {
+          const int r = k / CH, c = k % CH;
+          uint4* p = reinterpret_cast<uint4*>(sV + s * LY::TILE + (c >> 3) * 8192 + sw128_offset(r, (c & 7) * 16));
+          const uint4 v = *p;
+          if (has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w)) {
+            *p = make_uint4(finite_only(v.x), finite_only(v.y), finite_only(v.z), finite_only(v.w));
+            atomicOr(&bad_keys, 1ull << r);
+          }
+        }
+        fence_proxy_async_smem();
+        named_bar(2, act);
+        if (i_row == 0 && bad_keys != 0ull && n_bad < 8) {   // at most a tree, a last tile and three of the edge
+          bad_mask[n_bad] = bad_keys;
+          bad_tile[n_bad++] = t;
+        }
+      }
+      float sv[64];
+#pragma unroll
+      for (int c = 0; c < 64; c += 16)
+        tmem_ld16(tmem + s * 64 + c + trow, *reinterpret_cast<float(*)[16]>(&sv[c]));
+      tmem_wait_ld();
+      float mt = -INFINITY;
+      if (edge) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) {
+          bool see;
+          if (is_tree) {
+            see = (anc >> c) & 1ull;
+          } else {
+            int back = j0 + c - next;
+            if (back < 0) back += W;
+            see = j0 + c < nvalid && back > dep;
+          }
+          if (!see) sv[c] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 64; ++c) mt = fmaxf(mt, sv[c]);
+      mt *= a.scale_log2;
+      const bool grow = mt > m + TT_GROWTH || m == -INFINITY;
+      if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
+        // O of this warp's rows holds sequences .. i - 1: their MMAs end first
+        if (i > 0) mbar_wait(&v_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, nullptr);
+        tc_fence_after();
+        const float c = grow && m != -INFINITY ? exp2f(m - mt) : 1.f;
+        l *= c;
+#pragma unroll
+        for (int k = 0; k < HD; k += 16) {
+          float ov[16];
+          uint32_t ou[16];
+          tmem_ld16(tO + k + trow, ov);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ou[e] = __float_as_uint(ov[e] * c);
+          tmem_st16(tO + k + trow, ou);
+        }
+      }
+      if (grow) m = mt;
+      const float ref = m == -INFINITY ? 0.f : m;   // nothing seen yet: every weight below is 0
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = exp2f(fmaf(sv[h * 32 + 2 * e], a.scale_log2, -ref));
+          const float y = exp2f(fmaf(sv[h * 32 + 2 * e + 1], a.scale_log2, -ref));
+          l += x + y;
+          hi[e] = pack_bf16x2(x, y);
+          lo[e] = pack_bf16x2(x - bf16_lo(hi[e]), y - bf16_hi(hi[e]));
+        }
+        tmem_st16(tmem + s * 64 + h * 16 + trow, hi);
+        tmem_st16(tmem + s * 64 + 32 + h * 16 + trow, lo);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[s]);
+    }
+
+    // ---- O -> BF16 rows of out, or partials for the cluster
+    if (active && cnt > 0) mbar_wait(&v_empty[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1, nullptr);
+    tc_fence_after();
+    named_bar(1, 128);                   // bad_* is complete, no tile is in use any more
+    const float inv = 1.f / l;
+    float* part = reinterpret_cast<float*>(base) + (size_t)i_row * LY::OLD;
+    __nv_bfloat16* dst = a.out + ((size_t)b * N + node) * a.out_ld + (size_t)(g * rep + row % rep) * HD;
+    if (active) {
+#pragma unroll
+      for (int k = 0; k < HD; k += 16) {
+        float ov[16];
+        if (cnt > 0) {
+          tmem_ld16(tO + k + trow, ov);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) ov[e] = 0.f;
+        }
+        for (int q = 0; q < n_bad; ++q)
+          for (u64 rest = bad_mask[q]; rest; rest &= rest - 1) {
+            const int key = __ffsll((long long)rest) - 1, t = bad_tile[q];
+            int back = (t - 1) * TR_KT + key - next;
+            if (back < 0) back += W;
+            const bool see = t == 0 ? (anc >> key) & 1ull : (t - 1) * TR_KT + key < nvalid && back > dep;
+            if (!see) continue;
+            const __nv_bfloat16* v = t == 0 ? qrows + (size_t)key * a.qkv_ld + v_col
+                                            : a.vring + ring0 + (size_t)((t - 1) * TR_KT + key) * HD;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = __bfloat162float(v[k + e]);
+              if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) ov[e] += x;
+            }
+          }
+        if (S > 1) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(part + k + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+        } else if (valid) {
+          if (a.vec_out) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              *reinterpret_cast<uint4*>(dst + k + e) =
+                  make_uint4(pack_bf16x2(ov[e] * inv, ov[e + 1] * inv), pack_bf16x2(ov[e + 2] * inv, ov[e + 3] * inv),
+                             pack_bf16x2(ov[e + 4] * inv, ov[e + 5] * inv),
+                             pack_bf16x2(ov[e + 6] * inv, ov[e + 7] * inv));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dst[k + e] = __float2bfloat16(ov[e] * inv);
+          }
+        }
+      }
+    }
+    cml[0][i_row] = m;
+    cml[1][i_row] = l;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 256);
+  if (S == 1) return;
+  // every CTA finishes every S-th row of the block
+  cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  const int live = min(128, rows - row0);
+  float* part0 = reinterpret_cast<float*>(base);
+  for (int i = tid; i < (live - z + S - 1) / S * CH; i += TT_THREADS) {
+    const int r = z + i / CH * S, c8 = i % CH * 8, row = row0 + r;
+    float M = -INFINITY, L = 0.f, v[8];
+    for (int k = 0; k < S; ++k) M = fmaxf(M, cl.map_shared_rank(&cml[0][0], k)[r]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (int k = 0; k < S; ++k) {
+      const float* ml = cl.map_shared_rank(&cml[0][0], k);
+      const float mk = ml[r];
+      if (mk == -INFINITY) continue;     // a CTA whose keys this row does not see
+      const float f = exp2f(mk - M);
+      L += f * ml[128 + r];
+      const float* po = cl.map_shared_rank(part0, k) + (size_t)r * LY::OLD + c8;
+      const float4 x = reinterpret_cast<const float4*>(po)[0], y = reinterpret_cast<const float4*>(po)[1];
+      v[0] += f * x.x, v[1] += f * x.y, v[2] += f * x.z, v[3] += f * x.w;
+      v[4] += f * y.x, v[5] += f * y.y, v[6] += f * y.z, v[7] += f * y.w;
+    }
+    const float inv = 1.f / L;
+    __nv_bfloat16* dst = a.out + ((size_t)b * N + row / rep) * a.out_ld + (size_t)(g * rep + row % rep) * HD + c8;
+    if (a.vec_out) {
+      *reinterpret_cast<uint4*>(dst) =
+          make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
+                     pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dst[e] = __float2bfloat16(v[e] * inv);
+    }
+  }
+  cl.sync();                             // no CTA leaves while another still reads its partial
+}
+
+template <int HD>
+int launch_tree_tc(const TreeArgs& a, int B, cudaStream_t st) {
+  using LY = TtLayout<HD>;
+  static DeviceOnce attr;
+  UTTT_TRY(run_once_per_device(attr, [] {
+    return cuda_status(
+        cudaFuncSetAttribute(attn_tree_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, LY::SMEM));
+  }));
+  // the rings as [slots * n_kv][W][hd]: places past W read as zeros
+  CUtensorMap tmK, tmV;
+  const uint64_t dims[3] = {(uint64_t)HD, (uint64_t)a.W, (uint64_t)a.n_slots * a.n_kv};
+  const uint64_t str[2] = {(uint64_t)HD * 2, (uint64_t)a.W * HD * 2};
+  const uint32_t box[3] = {64, TR_KT, 1};
+  UTTT_TRY(make_tmap_bf16(&tmK, a.kring, 3, dims, str, box));
+  UTTT_TRY(make_tmap_bf16(&tmV, a.vring, 3, dims, str, box));
+  const int blocks = (a.N * a.rep + 127) / 128;
+  UTTT_REQUIRE((long long)a.n_kv * blocks <= 65535, UTTT_ERR_UNSUPPORTED);
+  const long long ctas = (long long)B * a.n_kv * blocks;
+  const int tiles = (a.W + TR_KT - 1) / TR_KT + 1;
+  int S = 1;
+  while (S < 8 && ctas * S < 2LL * num_sms() && tiles / (2 * S) >= 2) S *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(S, a.n_kv * blocks, B);
+  cfg.blockDim = dim3(TT_THREADS);
+  cfg.dynamicSmemBytes = LY::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = S;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1] = pdl_attribute();
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, attn_tree_tc_kernel<HD>, tmK, tmV, a) != cudaSuccess) return launch_status();
+  return launch_status();
+}
+
 template <int HD>
 int launch_tree_rows(const TreeArgs& a, int B, cudaStream_t st) {
   const int rows = a.N * a.rep;
+  if constexpr (HD >= 64)
+    if (rows > 32) return launch_tree_tc<HD>(a, B, st);
   if (rows <= 16) return launch_tree<HD, 1>(a, B, st);
   if (rows <= 32) return launch_tree<HD, 2>(a, B, st);
   if (rows <= 64) return launch_tree<HD, 4>(a, B, st);
