@@ -92,55 +92,272 @@ struct TreeArgs {
   int vec_in, vec_out;                   // whether rows of qkv (with the tables) and of out start on 16 bytes
 };
 
+// bits lo .. lo + len - 1, as far as they lie in 0 .. 63
+__device__ __forceinline__ u64 bit_range(int lo, int len) {
+  const int a = max(lo, 0), b = min(lo + len, 64);
+  return b > a ? (~0ull >> (64 - (b - a))) << a : 0ull;
+}
+// Of the ring places j0 .. j0 + 63: those that a node `depth` deep does not see any more, the depth + 1 places
+// behind `next`, the oldest one (place j holds the position (j - next) mod W behind the oldest).
+__device__ __forceinline__ u64 hidden_places(int j0, int next, int W, int depth) {
+  return bit_range(next - j0, depth + 1) | bit_range(next - W - j0, depth + 1);
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // 8 elements of a row of qkv
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int vec) {
-  if (vec) return *reinterpret_cast<const uint4*>(p);
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p) {
+  if (VEC) return *reinterpret_cast<const uint4*>(p);
   const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
   return make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
                     h[6] | (uint32_t)h[7] << 16);
 }
-__device__ __forceinline__ void load8f(float (&f)[8], const float* p, int vec) {
-  if (vec) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+// 8 table values, rounded to BF16 as apply_rope does
+template <bool VEC>
+__device__ __forceinline__ void load_trig(uint32_t (&t)[4], const float* p) {
+  if (VEC) {
+    const float4 x = reinterpret_cast<const float4*>(p)[0], y = reinterpret_cast<const float4*>(p)[1];
+    t[0] = pack_bf16x2(x.x, x.y), t[1] = pack_bf16x2(x.z, x.w);
+    t[2] = pack_bf16x2(y.x, y.y), t[3] = pack_bf16x2(y.z, y.w);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = p[i];
+    for (int i = 0; i < 4; ++i) t[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
+  }
+}
+__device__ __forceinline__ __nv_bfloat162& as_bf162(uint32_t& v) { return reinterpret_cast<__nv_bfloat162&>(v); }
+
+// Table values of 8 elements of the first half of a head vector and of their partners in the second.
+struct Trig {
+  uint32_t cl[4], ch[4], sl[4], sh[4];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const float* cosr, const float* sinr, int i0, int half) {
+    load_trig<VEC>(cl, cosr + i0);
+    load_trig<VEC>(ch, cosr + i0 + half);
+    load_trig<VEC>(sl, sinr + i0);
+    load_trig<VEC>(sh, sinr + i0 + half);
+  }
+  // rotate-half RoPE, every product and the sum rounded to BF16 as apply_rope (model/uttt_layer.py:946-958): BF16
+  // arithmetic rounds each of them once (a product of two BF16 values is exact in FP32, and so is every sum that
+  // is near a rounding border)
+  __device__ __forceinline__ void rotate(uint4& lo, uint4& hi) {
+    uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
+    uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 xl = as_bf162(l[k]), xh = as_bf162(h[k]);
+      as_bf162(l[k]) = __hsub2_rn(__hmul2_rn(xl, as_bf162(cl[k])), __hmul2_rn(xh, as_bf162(sl[k])));
+      as_bf162(h[k]) = __hadd2_rn(__hmul2_rn(xh, as_bf162(ch[k])), __hmul2_rn(xl, as_bf162(sh[k])));
+    }
+  }
+};
+
+// RoPE of the CTA's query rows row0 .. row0 + n_rows - 1 and, with `tree`, of the nodes' keys, and the nodes' values.
+// A thread takes 8 elements and their partners of every head of one node, so the table values are read once and all
+// of a node's loads are in flight together.  put_q / put_k / put_v(r, c, v) take 16-byte chunk c of row or node r;
+// `keep` marks the CTA that writes k_tree and v_tree.  Non-finite values are left out of put_v and their nodes
+// marked in *bad: 0 * NaN would let a key's value reach rows that do not see it; they are added at the end to the
+// rows that do.
+template <int HD, bool VEC, class Depth, class PutQ, class PutK, class PutV>
+__device__ __forceinline__ void rope_nodes_as(int tid, int threads, int n, int b, int g, int p0, int row0, int n_rows,
+                                              bool tree, const TreeArgs& a, u64* bad, Depth depth, PutQ put_q,
+                                              PutK put_k, PutV put_v) {
+  constexpr int HC = HD / 16, CH = HD / 8;
+  const __nv_bfloat16* rows = a.qkv + (size_t)b * a.N * a.qkv_ld;
+  const int rep = a.rep, nodes = tree ? n : min(n, (row0 + n_rows + rep - 1) / rep);
+  const int first = tree ? 0 : row0 / rep;
+  const bool keep = tree && row0 == 0;
+  for (int i = tid; i < (nodes - first) * HC; i += threads) {
+    const int node = first + i / HC, c = i % HC;
+    const __nv_bfloat16* x = rows + (size_t)node * a.qkv_ld + c * 8;
+    const __nv_bfloat16* xq = x + (size_t)g * rep * HD;
+    const __nv_bfloat16* xk = x + (size_t)(a.n_kv * rep + g) * HD;
+    const __nv_bfloat16* xv = xk + (size_t)a.n_kv * HD;
+    const size_t tr = (size_t)min((long long)p0 + depth(node), (long long)a.n_pos - 1) * HD;
+    const int r0 = node * rep - row0;
+    uint4 k0, k1, v0, v1;
+    if (tree) {
+      k0 = load8<VEC>(xk);
+      k1 = load8<VEC>(xk + HD / 2);
+      v0 = load8<VEC>(xv);
+      v1 = load8<VEC>(xv + HD / 2);
+    }
+    Trig t;
+#pragma unroll
+    for (int h0 = 0; h0 < TR_MAX_REP; h0 += 4) {
+      if (h0 >= rep) break;
+      uint4 lo[4], hi[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int r = r0 + h0 + h;
+        if (h0 + h < rep && r >= 0 && r < n_rows) {
+          lo[h] = load8<VEC>(xq + (size_t)(h0 + h) * HD);
+          hi[h] = load8<VEC>(xq + (size_t)(h0 + h) * HD + HD / 2);
+        }
+      }
+      if (h0 == 0) t.template load<VEC>(a.cos_t + tr, a.sin_t + tr, c * 8, HD / 2);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int r = r0 + h0 + h;
+        if (h0 + h < rep && r >= 0 && r < n_rows) {
+          t.rotate(lo[h], hi[h]);
+          put_q(r, c, lo[h]);
+          put_q(r, c + HC, hi[h]);
+        }
+      }
+    }
+    if (tree) {
+      t.rotate(k0, k1);
+      put_k(node, c, k0);
+      put_k(node, c + HC, k1);
+      if (keep) {
+        const size_t o = (((size_t)b * a.n_kv + g) * a.N + node) * HD + c * 8;
+        *reinterpret_cast<uint4*>(a.ktree + o) = k0;
+        *reinterpret_cast<uint4*>(a.ktree + o + HD / 2) = k1;
+        *reinterpret_cast<uint4*>(a.vtree + o) = v0;
+        *reinterpret_cast<uint4*>(a.vtree + o + HD / 2) = v1;
+      }
+      if (has_nonfinite(v0.x) || has_nonfinite(v0.y) || has_nonfinite(v0.z) || has_nonfinite(v0.w) ||
+          has_nonfinite(v1.x) || has_nonfinite(v1.y) || has_nonfinite(v1.z) || has_nonfinite(v1.w)) {
+        v0 = make_uint4(finite_only(v0.x), finite_only(v0.y), finite_only(v0.z), finite_only(v0.w));
+        v1 = make_uint4(finite_only(v1.x), finite_only(v1.y), finite_only(v1.z), finite_only(v1.w));
+        atomicOr(bad, 1ull << node);
+      }
+      put_v(node, c, v0);
+      put_v(node, c + HC, v1);
+    }
+  }
+  // zeros behind the last query row and the last node
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  for (int i = tid + max(0, min(n_rows, n * rep - row0)) * CH; i < n_rows * CH; i += threads) put_q(i / CH, i % CH, zero);
+  if (tree)
+    for (int i = tid + n * CH; i < TR_KT * CH; i += threads) {
+      put_k(i / CH, i % CH, zero);
+      put_v(i / CH, i % CH, zero);
+    }
+}
+template <int HD, class... F>
+__device__ __forceinline__ void rope_nodes(int tid, int threads, int n, int b, int g, int p0, int row0, int n_rows,
+                                           bool tree, const TreeArgs& a, u64* bad, F... f) {
+  if (a.vec_in)
+    rope_nodes_as<HD, true>(tid, threads, n, b, g, p0, row0, n_rows, tree, a, bad, f...);
+  else
+    rope_nodes_as<HD, false>(tid, threads, n, b, g, p0, row0, n_rows, tree, a, bad, f...);
+}
+
+// The same for the values of the keys `keys` of a ring tile in shared memory, at(r, c) being chunk c of key r.
+template <int HD, class At>
+__device__ __forceinline__ void finite_values(int tid, int threads, u64 keys, u64* bad, At at) {
+  constexpr int CH = HD / 8;
+  if (!keys) return;
+  const int r0 = __ffsll((long long)keys) - 1, r1 = 63 - __clzll((long long)keys);
+  for (int i = tid; i < (r1 - r0 + 1) * CH; i += threads) {
+    const int r = r0 + i / CH;
+    if (!((keys >> r) & 1ull)) continue;
+    uint4* p = at(r, i % CH);
+    const uint4 v = *p;
+    if (has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w)) {
+      *p = make_uint4(finite_only(v.x), finite_only(v.y), finite_only(v.z), finite_only(v.w));
+      atomicOr(bad, 1ull << r);
+    }
   }
 }
 
-// rotate-half RoPE of elements i0 .. i0 + 7 (`lo`) and their partners i0 + hd / 2 .. (`hi`) of a head vector,
-// rounded to BF16 as apply_rope (model/uttt_layer.py:946-958)
-__device__ __forceinline__ void rope8(uint4& lo, uint4& hi, const float* cosr, const float* sinr, int i0, int half,
-                                      int vec) {
-  uint32_t* l = reinterpret_cast<uint32_t*>(&lo);
-  uint32_t* h = reinterpret_cast<uint32_t*>(&hi);
-  float cl[8], ch[8], sl[8], sh[8];
-  load8f(cl, cosr + i0, vec);
-  load8f(ch, cosr + i0 + half, vec);
-  load8f(sl, sinr + i0, vec);
-  load8f(sh, sinr + i0 + half, vec);
+// What a CTA reads of qkv and of the tables, on its way to L2 while the nodes' paths are worked out.
+template <int HD>
+__device__ __forceinline__ void prefetch_nodes(int tid, int threads, int n, int b, int g, int p0, const TreeArgs& a) {
+  const char* q = reinterpret_cast<const char*>(a.qkv + (size_t)b * a.N * a.qkv_ld);
+  const int qb = a.rep * HD * 2, per = (qb + 127) / 128 + 2 * ((HD * 2 + 127) / 128);   // 128-byte lines per node
+  for (int i = tid; i < n * per; i += threads) {
+    const int r = i / per, k = i % per, kl = (HD * 2 + 127) / 128, ql = per - 2 * kl;
+    const int off = k < ql ? g * qb + k * 128
+                           : (a.n_kv * a.rep + g + (k >= ql + kl ? a.n_kv : 0)) * HD * 2 + (k - ql) % kl * 128;
+    prefetch_l2(q + (size_t)r * a.qkv_ld * 2 + off);
+  }
+  // positions p0 .. are the depths'; few trees are deeper than 16
+  const int rows = min(min(n, 16), a.n_pos - min(p0, a.n_pos));
+  for (int i = tid; i < rows * (HD * 4 / 128) * 2; i += threads) {
+    const float* t = (i & 1) ? a.sin_t : a.cos_t;
+    prefetch_l2(reinterpret_cast<const char*>(t + (size_t)p0 * HD) + (i >> 1) * 128);
+  }
+}
+
+// The partials of a row, joined by CTA r % S of the cluster: every CTA sends its maximum, sum and unnormalised output
+// there (remote stores, nobody waits for them one by one), at [sender][r / S].
+struct Joiner {
+  float* o;                              // [S][rows / S][old]
+  float (*ml)[2];                        // [S][rows / S]
+  int S, per, old;                       // per: rows per CTA
+  __device__ __forceinline__ void send_ml(cg::cluster_group& cl, int z, int r, float m, float l) const {
+    float* p = cl.map_shared_rank(&ml[z * per + r / S][0], r % S);
+    p[0] = m;
+    p[1] = l;
+  }
+  __device__ __forceinline__ float4* row(cg::cluster_group& cl, int z, int r) const {
+    return reinterpret_cast<float4*>(cl.map_shared_rank(o + (size_t)(z * per + r / S) * old, r % S));
+  }
+  // columns c8 .. c8 + 7 of this CTA's row number q (row q * S + rank); returns the sum
+  __device__ __forceinline__ float join(int q, int c8, float (&v)[8]) const {
+    float M = -INFINITY, L = 0.f;
+    for (int k = 0; k < S; ++k) M = fmaxf(M, ml[k * per + q][0]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float yl[2], yh[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float xl = e ? bf16_hi(l[k]) : bf16_lo(l[k]), xh = e ? bf16_hi(h[k]) : bf16_lo(h[k]);
-      yl[e] = bfr(xl * bfr(cl[2 * k + e])) + bfr(-xh * bfr(sl[2 * k + e]));
-      yh[e] = bfr(xh * bfr(ch[2 * k + e])) + bfr(xl * bfr(sh[2 * k + e]));
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    for (int k = 0; k < S; ++k) {
+      const float mk = ml[k * per + q][0];
+      if (mk == -INFINITY) continue;     // a CTA whose keys this row does not see
+      const float f = exp2f(mk - M);
+      L += f * ml[k * per + q][1];
+      const float4* p = reinterpret_cast<const float4*>(o + (size_t)(k * per + q) * old + c8);
+      const float4 x = p[0], y = p[1];
+      v[0] += f * x.x, v[1] += f * x.y, v[2] += f * x.z, v[3] += f * x.w;
+      v[4] += f * y.x, v[5] += f * y.y, v[6] += f * y.z, v[7] += f * y.w;
     }
-    l[k] = pack_bf16x2(yl[0], yl[1]);
-    h[k] = pack_bf16x2(yh[0], yh[1]);
+    return L;
+  }
+};
+
+// 8 columns of a row of out
+__device__ __forceinline__ void store_out(const TreeArgs& a, int b, int g, int row, int c8, int hd, const float (&v)[8],
+                                          float inv) {
+  const int node = row / a.rep, h = g * a.rep + row % a.rep;
+  __nv_bfloat16* dst = a.out + ((size_t)b * a.N + node) * a.out_ld + (size_t)h * hd + c8;
+  if (a.vec_out) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
+                                                pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dst[e] = __float2bfloat16(v[e] * inv);
   }
 }
 
 template <int HD, int WM>
 __host__ __device__ constexpr int tree_threads() { return 32 * (WM < 4 ? 4 : WM); }
-template <int HD>
-constexpr int tree_smem() { return TR_NS * 2 * TR_KT * HD * 2; }
+// the tiles; at the end the warps' partials and, behind them, the rows that the cluster sends
+template <int HD, int WM>
+constexpr int tree_smem() {
+  constexpr int tiles = TR_NS * 2 * TR_KT * HD * 2, ends = (tree_threads<HD, WM>() / 32 + WM) * 16 * (HD + 4) * 4;
+  return tiles > ends ? tiles : ends;
+}
+
+// CTAs that share a row's keys.  A CTA takes about as long as `head` tiles before and after its own tiles (node
+// paths, RoPE, output), a cluster `join` more; S minimises the waves of CTAs times that.
+inline int tree_split(long long ctas, int tiles, int per_sm, int head, int join) {
+  const long long slots = (long long)num_sms() * per_sm;
+  int best = 1;
+  long long least = 0;
+  for (int S = 1; S <= 8 && (S == 1 || tiles >= 2 * S); S *= 2) {
+    const long long waves = (ctas * S + slots - 1) / slots;
+    const long long cost = waves * (head + (tiles + S - 1) / S + (S > 1 ? join : 0));
+    if (S == 1 || cost < least) {
+      best = S;
+      least = cost;
+    }
+  }
+  return best;
+}
 
 // grid (S, n_kv * row blocks, B), cluster (S, 1, 1): CTA z takes tiles [nt * z / S, nt * (z + 1) / S) of the nt
-// 64-key tiles (the ring's, then the tree's).
+// 64-key tiles: tile 0 holds the drafted keys, tile t > 0 the ring's places 64 (t - 1) ..
 template <int HD, int WM>
 __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const TreeArgs a) {
   constexpr int THREADS = tree_threads<HD, WM>(), NW = THREADS / 32, WK = NW / WM;
@@ -150,9 +367,9 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
   constexpr int CH = HD / 8, TILE = TR_KT * HD * 2;
   constexpr int OLD = HD + 4;            // row stride of the partial outputs (floats): rows shift by 4 banks
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ u64 anc_s[2][TR_KT], bad_keys;
-  __shared__ int jump_s[2][TR_KT], depth_s[TR_KT];
-  __shared__ float m_s[NW][16], l_s[NW][16], fac_s[WK][RB], cml[2][RB];
+  __shared__ u64 anc_s[2][TR_KT], bad_keys, bad_tree;
+  __shared__ int jump_s[2][TR_KT], depth_s[TR_KT], deepest;
+  __shared__ float m_s[NW][16], l_s[NW][16], fac_s[WK][RB], cml[2][RB], ml_s[RB][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wm = warp % WM, wk = warp / WM;
   const int S = gridDim.x, z = blockIdx.x, b = blockIdx.z;
   const int g = blockIdx.y % a.n_kv, row0 = blockIdx.y / a.n_kv * RB;
@@ -166,59 +383,34 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
   if (row0 >= rows || sl < 0 || sl >= a.n_slots || p0 < 0) return;   // the same in the whole cluster
 
   // ---- ring tiles on their way first
-  const int nvalid = min(p0, W), nring = (nvalid + TR_KT - 1) / TR_KT, nt = nring + 1;
+  const int nvalid = min(p0, W), nt = (nvalid + TR_KT - 1) / TR_KT + 1;
   const int t_lo = (int)((long long)nt * z / S), t_hi = (int)((long long)nt * (z + 1) / S);
+  const bool has_tree = t_lo == 0 && t_hi > 0;
   const size_t ring0 = ((size_t)sl * a.n_kv + g) * (size_t)W * HD;
   const __nv_bfloat16* qrows = a.qkv + (size_t)b * N * a.qkv_ld;
-  const int k_col = (a.n_kv * rep + g) * HD, v_col = k_col + a.n_kv * HD;
-  auto table_row = [&](int node) {
-    return (size_t)min((long long)p0 + depth_s[node], (long long)a.n_pos - 1) * HD;
-  };
+  const int v_col = (a.n_kv * (rep + 1) + g) * HD;
   auto load_ring = [&](int t) {
     uint8_t* ks = smem + ((t - t_lo) % TR_NS) * 2 * TILE;
     for (int i = tid; i < TR_KT * CH; i += THREADS) {
-      const int r = i / CH, c = i % CH, j = t * TR_KT + r;
+      const int r = i / CH, c = i % CH, j = (t - 1) * TR_KT + r;
       const bool ok = j < nvalid;
       const size_t o = ring0 + (size_t)(ok ? j : 0) * HD + c * 8;
       cp_async_16(ks + tile_off<HD>(r, c), a.kring + o, ok);
       cp_async_16(ks + TILE + tile_off<HD>(r, c), a.vring + o, ok);
     }
   };
-  // the nodes' keys (RoPE'd) and values as the last tile; one CTA per (row, KV head) also writes them out
-  auto load_tree = [&]() {
-    uint8_t* ks = smem + ((nt - 1 - t_lo) % TR_NS) * 2 * TILE;
-    for (int i = tid; i < TR_KT * CH / 2; i += THREADS) {
-      const int r = i / (CH / 2), c = i % (CH / 2);
-      uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0, v0 = k0, v1 = k0;
-      if (r < n) {
-        const __nv_bfloat16* x = qrows + (size_t)r * a.qkv_ld;
-        k0 = load8(x + k_col + c * 8, a.vec_in);
-        k1 = load8(x + k_col + HD / 2 + c * 8, a.vec_in);
-        v0 = load8(x + v_col + c * 8, a.vec_in);
-        v1 = load8(x + v_col + HD / 2 + c * 8, a.vec_in);
-        const size_t tr = table_row(r);
-        rope8(k0, k1, a.cos_t + tr, a.sin_t + tr, c * 8, HD / 2, a.vec_in);
-        if (row0 == 0) {
-          const size_t o = (((size_t)b * a.n_kv + g) * N + r) * HD + c * 8;
-          *reinterpret_cast<uint4*>(a.ktree + o) = k0;
-          *reinterpret_cast<uint4*>(a.ktree + o + HD / 2) = k1;
-          *reinterpret_cast<uint4*>(a.vtree + o) = v0;
-          *reinterpret_cast<uint4*>(a.vtree + o + HD / 2) = v1;
-        }
-      }
-      *reinterpret_cast<uint4*>(ks + tile_off<HD>(r, c)) = k0;
-      *reinterpret_cast<uint4*>(ks + tile_off<HD>(r, c + CH / 2)) = k1;
-      *reinterpret_cast<uint4*>(ks + TILE + tile_off<HD>(r, c)) = v0;
-      *reinterpret_cast<uint4*>(ks + TILE + tile_off<HD>(r, c + CH / 2)) = v1;
-    }
-  };
 #pragma unroll
   for (int i = 0; i < TR_NS - 1; ++i) {
-    if (t_lo + i < t_hi && t_lo + i < nring) load_ring(t_lo + i);
+    if (t_lo + i < t_hi && t_lo + i > 0) load_ring(t_lo + i);
     cp_async_commit();
   }
+  prefetch_nodes<HD>(tid, THREADS, n, b, g, p0, a);
 
   // ---- every node's path as a bit mask, by pointer jumping (6 doublings reach 64 ancestors)
+  if (tid == 0) {
+    bad_tree = 0ull;
+    deepest = 0;
+  }
   if (tid < TR_KT) {
     anc_s[0][tid] = 1ull << tid;
     jump_s[0][tid] = tid < n && par_i >= 0 && par_i < tid ? par_i : -1;   // anything else makes a root
@@ -237,6 +429,7 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
     u64 m = anc_s[0][tid];
     const int d = __popcll(m) - 1;
     depth_s[tid] = d;
+    if (tid < n && d > 0) atomicMax(&deepest, d);
     if (d >= W)                          // ancestors that have left the window
       for (u64 rest = m; rest; rest &= rest - 1) {
         const int j = __ffsll((long long)rest) - 1;
@@ -246,25 +439,13 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
   }
   __syncthreads();
 
-  // ---- tiles of the tree that the prologue must fill, and Q: RoPE'd rows into the last stage, then registers
-#pragma unroll
-  for (int i = 0; i < TR_NS - 1; ++i)
-    if (t_lo + i < t_hi && t_lo + i == nt - 1) load_tree();
+  // ---- RoPE: Q into the last stage (then registers); the drafted keys and values are the first tile
   uint8_t* sQ = smem + (TR_NS - 1) * 2 * TILE;
-  for (int i = tid; i < RB * CH / 2; i += THREADS) {
-    const int r = i / (CH / 2), c = i % (CH / 2), row = row0 + r;
-    uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
-    if (row < rows) {
-      const int node = row / rep, h = g * rep + row % rep;
-      const __nv_bfloat16* x = qrows + (size_t)node * a.qkv_ld + (size_t)h * HD;
-      q0 = load8(x + c * 8, a.vec_in);
-      q1 = load8(x + HD / 2 + c * 8, a.vec_in);
-      const size_t tr = table_row(node);
-      rope8(q0, q1, a.cos_t + tr, a.sin_t + tr, c * 8, HD / 2, a.vec_in);
-    }
-    *reinterpret_cast<uint4*>(sQ + tile_off<HD>(r, c)) = q0;
-    *reinterpret_cast<uint4*>(sQ + tile_off<HD>(r, c + CH / 2)) = q1;
-  }
+  rope_nodes<HD>(
+      tid, THREADS, n, b, g, p0, row0, RB, has_tree, a, &bad_tree, [&](int node) { return depth_s[node]; },
+      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(sQ + tile_off<HD>(r, c)) = v; },
+      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(smem + tile_off<HD>(r, c)) = v; },
+      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(smem + TILE + tile_off<HD>(r, c)) = v; });
   __syncthreads();
   uint32_t qf[HD / 16][4];
 #pragma unroll
@@ -281,7 +462,7 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
     dep[e] = ok ? depth_s[row / rep] : -1;
     anc[e] = ok ? anc_s[1][row / rep] : ~0ull;
   }
-  const int next = p0 % W;               // the oldest place: place j holds position p0 - W + (j - next mod W)
+  const int next = p0 % W, max_dep = deepest;   // next: the oldest place
   float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < HD / 8; ++i)
@@ -291,44 +472,36 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
   for (int t = t_lo; t < t_hi; ++t) {
     cp_async_wait<TR_NS - 2>();
     __syncthreads();
-    if (t + TR_NS - 1 < t_hi) {
-      if (t + TR_NS - 1 < nring)
-        load_ring(t + TR_NS - 1);
-      else
-        load_tree();
-    }
+    if (t + TR_NS - 1 < t_hi) load_ring(t + TR_NS - 1);
     cp_async_commit();
     uint8_t* ks = smem + ((t - t_lo) % TR_NS) * 2 * TILE;
     const uint32_t ka = smem_u32(ks), va = ka + TILE;
-    const bool is_tree = t == nt - 1;
-    // a tile whose keys not every row sees: the tree's, the ring's last, and where the window's edge lies
-    // (places 0 .. 63 behind `next`, the most that a depth can hide)
-    const int rel = (t * TR_KT - next + W) % W;
-    const bool edge = is_tree || t * TR_KT + TR_KT > nvalid || rel < TR_KT || rel + TR_KT > W;
-    u64 bad = 0ull;
+    const bool is_tree = t == 0;
+    // keys that not every row sees: the tree's, the ring's behind the last valid place and around the window's edge
+    const int j0 = (t - 1) * TR_KT;
+    const u64 some = is_tree ? ~0ull : hidden_places(j0, next, W, max_dep);
+    const bool edge = is_tree || j0 + TR_KT > nvalid || some != 0ull;
+    u64 bad = 0ull, seen[2] = {~0ull, ~0ull};
     if (edge) {
-      // 0 * NaN would let a key's value reach rows that do not see it: such values leave the product and are
-      // added, below, to the rows that do
-      if (tid == 0) bad_keys = 0ull;
-      __syncthreads();
-      for (int i = tid; i < TR_KT * CH; i += THREADS) {
-        uint4* p = reinterpret_cast<uint4*>(ks + TILE + tile_off<HD>(i / CH, i % CH));
-        uint4 v = *p;
-        if (has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w)) {
-          *p = make_uint4(finite_only(v.x), finite_only(v.y), finite_only(v.z), finite_only(v.w));
-          atomicOr(&bad_keys, 1ull << (i / CH));
+      if (is_tree) {
+        bad = bad_tree;
+        seen[0] = anc[0];
+        seen[1] = anc[1];
+      } else {
+        const u64 valid = bit_range(0, nvalid - j0);
+        if (some & valid) {
+          if (tid == 0) bad_keys = 0ull;
+          __syncthreads();
+          finite_values<HD>(tid, THREADS, some & valid, &bad_keys, [&](int r, int c) {
+            return reinterpret_cast<uint4*>(ks + TILE + tile_off<HD>(r, c));
+          });
+          __syncthreads();
+          bad = bad_keys;
         }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) seen[e] = valid & ~hidden_places(j0, next, W, dep[e]);
       }
-      __syncthreads();
-      bad = bad_keys;
     }
-    auto sees = [&](int e, int key) -> bool {   // whether row e of this thread sees key `key` of the tile
-      if (is_tree) return (anc[e] >> key) & 1ull;
-      const int j = t * TR_KT + key;
-      int back = j - next;               // 0 for the oldest place
-      if (back < 0) back += W;
-      return j < nvalid && back > dep[e];
-    };
 #pragma unroll
     for (int sub = 0; sub < KW / SUB; ++sub) {
       const int kb = wk * KW + sub * SUB;
@@ -346,13 +519,21 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
           mma16816(s[2 * i], qf[k], kf[0], kf[1]);
           mma16816(s[2 * i + 1], qf[k], kf[2], kf[3]);
         }
+      if (edge) {
+        // bits of this thread's columns: i * 8 and i * 8 + 1 after the shift
+        const uint32_t v0 = (uint32_t)(seen[0] >> (kb + (lane & 3) * 2)), v1 = (uint32_t)(seen[1] >> (kb + (lane & 3) * 2));
+#pragma unroll
+        for (int i = 0; i < SUB / 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(((e >> 1) ? v1 : v0) >> (i * 8 + (e & 1)) & 1u)) s[i][e] = -INFINITY;
+      }
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int i = 0; i < SUB / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[i][e] *= a.scale_log2;
-          if (edge && !sees(e >> 1, kb + i * 8 + (lane & 3) * 2 + (e & 1))) s[i][e] = -INFINITY;
           mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e]);
         }
       float c[2];
@@ -405,13 +586,13 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
       const int key = __ffsll((long long)rest) - 1;
       if (key / KW != wk) continue;
       const __nv_bfloat16* v = is_tree ? qrows + (size_t)key * a.qkv_ld + v_col
-                                       : a.vring + ring0 + (size_t)(t * TR_KT + key) * HD;
+                                       : a.vring + ring0 + (size_t)(j0 + key) * HD;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = __bfloat162float(v[i * 8 + (lane & 3) * 2 + (e & 1)]);
-          if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u && sees(e >> 1, key)) o[i][e] += x;
+          if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u && (seen[e >> 1] >> key & 1ull)) o[i][e] += x;
         }
     }
   }
@@ -470,59 +651,34 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
       v[4] += f * y.x, v[5] += f * y.y, v[6] += f * y.z, v[7] += f * y.w;
     }
   };
-  auto store = [&](int r, int c8, const float (&v)[8], float inv) {
-    const int row = row0 + r, node = row / rep, h = g * rep + row % rep;
-    __nv_bfloat16* dst = a.out + ((size_t)b * N + node) * a.out_ld + (size_t)h * HD + c8;
-    if (a.vec_out) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
-                                                  pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dst[e] = __float2bfloat16(v[e] * inv);
-    }
-  };
   const int live = min(RB, rows - row0);
   if (S == 1) {
     for (int i = tid; i < live * CH; i += THREADS) {
       float v[8];
       joined(i / CH, i % CH * 8, v);
-      store(i / CH, i % CH * 8, v, 1.f / cml[1][i / CH]);
+      store_out(a, b, g, row0 + i / CH, i % CH * 8, HD, v, 1.f / cml[1][i / CH]);
     }
     return;
   }
-  // the CTA's own join in place (its first warp's copy), then each CTA finishes every S-th row
-  if (WK > 1) {
-    for (int i = tid; i < live * CH; i += THREADS) {
-      float v[8];
-      const int r = i / CH, c8 = i % CH * 8;
-      joined(r, c8, v);
-      float* po = part + ((size_t)(r >> 4) * 16 + (r & 15)) * OLD + c8;   // only this thread reads or writes it
-      reinterpret_cast<float4*>(po)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(po)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-  }
+  // behind the warps' partials, which other CTAs leave alone; their tiles have been read once all are here
+  const Joiner jn{part + NW * 16 * OLD, ml_s, S, RB / S, OLD};
   cg::cluster_group cl = cg::this_cluster();
   cl.sync();
-  for (int i = tid; i < (live - z + S - 1) / S * CH; i += THREADS) {
-    const int r = z + i / CH * S, c8 = i % CH * 8;
-    float M = -INFINITY, L = 0.f, v[8];
-    for (int k = 0; k < S; ++k) M = fmaxf(M, cl.map_shared_rank(&cml[0][0], k)[r]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    for (int k = 0; k < S; ++k) {
-      const float* ml = cl.map_shared_rank(&cml[0][0], k);
-      const float mk = ml[r];
-      if (mk == -INFINITY) continue;     // a CTA whose keys this row does not see
-      const float f = exp2f(mk - M);
-      L += f * ml[RB + r];
-      const float* po = cl.map_shared_rank(part, k) + ((size_t)(r >> 4) * 16 + (r & 15)) * OLD + c8;
-      const float4 x = reinterpret_cast<const float4*>(po)[0], y = reinterpret_cast<const float4*>(po)[1];
-      v[0] += f * x.x, v[1] += f * x.y, v[2] += f * x.z, v[3] += f * x.w;
-      v[4] += f * y.x, v[5] += f * y.y, v[6] += f * y.z, v[7] += f * y.w;
-    }
-    store(r, c8, v, 1.f / L);
+  for (int i = tid; i < live * CH; i += THREADS) {
+    float v[8];
+    const int r = i / CH, c = i % CH;
+    joined(r, c * 8, v);
+    float4* p = jn.row(cl, z, r) + c * 2;
+    p[0] = make_float4(v[0], v[1], v[2], v[3]);
+    p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    if (c == 0) jn.send_ml(cl, z, r, cml[0][r], cml[1][r]);
   }
-  cl.sync();                             // no CTA leaves while another still reads its partial
+  cl.sync();                             // nothing remote after this
+  for (int i = tid; i < (live - z + S - 1) / S * CH; i += THREADS) {
+    float v[8];
+    const float L = jn.join(i / CH, i % CH * 8, v);
+    store_out(a, b, g, row0 + z + i / CH * S, i % CH * 8, HD, v, 1.f / L);
+  }
 }
 
 template <int HD, int WM>
@@ -530,19 +686,15 @@ int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
   static DeviceOnce attr;
   UTTT_TRY(run_once_per_device(attr, [] {
     return cuda_status(cudaFuncSetAttribute(attn_tree_kernel<HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            tree_smem<HD>()));
+                                            tree_smem<HD, WM>()));
   }));
   const int blocks = (a.N * a.rep + 16 * WM - 1) / (16 * WM);
   UTTT_REQUIRE((long long)a.n_kv * blocks <= 65535, UTTT_ERR_UNSUPPORTED);
-  // split the keys over a cluster while the batch leaves SMs idle (at least two tiles per CTA)
-  const long long ctas = (long long)B * a.n_kv * blocks;
-  const int tiles = (a.W + TR_KT - 1) / TR_KT + 1;
-  int S = 1;
-  while (S < 8 && ctas * S < 2LL * num_sms() && tiles / (2 * S) >= 2) S *= 2;
+  const int S = tree_split((long long)B * a.n_kv * blocks, (a.W + TR_KT - 1) / TR_KT + 1, WM == 8 ? 1 : 2, 4, 1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(S, a.n_kv * blocks, B);
   cfg.blockDim = dim3(tree_threads<HD, WM>());
-  cfg.dynamicSmemBytes = tree_smem<HD>();
+  cfg.dynamicSmemBytes = tree_smem<HD, WM>();
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -614,10 +766,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], ready;
   __shared__ uint32_t tmem_slot;
-  __shared__ u64 anc_s[2][TR_KT], bad_keys;
-  __shared__ int jump_s[2][TR_KT], depth_s[TR_KT];
-  __shared__ float cml[2][128];
-  __shared__ u64 bad_mask[8];            // tiles with non-finite values: their keys ...
+  __shared__ u64 anc_s[2][TR_KT], bad_keys, bad_tree;
+  __shared__ int jump_s[2][TR_KT], depth_s[TR_KT], deepest;
+  __shared__ float ml_s[128][2];         // of the rows that the cluster sends
+  __shared__ u64 bad_mask[8];            // ring tiles with non-finite values: their keys ...
   __shared__ int bad_tile[8], n_bad;     // ... and numbers
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sQ = base, *sK = base + LY::K0, *sV = base + LY::V0;
@@ -627,6 +779,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   const int N = a.N, rep = a.rep, W = a.W;
   pdl_wait();
   pdl_trigger();
+  const int ti = tid - 64;               // warps 2-5: 0 .. 127
+  const int par_i = ti >= 0 && ti < N ? a.parents[(size_t)b * N + ti] : -1;
   const int n = a.n_nodes ? min(a.n_nodes[b], N) : N;
   const int p0 = a.pos[b], sl = a.slot[b];
   const int rows = n * rep;
@@ -650,7 +804,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
     mbar_init(&ready, 128);
     fence_mbarrier_init();
     n_bad = 0;
+    bad_tree = 0ull;
+    deepest = 0;
   }
+  if (ti >= 0) prefetch_nodes<HD>(ti, 128, n, b, g, p0, a);
   if (warp == 1) tmem_alloc(&tmem_slot, 256);
   tc_fence_before();
   __syncthreads();
@@ -713,9 +870,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       }
     }
   } else {
-    const int ti = tid - 64;             // 0 .. 127
     // ---- every node's path, as in attn_tree_kernel
-    const int par_i = ti < N ? a.parents[(size_t)b * N + ti] : -1;
     if (ti < TR_KT) {
       anc_s[0][ti] = 1ull << ti;
       jump_s[0][ti] = ti < n && par_i >= 0 && par_i < ti ? par_i : -1;
@@ -734,6 +889,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       u64 m = anc_s[0][ti];
       const int d = __popcll(m) - 1;
       depth_s[ti] = d;
+      if (ti < n && d > 0) atomicMax(&deepest, d);
       if (d >= W)
         for (u64 rest = m; rest; rest &= rest - 1) {
           const int j = __ffsll((long long)rest) - 1;
@@ -742,56 +898,18 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       anc_s[1][ti] = m;
     }
     named_bar(1, 128);
-    // ---- Q, and the drafted keys and values
+    // ---- Q, and the drafted keys and values (the rows behind the last warp of rows are never looked at)
     const __nv_bfloat16* qrows = a.qkv + (size_t)b * N * a.qkv_ld;
-    const int k_col = (a.n_kv * rep + g) * HD, v_col = k_col + a.n_kv * HD;
+    const int v_col = (a.n_kv * (rep + 1) + g) * HD;
     const size_t ring0 = ((size_t)sl * a.n_kv + g) * (size_t)W * HD;
-    auto table_row = [&](int node) {
-      return (size_t)min((long long)p0 + depth_s[node], (long long)a.n_pos - 1) * HD;
-    };
     auto put = [&](uint8_t* t, int blk, int r, int c, uint4 v) {
       *reinterpret_cast<uint4*>(t + (c >> 3) * blk + sw128_offset(r, (c & 7) * 16)) = v;
     };
-    for (int i = ti; i < 128 * CH / 2; i += 128) {
-      const int r = i / (CH / 2), c = i % (CH / 2), row = row0 + r;
-      uint4 q0 = make_uint4(0, 0, 0, 0), q1 = q0;
-      if (row < rows) {
-        const int node = row / rep;
-        const __nv_bfloat16* x = qrows + (size_t)node * a.qkv_ld + (size_t)(g * rep + row % rep) * HD;
-        q0 = load8(x + c * 8, a.vec_in);
-        q1 = load8(x + HD / 2 + c * 8, a.vec_in);
-        const size_t tr = table_row(node);
-        rope8(q0, q1, a.cos_t + tr, a.sin_t + tr, c * 8, HD / 2, a.vec_in);
-      }
-      put(sQ, 16384, r, c, q0);
-      put(sQ, 16384, r, c + CH / 2, q1);
-    }
-    if (has_tree) {
-      for (int i = ti; i < TR_KT * CH / 2; i += 128) {
-        const int r = i / (CH / 2), c = i % (CH / 2);
-        uint4 k0 = make_uint4(0, 0, 0, 0), k1 = k0, v0 = k0, v1 = k0;
-        if (r < n) {
-          const __nv_bfloat16* x = qrows + (size_t)r * a.qkv_ld;
-          k0 = load8(x + k_col + c * 8, a.vec_in);
-          k1 = load8(x + k_col + HD / 2 + c * 8, a.vec_in);
-          v0 = load8(x + v_col + c * 8, a.vec_in);
-          v1 = load8(x + v_col + HD / 2 + c * 8, a.vec_in);
-          const size_t tr = table_row(r);
-          rope8(k0, k1, a.cos_t + tr, a.sin_t + tr, c * 8, HD / 2, a.vec_in);
-          if (row0 == 0) {
-            const size_t o = (((size_t)b * a.n_kv + g) * N + r) * HD + c * 8;
-            *reinterpret_cast<uint4*>(a.ktree + o) = k0;
-            *reinterpret_cast<uint4*>(a.ktree + o + HD / 2) = k1;
-            *reinterpret_cast<uint4*>(a.vtree + o) = v0;
-            *reinterpret_cast<uint4*>(a.vtree + o + HD / 2) = v1;
-          }
-        }
-        put(sK, 8192, r, c, k0);
-        put(sK, 8192, r, c + CH / 2, k1);
-        put(sV, 8192, r, c, v0);
-        put(sV, 8192, r, c + CH / 2, v1);
-      }
-    }
+    rope_nodes<HD>(
+        ti, 128, n, b, g, p0, row0, act, has_tree, a, &bad_tree, [&](int node) { return depth_s[node]; },
+        [&](int r, int c, uint4 v) { put(sQ, 16384, r, c, v); },
+        [&](int r, int c, uint4 v) { put(sK, 8192, r, c, v); },
+        [&](int r, int c, uint4 v) { put(sV, 8192, r, c, v); });
     fence_proxy_async_smem();
     mbar_arrive(&ready);
 
@@ -800,62 +918,53 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
     const bool valid = row < rows, active = i_row < act;
     const int node = valid ? row / rep : 0, dep = depth_s[node];
     const u64 anc = anc_s[1][node];
-    const int next = p0 % W;
+    const int next = p0 % W, max_dep = deepest;
     const uint32_t trow = (uint32_t)(quad * 32) << 16;
     float m = -INFINITY, l = 0.f;
     for (int i = 0; active && i < cnt; ++i) {
       const int t = t_lo + i, s = i & 1, j0 = (t - 1) * TR_KT;
       const bool is_tree = t == 0;
-      const int rel = is_tree ? 0 : (j0 - next + W) % W;
-      const bool edge = is_tree || j0 + TR_KT > nvalid || rel < TR_KT || rel + TR_KT > W;
+      // keys that not every row sees: the tree's, the ring's behind the last valid place and around the window's
+      // edge.  Values that must not reach the rows that do not see them leave the product (tree_values).
+      const u64 valid_keys = is_tree ? ~0ull : bit_range(0, nvalid - j0);
+      const u64 some = is_tree ? 0ull : hidden_places(j0, next, W, max_dep) & valid_keys;
       // scores i are issued once values i - 2 have been used: after this wait v_full's phase can be told
       mbar_wait(&s_full[s], (i >> 1) & 1, nullptr);
       tc_fence_after();
-      if (edge) {
-        // 0 * NaN would let a key's value reach rows that do not see it: such values leave the product and
-        // are added at the end to the rows that do
-        if (!is_tree) mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
-        if (i_row == 0) bad_keys = 0ull;
-        named_bar(2, act);
-        for (int k = i_row; k < TR_KT * CH; k += act) {
-          const int r = k / CH, c = k % CH;
-          uint4* p = reinterpret_cast<uint4*>(sV + s * LY::TILE + (c >> 3) * 8192 + sw128_offset(r, (c & 7) * 16));
-          const uint4 v = *p;
-          if (has_nonfinite(v.x) || has_nonfinite(v.y) || has_nonfinite(v.z) || has_nonfinite(v.w)) {
-            *p = make_uint4(finite_only(v.x), finite_only(v.y), finite_only(v.z), finite_only(v.w));
-            atomicOr(&bad_keys, 1ull << r);
+      if (some != 0ull || valid_keys != ~0ull) {
+        mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
+        auto at = [&](int r, int c) {
+          return reinterpret_cast<uint4*>(sV + s * LY::TILE + (c >> 3) * 8192 + sw128_offset(r, (c & 7) * 16));
+        };
+        for (int k = (nvalid - j0) * CH + i_row; k < TR_KT * CH; k += act)   // places never written
+          *at(k / CH, k % CH) = make_uint4(0, 0, 0, 0);
+        if (some != 0ull) {
+          if (i_row == 0) bad_keys = 0ull;
+          named_bar(2, act);
+          finite_values<HD>(i_row, act, some, &bad_keys, at);
+          named_bar(2, act);
+          if (i_row == 0 && bad_keys != 0ull && n_bad < 8) {   // at most three tiles around the edge
+            bad_mask[n_bad] = bad_keys;
+            bad_tile[n_bad++] = t;
           }
         }
         fence_proxy_async_smem();
-        named_bar(2, act);
-        if (i_row == 0 && bad_keys != 0ull && n_bad < 8) {   // at most a tree, a last tile and three of the edge
-          bad_mask[n_bad] = bad_keys;
-          bad_tile[n_bad++] = t;
-        }
       }
+      const u64 seen = is_tree ? anc : valid_keys & ~hidden_places(j0, next, W, dep);
       float sv[64];
 #pragma unroll
       for (int c = 0; c < 64; c += 16)
         tmem_ld16(tmem + s * 64 + c + trow, *reinterpret_cast<float(*)[16]>(&sv[c]));
       tmem_wait_ld();
-      float mt = -INFINITY;
-      if (edge) {
+      if (__any_sync(0xffffffffu, seen != ~0ull)) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) {
-          bool see;
-          if (is_tree) {
-            see = (anc >> c) & 1ull;
-          } else {
-            int back = j0 + c - next;
-            if (back < 0) back += W;
-            see = j0 + c < nvalid && back > dep;
-          }
-          if (!see) sv[c] = -INFINITY;
-        }
+        for (int c = 0; c < 64; ++c)
+          if (!((c < 32 ? (uint32_t)seen : (uint32_t)(seen >> 32)) >> (c & 31) & 1u)) sv[c] = -INFINITY;
       }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 64; ++c) mt = fmaxf(mt, sv[c]);
-      mt *= a.scale_log2;
+      for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
       const bool grow = mt > m + TT_GROWTH || m == -INFINITY;
       if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
         // O of this warp's rows holds sequences .. i - 1: their MMAs end first
@@ -876,6 +985,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       }
       if (grow) m = mt;
       const float ref = m == -INFINITY ? 0.f : m;   // nothing seen yet: every weight below is 0
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t hi[16], lo[16];
@@ -883,13 +993,14 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         for (int e = 0; e < 16; ++e) {
           const float x = exp2f(fmaf(sv[h * 32 + 2 * e], a.scale_log2, -ref));
           const float y = exp2f(fmaf(sv[h * 32 + 2 * e + 1], a.scale_log2, -ref));
-          l += x + y;
+          sum[e & 3] += x + y;
           hi[e] = pack_bf16x2(x, y);
           lo[e] = pack_bf16x2(x - bf16_lo(hi[e]), y - bf16_hi(hi[e]));
         }
         tmem_st16(tmem + s * 64 + h * 16 + trow, hi);
         tmem_st16(tmem + s * 64 + 32 + h * 16 + trow, lo);
       }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[s]);
@@ -899,95 +1010,73 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
     if (active && cnt > 0) mbar_wait(&v_empty[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1, nullptr);
     tc_fence_after();
     named_bar(1, 128);                   // bad_* is complete, no tile is in use any more
-    const float inv = 1.f / l;
-    float* part = reinterpret_cast<float*>(base) + (size_t)i_row * LY::OLD;
-    __nv_bfloat16* dst = a.out + ((size_t)b * N + node) * a.out_ld + (size_t)(g * rep + row % rep) * HD;
+    if (S > 1) cg::this_cluster().sync();   // every CTA has read its tiles: rows may be sent over them
+    const Joiner jn{reinterpret_cast<float*>(base), ml_s, S, 128 / S, LY::OLD};
+    cg::cluster_group cl = cg::this_cluster();
     if (active) {
-#pragma unroll
-      for (int k = 0; k < HD; k += 16) {
-        float ov[16];
+      const float inv = 1.f / l;
+      const bool any_bad = bad_tree != 0ull || n_bad > 0;
+      if (S > 1 && valid) jn.send_ml(cl, z, i_row, m, l);
+      float4* far = jn.row(cl, z, i_row);
+      __nv_bfloat16* dst = a.out + ((size_t)b * N + node) * a.out_ld + (size_t)(g * rep + row % rep) * HD;
+#pragma unroll 1
+      for (int k = 0; k < HD; k += 32) {
+        float ov[32];
         if (cnt > 0) {
-          tmem_ld16(tO + k + trow, ov);
+          tmem_ld16(tO + k + trow, *reinterpret_cast<float(*)[16]>(&ov[0]));
+          tmem_ld16(tO + k + 16 + trow, *reinterpret_cast<float(*)[16]>(&ov[16]));
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) ov[e] = 0.f;
+          for (int e = 0; e < 32; ++e) ov[e] = 0.f;
         }
-        for (int q = 0; q < n_bad; ++q)
-          for (u64 rest = bad_mask[q]; rest; rest &= rest - 1) {
-            const int key = __ffsll((long long)rest) - 1, t = bad_tile[q];
-            int back = (t - 1) * TR_KT + key - next;
-            if (back < 0) back += W;
-            const bool see = t == 0 ? (anc >> key) & 1ull : (t - 1) * TR_KT + key < nvalid && back > dep;
-            if (!see) continue;
-            const __nv_bfloat16* v = t == 0 ? qrows + (size_t)key * a.qkv_ld + v_col
-                                            : a.vring + ring0 + (size_t)((t - 1) * TR_KT + key) * HD;
+        if (any_bad)
+          for (int q = -1; q < n_bad; ++q) {   // the tree's, then the ring tiles'
+            const int t = q < 0 ? 0 : bad_tile[q];
+            u64 rest = q < 0 ? (has_tree ? bad_tree & anc : 0ull)
+                             : bad_mask[q] & ~hidden_places((t - 1) * TR_KT, next, W, dep);
+            for (; rest; rest &= rest - 1) {
+              const int key = __ffsll((long long)rest) - 1;
+              const __nv_bfloat16* v = t == 0 ? qrows + (size_t)key * a.qkv_ld + v_col
+                                              : a.vring + ring0 + (size_t)((t - 1) * TR_KT + key) * HD;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float x = __bfloat162float(v[k + e]);
-              if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) ov[e] += x;
+              for (int e = 0; e < 32; ++e) {
+                const float x = __bfloat162float(v[k + e]);
+                if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) ov[e] += x;
+              }
             }
           }
+        if (!valid) continue;
         if (S > 1) {
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4*>(part + k + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
-        } else if (valid) {
-          if (a.vec_out) {
+          for (int e = 0; e < 32; e += 4) far[(k + e) / 4] = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+        } else if (a.vec_out) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 8)
-              *reinterpret_cast<uint4*>(dst + k + e) =
-                  make_uint4(pack_bf16x2(ov[e] * inv, ov[e + 1] * inv), pack_bf16x2(ov[e + 2] * inv, ov[e + 3] * inv),
-                             pack_bf16x2(ov[e + 4] * inv, ov[e + 5] * inv),
-                             pack_bf16x2(ov[e + 6] * inv, ov[e + 7] * inv));
-          } else {
+          for (int e = 0; e < 32; e += 8)
+            *reinterpret_cast<uint4*>(dst + k + e) =
+                make_uint4(pack_bf16x2(ov[e] * inv, ov[e + 1] * inv), pack_bf16x2(ov[e + 2] * inv, ov[e + 3] * inv),
+                           pack_bf16x2(ov[e + 4] * inv, ov[e + 5] * inv), pack_bf16x2(ov[e + 6] * inv, ov[e + 7] * inv));
+        } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) dst[k + e] = __float2bfloat16(ov[e] * inv);
-          }
+          for (int e = 0; e < 32; ++e) dst[k + e] = __float2bfloat16(ov[e] * inv);
         }
       }
     }
-    cml[0][i_row] = m;
-    cml[1][i_row] = l;
   }
+  __syncwarp();
+  if (S > 1 && warp < 2) cg::this_cluster().sync();   // the same barrier, for the warps that issued
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, 256);
   if (S == 1) return;
-  // every CTA finishes every S-th row of the block
-  cg::cluster_group cl = cg::this_cluster();
-  cl.sync();
+  cg::this_cluster().sync();             // all rows have arrived; nothing remote after this
+  const Joiner jn{reinterpret_cast<float*>(base), ml_s, S, 128 / S, LY::OLD};
   const int live = min(128, rows - row0);
-  float* part0 = reinterpret_cast<float*>(base);
   for (int i = tid; i < (live - z + S - 1) / S * CH; i += TT_THREADS) {
-    const int r = z + i / CH * S, c8 = i % CH * 8, row = row0 + r;
-    float M = -INFINITY, L = 0.f, v[8];
-    for (int k = 0; k < S; ++k) M = fmaxf(M, cl.map_shared_rank(&cml[0][0], k)[r]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    for (int k = 0; k < S; ++k) {
-      const float* ml = cl.map_shared_rank(&cml[0][0], k);
-      const float mk = ml[r];
-      if (mk == -INFINITY) continue;     // a CTA whose keys this row does not see
-      const float f = exp2f(mk - M);
-      L += f * ml[128 + r];
-      const float* po = cl.map_shared_rank(part0, k) + (size_t)r * LY::OLD + c8;
-      const float4 x = reinterpret_cast<const float4*>(po)[0], y = reinterpret_cast<const float4*>(po)[1];
-      v[0] += f * x.x, v[1] += f * x.y, v[2] += f * x.z, v[3] += f * x.w;
-      v[4] += f * y.x, v[5] += f * y.y, v[6] += f * y.z, v[7] += f * y.w;
-    }
-    const float inv = 1.f / L;
-    __nv_bfloat16* dst = a.out + ((size_t)b * N + row / rep) * a.out_ld + (size_t)(g * rep + row % rep) * HD + c8;
-    if (a.vec_out) {
-      *reinterpret_cast<uint4*>(dst) =
-          make_uint4(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv),
-                     pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dst[e] = __float2bfloat16(v[e] * inv);
-    }
+    float v[8];
+    const float L = jn.join(i / CH, i % CH * 8, v);
+    store_out(a, b, g, row0 + z + i / CH * S, i % CH * 8, HD, v, 1.f / L);
   }
-  cl.sync();                             // no CTA leaves while another still reads its partial
 }
 
 template <int HD>
@@ -1007,10 +1096,7 @@ int launch_tree_tc(const TreeArgs& a, int B, cudaStream_t st) {
   UTTT_TRY(make_tmap_bf16(&tmV, a.vring, 3, dims, str, box));
   const int blocks = (a.N * a.rep + 127) / 128;
   UTTT_REQUIRE((long long)a.n_kv * blocks <= 65535, UTTT_ERR_UNSUPPORTED);
-  const long long ctas = (long long)B * a.n_kv * blocks;
-  const int tiles = (a.W + TR_KT - 1) / TR_KT + 1;
-  int S = 1;
-  while (S < 8 && ctas * S < 2LL * num_sms() && tiles / (2 * S) >= 2) S *= 2;
+  const int S = tree_split((long long)B * a.n_kv * blocks, (a.W + TR_KT - 1) / TR_KT + 1, 2, 4, 1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(S, a.n_kv * blocks, B);
   cfg.blockDim = dim3(TT_THREADS);
@@ -1031,12 +1117,14 @@ int launch_tree_tc(const TreeArgs& a, int B, cudaStream_t st) {
 template <int HD>
 int launch_tree_rows(const TreeArgs& a, int B, cudaStream_t st) {
   const int rows = a.N * a.rep;
-  if constexpr (HD >= 64)
-    if (rows > 32) return launch_tree_tc<HD>(a, B, st);
   if (rows <= 16) return launch_tree<HD, 1>(a, B, st);
   if (rows <= 32) return launch_tree<HD, 2>(a, B, st);
-  if (rows <= 64) return launch_tree<HD, 4>(a, B, st);
-  return launch_tree<HD, 8>(a, B, st);
+  if constexpr (HD >= 64) {
+    return launch_tree_tc<HD>(a, B, st);
+  } else {
+    if (rows <= 64) return launch_tree<HD, 4>(a, B, st);
+    return launch_tree<HD, 8>(a, B, st);
+  }
 }
 
 // One warp per row; lane l holds nodes l and l + 32.  From node 0 on, the path goes to the lowest later child
