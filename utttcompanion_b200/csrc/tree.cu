@@ -753,6 +753,29 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// whether the phase with this parity has completed (does not wait)
+__device__ __forceinline__ bool mbar_test(uint32_t bar_addr, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar_addr), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+constexpr uint32_t kMaxLoadPolls = 1u << 26;   // of some tens of cycles: far beyond any launch
+// one thread of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // grid (S, n_kv * row blocks, B), cluster (S, 1, 1): CTA z takes tiles [nt * z / S, nt * (z + 1) / S) of the nt
@@ -819,26 +842,36 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
       const int head = sl * a.n_kv + g;
-      auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, uint64_t* empty, int i) {
-        if (i >= cnt || (has_tree && i == 0)) return;
+      auto load = [&](const CUtensorMap* tm, uint8_t* ring, uint64_t* full, int i) {
+        if (has_tree && i == 0) return;  // written by warps 2-5
         const int s = i & 1;
-        if (i >= 2) mbar_wait(&empty[s], ((i >> 1) - 1) & 1, nullptr);
         mbar_arrive_expect_tx(&full[s], LY::TILE);
 #pragma unroll
         for (int h = 0; h < LY::BLK; ++h)
           tma_load_3d(ring + s * LY::TILE + h * 8192, tm, &full[s], h * 64, (t_lo + i - 1) * TR_KT, head);
       };
-      load(&tmK, sK, k_full, k_empty, 0);
-      for (int i = 0; i < cnt; ++i) {
-        load(&tmK, sK, k_full, k_empty, i + 1);
-        load(&tmV, sV, v_full, v_empty, i);
+      // keys and values each as soon as their own slot is free: keys' slots are released by the scores, a tile
+      // period before the values'
+      auto free_slot = [&](uint64_t* empty, int i) {
+        return i < 2 || mbar_test(smem_u32(&empty[i & 1]), ((i >> 1) - 1) & 1);
+      };
+      int ik = 0, iv = 0;
+      for (uint32_t polls = 0; (ik < cnt || iv < cnt) && polls < kMaxLoadPolls; ++polls) {
+        if (ik < cnt && free_slot(k_empty, ik)) load(&tmK, sK, k_full, ik++);
+        if (iv < cnt && free_slot(v_empty, iv)) load(&tmV, sV, v_full, iv++);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && cnt > 0) {
+    if (cnt > 0) {
+      // The whole warp runs this loop and one elected thread issues, so that descriptors stay in uniform registers
+      // (under a branch on the lane every MMA cost about 70 cycles to issue).  A descriptor's start address, in
+      // units of 16 bytes, is its low bits and moves by constants.
       const uint32_t id_s = idesc_bf16(128, 64, false, false);   // A = Q K-major, B = K K-major
       const uint32_t id_o = idesc_bf16(128, HD, false, true);    // A = P in TMEM, B = V MN-major
-      const uint32_t qa = smem_u32(sQ);
+      const uint64_t qd = sdesc_sw128(smem_u32(sQ), 16, 1024), kd = sdesc_sw128(smem_u32(sK), 16, 1024),
+                     vd = sdesc_sw128(smem_u32(sV), 8192, 1024);
+      const uint32_t tS = __shfl_sync(0xffffffffu, tmem, 0);
+      const bool leader = elect_one();
       mbar_wait(&ready, 0, nullptr);
       auto issue_s = [&](int i) {
         const int s = i & 1;
@@ -846,13 +879,15 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         // P of sequence i - 2 has left this buffer
         if (i >= 2) mbar_wait(&v_empty[s], ((i >> 1) - 1) & 1, nullptr);
         tc_fence_after();
-        const uint32_t ka = smem_u32(sK + s * LY::TILE);
+        const uint64_t ks = kd + (uint64_t)(s * (LY::TILE >> 4));
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          mma_bf16(tmem + s * 64, sdesc_sw128(qa + (k >> 2) * 16384 + (k & 3) * 32, 16, 1024),
-                   sdesc_sw128(ka + (k >> 2) * 8192 + (k & 3) * 32, 16, 1024), id_s, k > 0 ? 1u : 0u);
-        mma_commit(&s_full[s]);
-        mma_commit(&k_empty[s]);
+          for (int k = 0; k < HD / 16; ++k)
+            mma_bf16(tS + s * 64, qd + ((k >> 2) * 16384 + (k & 3) * 32) / 16,
+                     ks + ((k >> 2) * 8192 + (k & 3) * 32) / 16, id_s, k > 0 ? 1u : 0u);
+          mma_commit(&s_full[s]);
+          mma_commit(&k_empty[s]);
+        }
       };
       issue_s(0);
       for (int i = 0; i < cnt; ++i) {
@@ -861,12 +896,14 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         if (!(has_tree && i == 0)) mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
         mbar_wait(&p_full[s], (i >> 1) & 1, nullptr);
         tc_fence_after();
-        const uint32_t va = smem_u32(sV + s * LY::TILE), pa = tmem + s * 64;
+        const uint64_t vs = vd + (uint64_t)(s * (LY::TILE >> 4));
+        const uint32_t pa = tS + s * 64;
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)      // P_hi V (columns 0 .. 31), then P_lo V (32 .. 63): 8 columns per 16 keys
-          mma_bf16_ts(tO, pa + k * 8, sdesc_sw128(va + (k & 3) * 2048, 8192, 1024), id_o,
-                      (i > 0 || k > 0) ? 1u : 0u);
-        mma_commit(&v_empty[s]);
+          for (int k = 0; k < 8; ++k)    // P_hi V (columns 0 .. 31), then P_lo V (32 .. 63): 8 columns per 16 keys
+            mma_bf16_ts(tS + 128, pa + k * 8, vs + (k & 3) * 2048 / 16, id_o, (i > 0 || k > 0) ? 1u : 0u);
+          mma_commit(&v_empty[s]);
+        }
       }
     }
   } else {
