@@ -5,26 +5,30 @@
 //
 // Mathematics.  A row's candidates are its ids below active_limit that are not
 // PAD / BOS / UNK and whose logit is neither NaN nor -inf.  With m the largest
-// logit, w_i = exp((s_i - m) / T).  Candidates are ordered by (s descending, id
-// ascending); top-k keeps the first k, top-p those whose mass before them is at
-// most top_p times the mass top-k left, min-p those with w_i >= min_p.  All three
-// keep a prefix of that order, so the kept set is one cut element.  The pick is
-// the lowest id i with (sum of kept w_j, j <= i) > u * (sum of all kept w_j).
+// logit, w_i = exp((s_i - m) / T) = 2^-x_i, x_i = (m - s_i) log2(e) / T.  Candidates
+// are ordered by (s descending, id ascending); top-k keeps the first k, top-p
+// those whose mass before them is at most top_p times the mass top-k left, min-p
+// those with w_i >= min_p.  All three keep a prefix of that order, so the kept set
+// is one cut element.  The pick is the lowest id i with (sum of kept w_j, j <= i)
+// > u * (sum of all kept w_j).
 //
-// Exactness.  w_i is evaluated in 64 bits (table of 2^(j/32) and a short Taylor
-// polynomial: the table-driven method of Tang, ACM TOMS 15, 1989) and rounded
-// once to a whole number of 2^-45, so every sum of weights is an exact 64-bit
+// Whole-number weights.  x_i is computed in 64 bits and taken to a whole number of
+// 2^-32; 2^-x_i comes from its integer part (a shift), the next 7 bits (a table of
+// 2^(-j/128)) and the rest (a cubic Taylor polynomial: the table-driven method of
+// Tang, ACM TOMS 15, 1989), as a whole number of 2^-45, good to 2^-29 of itself
+// (all carry one common factor, 1 - 2^-20, which keeps the table within 32 bits
+// and leaves every ratio alone).  So every sum of weights is an exact 64-bit
 // integer that does not depend on the order of the additions: histograms with
 // atomics, splits over CTAs and any grid give the same cut and the same pick.
-// A rounding moves a sum of n weights by at most n * 2^-46 of the largest one.
 //
-// Layout.  One cluster of S CTAs per row; CTA r keeps its part of the row's
-// logits in shared memory as order-preserving 32-bit keys, read from HBM once.
-// A cut is found by a histogram over 2048 bins of the exponent (linear in
-// s - m), merged over the cluster in distributed shared memory, and the few
-// candidates of the bin that holds it are ranked against each other; a bin with
-// too many (equal or nearly equal logits) is split again by the bits of its
-// (key, id) pairs until few are left.
+// Layout.  One cluster of S CTAs per row; each warp owns a contiguous piece of the
+// row and streams it in 16-byte loads, once per step (the row comes from HBM once
+// and stays in L1 / L2 for the others): (1) largest logit; (2) where top-k or top-p
+// ask for it, a histogram over 2048 bins of x, merged over the cluster in
+// distributed shared memory, and (3) the candidates of the bin that holds the cut,
+// ranked against each other; a bin with too many of them (equal or nearly equal
+// logits) is split again by the bits of its (key, id) pairs; (4) kept mass per
+// warp; the warp that holds the pick walks its piece again.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -41,7 +45,9 @@ constexpr int SM_BINS = 2048;
 constexpr int SM_CAP = 256;              // candidates ranked against each other directly
 constexpr int SM_MAX_CTAS = 8;
 constexpr int SM_MAX_V = 262144;         // 8 CTAs of 32768 keys
-constexpr double SM_RANGE = 46.0;        // weights below 2^-46 round to zero
+constexpr int SM_MAX_PART = 65536;       // ids per CTA: sums of as many 16-bit limbs stay below 2^32
+constexpr float SM_RANGE = 62.f;         // x from here on is the last bin; weights below 2^-46 are zero
+constexpr int SM_STEPS = 128;            // table entries per octave
 constexpr float SM_GREEDY_T = 1e-5f;     // _sample_next_token's greedy border
 
 typedef unsigned long long u64;
@@ -51,7 +57,7 @@ struct Sel {     // value exchanged between the CTAs of a cluster
 };
 
 struct SampleShared {
-  double tab[32];                        // 2^(j / 32)
+  unsigned tab[SM_STEPS * 32];           // the table once per lane: no bank conflicts
   Sel xch[2][SM_MAX_CTAS];               // one slot per CTA, two phases
   u64 wred[SM_WARPS], wred2[SM_WARPS];
   u64 cand[2][SM_CAP];                   // rank 0: gathered candidates; others: their copies of them
@@ -62,42 +68,86 @@ struct SampleShared {
   unsigned hist[3][SM_BINS];             // count, or 16-bit limbs of the mass
 };
 
-// order-preserving key of a logit: larger logit, larger key; 0 for excluded ones.  Both zeros are one value.
+// floor(2^32 * 2^(-j / 128) * (1 - 2^-20))
+__device__ const unsigned kPow2[SM_STEPS] = {
+    0xfffff000u, 0xfe9e0172u, 0xfd3dfc39u, 0xfbdfddaeu, 0xfa83a333u, 0xf9294a28u, 0xf7d0cff5u, 0xf67a3204u,
+    0xf5256dc2u, 0xf3d280a1u, 0xf2816814u, 0xf1322194u, 0xefe4aa9du, 0xee9900aeu, 0xed4f2149u, 0xec0709f5u,
+    0xeac0b83bu, 0xe97c29a8u, 0xe8395bccu, 0xe6f84c3bu, 0xe5b8f88bu, 0xe47b5e58u, 0xe33f7b3eu, 0xe2054cdfu,
+    0xe0ccd0dfu, 0xdf9604e5u, 0xde60e69cu, 0xdd2d73b2u, 0xdbfba9d8u, 0xdacb86c2u, 0xd99d0828u, 0xd8702bc5u,
+    0xd744ef56u, 0xd61b509cu, 0xd4f34d5cu, 0xd3cce35cu, 0xd2a81067u, 0xd184d24au, 0xd06326d4u, 0xcf430bdau,
+    0xce247f32u, 0xcd077eb5u, 0xcbec0840u, 0xcad219b1u, 0xc9b9b0eau, 0xc8a2cbd2u, 0xc78d684fu, 0xc679844eu,
+    0xc5671dbau, 0xc4563286u, 0xc346c0a5u, 0xc238c60du, 0xc12c40b7u, 0xc0212e9fu, 0xbf178dc5u, 0xbe0f5c28u,
+    0xbd0897ceu, 0xbc033ebeu, 0xbaff4f02u, 0xb9fcc6a5u, 0xb8fba3b7u, 0xb7fbe44au, 0xb6fd8673u, 0xb6008848u,
+    0xb504e7e3u, 0xb40aa361u, 0xb311b8e1u, 0xb21a2684u, 0xb123ea6fu, 0xb02f02c8u, 0xaf3b6db9u, 0xae49296eu,
+    0xad583414u, 0xac688bdeu, 0xab7a2efeu, 0xaa8d1baau, 0xa9a1501au, 0xa8b6ca8bu, 0xa7cd8938u, 0xa6e58a61u,
+    0xa5fecc49u, 0xa5194d35u, 0xa4350b6au, 0xa3520533u, 0xa27038dcu, 0xa18fa4b1u, 0xa0b04704u, 0x9fd21e28u,
+    0x9ef52871u, 0x9e196437u, 0x9d3ecfd3u, 0x9c6569a1u, 0x9b8d3001u, 0x9ab62151u, 0x99e03bf5u, 0x990b7e51u,
+    0x9837e6ceu, 0x976573d3u, 0x969423cdu, 0x95c3f52au, 0x94f4e659u, 0x9426f5cdu, 0x935a21f9u, 0x928e6954u,
+    0x91c3ca57u, 0x90fa437cu, 0x9031d33fu, 0x8f6a7821u, 0x8ea430a1u, 0x8ddefb42u, 0x8d1ad689u, 0x8c57c0feu,
+    0x8b95b92au, 0x8ad4bd97u, 0x8a14ccd3u, 0x8955e56eu, 0x889805f7u, 0x87db2d02u, 0x871f5924u, 0x866488f5u,
+    0x85aabb0du, 0x84f1ee07u, 0x843a2080u, 0x83835116u, 0x82cd7e6bu, 0x8218a721u, 0x8164c9ddu, 0x80b1e544u,
+};
+
+// order-preserving key of a logit: larger logit, larger key.  Both zeros are one value.
 __device__ __forceinline__ unsigned order_key(unsigned bits) {
-  if ((bits << 1) > 0xff000000u || bits == 0xff800000u) return 0u;   // NaN, -inf
-  if ((bits << 1) == 0u) bits = 0u;
-  return (bits & 0x80000000u) ? ~bits : (bits | 0x80000000u);
+  const unsigned k = bits ^ ((unsigned)((int)bits >> 31) | 0x80000000u);
+  return k == 0x7fffffffu ? 0x80000000u : k;
 }
+// whether a key is a candidate's: neither NaN (beyond either end) nor -inf
+__device__ __forceinline__ bool is_candidate(unsigned k) { return k - 0x00800000u <= 0xff000000u; }
+constexpr unsigned kInfKey = 0xff800000u;   // of +inf, the largest candidate
 __device__ __forceinline__ float key_value(unsigned k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
 // (key, id) as one number: larger comes first in the order
 __device__ __forceinline__ u64 pair_of(unsigned key, unsigned id) { return ((u64)key << 32) | (0xffffffffu - id); }
 
+// a FP32 number as a double, without the slow conversion (subnormals come out as other numbers below 2^-126,
+// next to any logit that is not one itself as good as zero)
+__device__ __forceinline__ double widen(unsigned bits) {
+  return __hiloint2double((int)((bits & 0x80000000u) | (((bits & 0x7fffffffu) >> 3) + 0x38000000u)),
+                          (int)(bits << 29));
+}
+
 struct Weigher {
   double m, c;          // largest logit, log2(e) / T
-  unsigned mkey;
+  float mf, cf;
   bool top_inf;         // the largest logit is +inf: only its equals have weight
-  const double* tab;
-  // log2 of the weight (<= 0)
-  __device__ __forceinline__ double exponent(unsigned key) const {
-    if (key == mkey) return 0.0;
-    if (top_inf) return -1e300;
-    return ((double)key_value(key) - m) * c;
+  const unsigned* tab;  // this lane's copy
+  // whether x is in range (else the element is in the last bin and has no weight)
+  __device__ __forceinline__ bool in_range(unsigned bits) const {
+    const float s = __uint_as_float(bits);
+    if (top_inf) return bits == 0x7f800000u;
+    return (mf - s) * cf <= SM_RANGE;    // not for NaN and -inf
   }
-  // the weight in units of 2^-45
-  __device__ __forceinline__ u64 weight(double x) const {
-    if (x < -SM_RANGE) return 0ull;
-    const double t = x * 32.0, n = rint(t);
-    const double r = (t - n) * 0.021660849392498290;      // ln 2 / 32; |r| <= ln 2 / 64
-    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);           // exp(r), error r^6 / 720 <= 2.3e-15
-    p = fma(r, p, 1.0 / 6.0);
-    p = fma(r, p, 0.5);
-    p = fma(r, p, 1.0);
-    p = fma(r, p, 1.0);
-    const int ni = (int)n;
-    const double scale = __longlong_as_double((long long)(1023 + 45 + (ni >> 5)) << 52);
-    return __double2ull_rn(tab[ni & 31] * p * scale);
+  // x >= 0 of an element in range
+  __device__ __forceinline__ double exponent(unsigned bits) const {
+    return top_inf ? 0.0 : (m - widen(bits)) * c;
+  }
+  // x as a whole number of 2^-32 (high word: integer part)
+  __device__ __forceinline__ uint2 fixed(double x) const {
+    const double t = x + 1048576.0;      // 2^20: the last place is 2^-32
+    return make_uint2((unsigned)__double2loint(t), (unsigned)__double2hiint(t) & 0xfffffu);
+  }
+  // 1/32 wide bins of x
+  __device__ __forceinline__ int bin(uint2 x) const { return (int)__funnelshift_l(x.x, x.y, 5); }
+  // 2^-x in units of 2^-45
+  __device__ __forceinline__ u64 weight(uint2 x) const {
+    const unsigned t = tab[(x.x >> 25) * 32];
+    // q = 1 - 2^-r = r ln 2 - (r ln 2)^2 / 2 + (r ln 2)^3 / 6, r < 2^-7 (the next term is below 2^-34)
+    const float r = (float)(x.x & 0x1ffffffu);           // in units of 2^-32
+    constexpr float a1 = 1.61385904e-10f, a2 = 1.3022705e-20f, a3 = 7.0056034e-31f;
+    const float q = r * (a1 - r * (a2 - r * a3));
+    // its mantissa bits behind 2^-7 are q in units of 2^-30
+    const unsigned qi = __float_as_uint(q + 0.0078125f) & 0x7fffffu;
+    const unsigned w = t - __umulhi(t, qi << 2);
+    const int sh = 13 - (int)x.y;
+    if (sh >= 0) return (u64)w << sh;
+    return sh < -32 ? 0ull : (u64)(((w >> (-sh - 1)) + 1u) >> 1);
+  }
+  __device__ __forceinline__ u64 weight_of(unsigned key) const {
+    const unsigned bits = __float_as_uint(key_value(key));
+    return in_range(bits) ? weight(fixed(exponent(bits))) : 0ull;
   }
 };
 
@@ -142,7 +192,7 @@ struct Cluster {
   __device__ __forceinline__ int exchange(Sel v) {
     const int ph = phase;
     phase ^= 1;
-    if (threadIdx.x < S) peer(threadIdx.x)->xch[ph][rank] = v;   // v is the same in every thread
+    if ((int)threadIdx.x < S) peer(threadIdx.x)->xch[ph][rank] = v;   // v is the same in every thread
     sync();
     return ph;
   }
@@ -150,12 +200,63 @@ struct Cluster {
 
 enum { FIND_COUNT, FIND_MASS };
 
+// A row's piece of one warp: 8-logit vectors v0 .. v1 - 1, the lanes side by side.
 struct Row {
-  const unsigned* keys;   // this CTA's part, shared memory
-  int n, id0;             // its length and first id
+  const char* src;        // the row
+  bool f32, vec;          // its type; whether it starts on 16 bytes
+  int V, lim, stop_free;
+  int v0, v1;
+
+  __device__ __forceinline__ void load(int v, uint4& a, uint4& b) const {
+    if (vec && v * 8 + 8 <= V) {
+      const uint4* p = reinterpret_cast<const uint4*>(src) + (size_t)v * (f32 ? 2 : 1);
+      a = __ldg(p);
+      if (f32) b = __ldg(p + 1);
+      return;
+    }
+    unsigned x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int i = min(v * 8 + e, V - 1);   // what lies behind the row is masked below
+      x[e] = f32 ? __ldg(reinterpret_cast<const unsigned*>(src) + i)
+                 : (unsigned)__ldg(reinterpret_cast<const unsigned short*>(src) + i);
+    }
+    if (f32) {
+      a = make_uint4(x[0], x[1], x[2], x[3]);
+      b = make_uint4(x[4], x[5], x[6], x[7]);
+    } else {
+      a = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+    }
+  }
+  // f(bits[8], first id) for every vector of the piece, in step over the warp; ids that are never picked come as -inf
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    const int lane = threadIdx.x & 31;
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (v0 + lane < v1) load(v0 + lane, a, b);
+    for (int t = v0; t < v1; t += 32) {
+      const int v = t + lane;
+      unsigned x[8];
+      if (f32) {
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+      } else {
+        x[0] = a.x << 16, x[1] = a.x & 0xffff0000u, x[2] = a.y << 16, x[3] = a.y & 0xffff0000u;
+        x[4] = a.z << 16, x[5] = a.z & 0xffff0000u, x[6] = a.w << 16, x[7] = a.w & 0xffff0000u;
+      }
+      if (v + 32 < v1) load(v + 32, a, b);
+      if (v == 0 || v >= v1 || v * 8 + 8 > lim) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int id = v * 8 + e;
+          if (v >= v1 || id >= lim || id == 0 || id == 1 || id == 3 || (stop_free && id < 6)) x[e] = 0xff800000u;
+        }
+      }
+      if (!f(x, v * 8)) return;
+    }
+  }
 };
 
-// Gather the pairs that in_range takes (of all CTAs) into rank 0's list; returns how many there are.  Every CTA
+// Gather the pairs that f(bits) takes (of all CTAs) into rank 0's list; returns how many there are.  Every CTA
 // then holds a copy in cand[c.list] if they are at most SM_CAP.  Consecutive gathers use the two lists in turn, so
 // a CTA may start the next one while another still ranks this one's; the other list's counter is cleared between
 // this gather's two barriers, after its last reader and before its next writer.
@@ -163,15 +264,15 @@ template <class InRange>
 __device__ unsigned gather(Cluster& c, const Row& row, InRange in_range) {
   SampleShared* lead = c.peer(0);
   const int q = c.list ^= 1;
-  for (int i = threadIdx.x; i < row.n; i += SM_THREADS) {
-    const unsigned key = row.keys[i];
-    if (key == 0u) continue;
-    const u64 pr = pair_of(key, row.id0 + i);
-    if (in_range(key, pr)) {
-      const unsigned at = atomicAdd(&lead->n_cand[q], 1u);
-      if (at < SM_CAP) lead->cand[q][at] = pr;
-    }
-  }
+  row.each([&](const unsigned (&x)[8], int id) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (in_range(x[e], id + e)) {
+        const unsigned at = atomicAdd(&lead->n_cand[q], 1u);
+        if (at < SM_CAP) lead->cand[q][at] = pair_of(order_key(x[e]), id + e);
+      }
+    return true;
+  });
   c.sync();
   const unsigned n = lead->n_cand[q];
   if (n <= SM_CAP && c.rank != 0)
@@ -191,7 +292,7 @@ __device__ u64 rank_candidates(Cluster& c, unsigned n, int mode, u64 target, con
   if (threadIdx.x == 0) sh->res_cut = 0ull;
   if (threadIdx.x < n) {
     mine = cand[threadIdx.x];
-    own = mode == FIND_COUNT ? 1ull : w.weight(w.exponent((unsigned)(mine >> 32)));
+    own = mode == FIND_COUNT ? 1ull : w.weight_of((unsigned)(mine >> 32));
     sh->cand_w[threadIdx.x] = own;
   }
   __syncthreads();
@@ -211,10 +312,13 @@ __device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, int mode, 
                         u64 cut, unsigned n_eligible) {
   SampleShared* sh = c.sh;
   if (n_eligible <= SM_CAP) {            // few enough to rank at once
-    const unsigned n = gather(c, row, [&](unsigned, u64 pr) { return pr >= cut; });
+    const unsigned n = gather(c, row, [&](unsigned bits, int id) {
+      const unsigned key = order_key(bits);
+      return is_candidate(key) && pair_of(key, id) >= cut;
+    });
     u64 target = count_target;
     if (mode == FIND_MASS) {
-      u64 v = threadIdx.x < n ? w.weight(w.exponent((unsigned)(sh->cand[c.list][threadIdx.x] >> 32))) : 0ull;
+      u64 v = threadIdx.x < n ? w.weight_of((unsigned)(sh->cand[c.list][threadIdx.x] >> 32)) : 0ull;
       v = warp_sum64(v);
       __syncthreads();
       if ((threadIdx.x & 31) == 0) sh->wred[threadIdx.x >> 5] = v;
@@ -230,35 +334,40 @@ __device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, int mode, 
   u64 lo = 0ull, hi = ~0ull, target = count_target;
   int sh_bits = -1;
   for (int pass = 0; pass < 10; ++pass) {
-    auto bin_of = [&](unsigned key, u64 pr, double x) -> int {
-      if (sh_bits >= 0) return (int)((hi - pr) >> sh_bits);
-      const float f = (float)(-x) * (float)((SM_BINS - 1) / SM_RANGE);
-      return f < (float)(SM_BINS - 1) ? (int)f : SM_BINS - 1;
-    };
     for (int i = threadIdx.x; i < 3 * SM_BINS; i += SM_THREADS) (&sh->hist[0][0])[i] = 0u;
     __syncthreads();
     unsigned tail = 0u;
-    for (int i = threadIdx.x; i < row.n; i += SM_THREADS) {
-      const unsigned key = row.keys[i];
-      if (key == 0u) continue;
-      const u64 pr = pair_of(key, row.id0 + i);
-      if (pr < cut || pr < lo || pr > hi) continue;
-      const double x = w.exponent(key);
-      const int bin = bin_of(key, pr, x);
-      if (mode == FIND_COUNT) {
-        if (sh_bits < 0 && bin == SM_BINS - 1)
-          ++tail;                        // the far tail is one bin: counted in registers
-        else
-          atomicAdd(&sh->hist[0][bin], 1u);
-      } else {
-        const u64 wt = w.weight(x);
-        if (wt) {
-          atomicAdd(&sh->hist[0][bin], (unsigned)(wt & 0xffffu));
-          atomicAdd(&sh->hist[1][bin], (unsigned)((wt >> 16) & 0xffffu));
-          atomicAdd(&sh->hist[2][bin], (unsigned)(wt >> 32));
+    row.each([&](const unsigned (&x)[8], int id) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = w.in_range(x[e]);
+        int bin;
+        uint2 fx;
+        if (sh_bits >= 0 || cut != 0ull || !in) {   // anything but the first pass over a whole row
+          const unsigned key = order_key(x[e]);
+          const u64 pr = pair_of(key, id + e);
+          if (!is_candidate(key) || pr < cut || pr < lo || pr > hi) continue;
+          bin = sh_bits >= 0 ? (int)((hi - pr) >> sh_bits) : SM_BINS - 1;
+        }
+        if (in) {
+          fx = w.fixed(w.exponent(x[e]));
+          if (sh_bits < 0) bin = w.bin(fx);
+        }
+        if (mode == FIND_COUNT) {
+          if (sh_bits < 0 && !in)
+            ++tail;                      // the far tail is one bin: counted in registers
+          else
+            atomicAdd(&sh->hist[0][bin], 1u);
+        } else if (in) {
+          const u64 wt = w.weight(fx);
+          const unsigned l0 = (unsigned)wt & 0xffffu, l1 = (unsigned)wt >> 16, l2 = (unsigned)(wt >> 32);
+          if (l0) atomicAdd(&sh->hist[0][bin], l0);
+          if (l1) atomicAdd(&sh->hist[1][bin], l1);
+          if (l2) atomicAdd(&sh->hist[2][bin], l2);
         }
       }
-    }
+      return true;
+    });
     if (mode == FIND_COUNT) {
       const unsigned t = __reduce_add_sync(0xffffffffu, tail);
       if ((threadIdx.x & 31) == 0 && t) atomicAdd(&sh->hist[0][SM_BINS - 1], t);
@@ -319,14 +428,16 @@ __device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, int mode, 
     if (bin < 0) return cut;             // everything is within the target
     target -= sh->res_base;
     u64 mn = ~0ull, mx = 0ull;
-    const unsigned n = gather(c, row, [&](unsigned key, u64 pr) {
-      if (pr < cut || pr < lo || pr > hi) return false;
-      const bool in = bin_of(key, pr, sh_bits >= 0 ? 0.0 : w.exponent(key)) == bin;
-      if (in) {
-        mn = pr < mn ? pr : mn;
-        mx = pr > mx ? pr : mx;
-      }
-      return in;
+    const unsigned n = gather(c, row, [&](unsigned bits, int id) {
+      const bool in = w.in_range(bits);
+      if (sh_bits < 0 && (in ? w.bin(w.fixed(w.exponent(bits))) : SM_BINS - 1) != bin) return false;
+      const unsigned key = order_key(bits);
+      const u64 pr = pair_of(key, id);
+      if (!is_candidate(key) || pr < cut || pr < lo || pr > hi) return false;
+      if (sh_bits >= 0 && (int)((hi - pr) >> sh_bits) != bin) return false;
+      mn = pr < mn ? pr : mn;
+      mx = pr > mx ? pr : mx;
+      return true;
     });
     if (n <= SM_CAP) {
       const u64 r = rank_candidates(c, n, mode, target, w);
@@ -358,77 +469,47 @@ __device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, int mode, 
 }
 
 template <bool F32>
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(
-    const void* __restrict__ logits, long long ld, int lim, int part, int stop_free, UtttSampling opt,
+__global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
+    const void* __restrict__ logits, long long ld, int V, int lim, int part, int stop_free, UtttSampling opt,
     const float* __restrict__ u, long long u_ld, const int* __restrict__ u_index, int u_len, int* __restrict__ ids,
     int* __restrict__ kept, float* __restrict__ prob) {
-  extern __shared__ __align__(16) unsigned keys[];
-  __shared__ SampleShared shared;
-  SampleShared* sh = &shared;
+  extern __shared__ __align__(16) uint8_t smem[];
+  SampleShared* sh = reinterpret_cast<SampleShared*>(smem);
   Cluster c{cg::this_cluster(), sh, (int)blockIdx.x, (int)gridDim.x, 0, 0};
   const int row_i = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  pdl_wait();
-  pdl_trigger();
-  if (tid < 32) sh->tab[tid] = exp2((double)tid / 32.0);
   if (tid < 2) sh->n_cand[tid] = 0u;
   c.arrive();                            // peers write here only once every CTA of the cluster has started
-  // ---- this CTA's part of the row, as keys
+  for (int i = tid; i < SM_STEPS * 32; i += SM_THREADS) sh->tab[i] = kPow2[i >> 5];
+  pdl_wait();
+  pdl_trigger();
+  // ---- the warp's piece of the row (`part` 8-logit vectors per CTA)
   Row row;
-  row.keys = keys;
-  row.id0 = c.rank * part;
-  row.n = max(0, min(part, lim - row.id0));
-  constexpr int E = F32 ? 4 : 8;         // logits per 16-byte load
-  const char* src = reinterpret_cast<const char*>(logits) + ((size_t)row_i * ld + row.id0) * (F32 ? 4 : 2);
+  row.src = reinterpret_cast<const char*>(logits) + (size_t)row_i * ld * (F32 ? 4 : 2);
+  row.f32 = F32;
+  row.vec = (reinterpret_cast<uintptr_t>(row.src) & 15u) == 0;
+  row.V = V;
+  row.lim = lim;
+  row.stop_free = stop_free;
+  const int end = min((c.rank + 1) * part, (lim + 7) / 8), per = ((part + SM_WARPS - 1) / SM_WARPS + 31) & ~31;
+  row.v0 = min(end, c.rank * part + warp * per);
+  row.v1 = min(end, row.v0 + per);
   u64 best = 0ull;
-  unsigned count = 0u;
-  auto put = [&](int i, unsigned bits) {
-    const int id = row.id0 + i;
-    const bool out = id == 0 || id == 1 || id == 3 || (stop_free && id < 6);
-    const unsigned k = out ? 0u : order_key(bits);
-    keys[i] = k;
-    if (k) {
-      ++count;
-      const u64 pr = pair_of(k, id);
-      best = pr > best ? pr : best;
-    }
-  };
-  const int nv = (reinterpret_cast<uintptr_t>(src) & 15u) == 0 ? row.n / E : 0;
-  for (int j = tid; j < nv; j += SM_THREADS) {
-    const uint4 v = reinterpret_cast<const uint4*>(src)[j];
-    const unsigned x[4] = {v.x, v.y, v.z, v.w};
+  row.each([&](const unsigned (&x)[8], int id) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (F32) {
-        put(j * E + e, x[e]);
-      } else {
-        put(j * E + 2 * e, x[e] << 16);
-        put(j * E + 2 * e + 1, x[e] & 0xffff0000u);
-      }
+    for (int e = 0; e < 8; ++e) {
+      const unsigned k = order_key(x[e]);
+      if (k > (unsigned)(best >> 32) && k <= kInfKey) best = pair_of(k, id + e);   // ids rise: the first stays
     }
-  }
-  for (int i = nv * E + tid; i < row.n; i += SM_THREADS)
-    put(i, F32 ? reinterpret_cast<const unsigned*>(src)[i]
-               : (unsigned)reinterpret_cast<const unsigned short*>(src)[i] << 16);
+    return true;
+  });
   best = warp_max64(best);
-  count = __reduce_add_sync(0xffffffffu, count);
-  if (lane == 0) {
-    sh->wred[warp] = best;
-    sh->wred2[warp] = count;
-  }
+  if (lane == 0) sh->wred[warp] = best;
   __syncthreads();
-  u64 cnt = 0ull;
-  for (int i = 0; i < SM_WARPS; ++i) {
-    best = sh->wred[i] > best ? sh->wred[i] : best;
-    cnt += sh->wred2[i];
-  }
+  for (int i = 0; i < SM_WARPS; ++i) best = sh->wred[i] > best ? sh->wred[i] : best;
   c.wait();
-  const int ph = c.exchange(Sel{best, cnt});
-  cnt = 0ull;
-  for (int r = 0; r < c.S; ++r) {
-    best = sh->xch[ph][r].a > best ? sh->xch[ph][r].a : best;
-    cnt += sh->xch[ph][r].b;
-  }
-  if (cnt == 0ull) {                     // nothing to choose from: an allowed id, as the greedy pick gives
+  const int ph = c.exchange(Sel{best, 0ull});
+  for (int r = 0; r < c.S; ++r) best = sh->xch[ph][r].a > best ? sh->xch[ph][r].a : best;
+  if (!is_candidate((unsigned)(best >> 32))) {   // nothing to choose from: an allowed id, as the greedy pick gives
     if (c.rank == 0 && tid == 0) {
       ids[row_i] = (stop_free ? 6 : 2) % lim;
       if (kept) kept[row_i] = 0;
@@ -445,43 +526,47 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(
   const bool greedy = !(T > SM_GREEDY_T) || top_k == 1;
   if (greedy) T = 1.f;
   Weigher w;
-  w.mkey = (unsigned)(best >> 32);
-  w.m = (double)key_value(w.mkey);
-  w.top_inf = w.mkey == 0xff800000u;
+  const unsigned mkey = (unsigned)(best >> 32);
+  w.mf = key_value(mkey);
+  w.m = widen(__float_as_uint(w.mf));
+  w.top_inf = mkey == kInfKey;
   w.c = 1.4426950408889634074 / (double)T;
-  w.tab = sh->tab;
+  w.cf = (float)w.c;
+  w.tab = sh->tab + lane;
   u64 cut = 0ull;
   if (greedy) {
     cut = best;
   } else {
-    u64 eligible = cnt;
-    if (top_k > 0 && (u64)top_k < cnt) {
-      cut = find_cut(c, row, w, FIND_COUNT, (u64)(top_k - 1), 0.f, cut, (unsigned)eligible);
-      eligible = top_k;
+    unsigned eligible = (unsigned)lim;
+    if (top_k > 0 && top_k < lim) {
+      cut = find_cut(c, row, w, FIND_COUNT, (u64)(top_k - 1), 0.f, cut, eligible);
+      eligible = (unsigned)top_k;
     }
-    if (top_p < 1.f) cut = find_cut(c, row, w, FIND_MASS, 0ull, top_p, cut, (unsigned)eligible);
+    if (top_p < 1.f) cut = find_cut(c, row, w, FIND_MASS, 0ull, top_p, cut, eligible);
   }
-  const double x_min = min_p > 0.f ? log2((double)fminf(min_p, 1.f)) : -INFINITY;
-  // ---- mass of the kept elements per warp; warp k of the CTA has ids [k * seg, (k + 1) * seg) of its part
-  const int seg = ((row.n + SM_WARPS - 1) / SM_WARPS + 31) & ~31;
-  const int i0 = warp * seg, i1 = min(row.n, i0 + seg);
-  auto weigh = [&](int i, bool& in) -> u64 {
-    in = false;
-    if (i >= i1) return 0ull;
-    const unsigned key = keys[i];
-    if (key == 0u || pair_of(key, row.id0 + i) < cut) return 0ull;
-    const double x = w.exponent(key);
-    if (!(x >= x_min)) return 0ull;
-    in = true;
-    return w.weight(x);
+  const double x_max = min_p > 0.f ? -log2((double)fminf(min_p, 1.f)) : INFINITY;
+  // ---- kept mass per warp
+  const unsigned cut_key = max((unsigned)(cut >> 32), 0x00800000u);
+  auto weigh = [&](unsigned bits, int id, bool& in) -> u64 {
+    const unsigned key = order_key(bits);
+    in = key >= cut_key && key <= kInfKey && pair_of(key, id) >= cut;
+    if (!in) return 0ull;
+    const bool near = w.in_range(bits);
+    const double x = near ? w.exponent(bits) : 1e300;
+    in = x <= x_max;
+    return near && in ? w.weight(w.fixed(x)) : 0ull;
   };
   u64 mass = 0ull;
-  count = 0u;
-  for (int i = i0 + lane; i < i0 + seg; i += 32) {
-    bool in;
-    mass += weigh(i, in);
-    count += in;
-  }
+  unsigned count = 0u;
+  row.each([&](const unsigned (&x)[8], int id) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      bool in;
+      mass += weigh(x[e], id + e, in);
+      count += in;
+    }
+    return true;
+  });
   mass = warp_sum64(mass);
   count = __reduce_add_sync(0xffffffffu, count);
   __syncthreads();
@@ -490,8 +575,7 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(
     sh->wred2[warp] = count;
   }
   __syncthreads();
-  u64 all = 0ull, below = 0ull;
-  cnt = 0ull;
+  u64 all = 0ull, below = 0ull, cnt = 0ull;
   for (int i = 0; i < SM_WARPS; ++i) {
     if (i < warp) below += sh->wred[i];
     all += sh->wred[i];
@@ -509,26 +593,38 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(
   const u64 target = part_of(uv, total);
   if (below <= target && target < below + mass) {   // one warp of the cluster
     u64 at = below;
-    for (int i = i0 + lane; i < i0 + seg; i += 32) {
-      bool in;
-      const u64 wt = weigh(i, in);
-      u64 inc = wt;
+    row.each([&](const unsigned (&x)[8], int id) {
+      u64 wt[8], sum = 0ull;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bool in;
+        sum += wt[e] = weigh(x[e], id + e, in);
+      }
+      u64 inc = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += t;
       }
       const u64 tile = __shfl_sync(0xffffffffu, inc, 31);
-      if (target < at + tile) {
-        if (at + inc - wt <= target && target < at + inc) {
-          ids[row_i] = row.id0 + i;
-          if (kept) kept[row_i] = (int)n_kept;
-          if (prob) prob[row_i] = (float)((double)wt / (double)total);
-        }
-        break;
+      if (target >= at + tile) {
+        at += tile;
+        return true;
       }
-      at += tile;
-    }
+      u64 run = at + inc - sum;
+      if (run <= target && target < run + sum) {   // one lane
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (run <= target && target < run + wt[e]) {
+            ids[row_i] = id + e;
+            if (kept) kept[row_i] = (int)n_kept;
+            if (prob) prob[row_i] = (float)((double)wt[e] / (double)total);
+          }
+          run += wt[e];
+        }
+      }
+      return false;
+    });
   }
   c.sync();                              // no CTA leaves while a peer may still read or write its shared memory
 }
@@ -547,24 +643,26 @@ extern "C" int uttt_sample(int rows, int V, const void* logits, int logits_f32, 
   cudaStream_t st = (cudaStream_t)stream;
   ProfScope ps(UTTT_PROF_ARGMAX, st);
   const int lim = active_limit < V ? active_limit : V;
-  // split a row over a cluster while the rows alone leave SMs idle (at least 1024 logits per CTA), or while
-  // a CTA's part does not fit its shared memory
+  // a row is split over a cluster while the rows alone leave SMs idle (two CTAs fit an SM; at least 2048 logits per
+  // CTA), and where a CTA's part would be too large for the histogram's limbs
+  const int nvec = (lim + 7) / 8;
   int S = 1;
-  while (S < SM_MAX_CTAS && ((lim + S - 1) / S > 32768 || ((long long)rows * S < num_sms() && lim / (2 * S) >= 1024)))
+  while (S < SM_MAX_CTAS &&
+         ((lim + S - 1) / S > SM_MAX_PART || ((long long)rows * 2 * S <= 2 * num_sms() && lim / (2 * S) >= 2048)))
     S *= 2;
-  const int part = ((lim + S - 1) / S + 7) & ~7;
+  const int part = (nvec + S - 1) / S;
   auto kernel = logits_f32 ? sample_kernel<true> : sample_kernel<false>;
   static DeviceOnce attr;
   UTTT_TRY(run_once_per_device(attr, [] {
     UTTT_TRY(cuda_status(cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              32768 * 4)));
+                                              (int)sizeof(SampleShared))));
     return cuda_status(cudaFuncSetAttribute(sample_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            32768 * 4));
+                                            (int)sizeof(SampleShared)));
   }));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(S, rows);
   cfg.blockDim = dim3(SM_THREADS);
-  cfg.dynamicSmemBytes = (size_t)part * sizeof(unsigned);
+  cfg.dynamicSmemBytes = sizeof(SampleShared);
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -574,7 +672,7 @@ extern "C" int uttt_sample(int rows, int V, const void* logits, int logits_f32, 
   at[1] = pdl_attribute();
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, kernel, logits, ld, lim, part, stop_free, *opt, u, u_ld, u_index, u_len, ids, kept,
+  if (cudaLaunchKernelEx(&cfg, kernel, logits, ld, V, lim, part, stop_free, *opt, u, u_ld, u_index, u_len, ids, kept,
                          prob) != cudaSuccess)
     return launch_status();
   return launch_status();
