@@ -17,7 +17,9 @@
 // 2^(-j/128)) and the rest (a cubic Taylor polynomial: the table-driven method of
 // Tang, ACM TOMS 15, 1989), as a whole number of 2^-45, good to 2^-29 of itself
 // (all carry one common factor, 1 - 2^-20, which keeps the table within 32 bits
-// and leaves every ratio alone).  So every sum of weights is an exact 64-bit
+// and leaves every ratio alone).  Weights below 2^-24 take x and 2^-x from FP32
+// instead: off by 2^-19 of themselves, they are still good to 2^-43 of the largest.
+// So every sum of weights is an exact 64-bit
 // integer that does not depend on the order of the additions: histograms with
 // atomics, splits over CTAs and any grid give the same cut and the same pick.
 //
@@ -26,9 +28,12 @@
 // and stays in L1 / L2 for the others): (1) largest logit; (2) where top-k or top-p
 // ask for it, a histogram over 2048 bins of x, merged over the cluster in
 // distributed shared memory, and (3) the candidates of the bin that holds the cut,
-// ranked against each other; a bin with too many of them (equal or nearly equal
-// logits) is split again by the bits of its (key, id) pairs; (4) kept mass per
-// warp; the warp that holds the pick walks its piece again.
+// ranked against each other; of too many equal logits the last kept one is counted
+// off in id order, and a bin with too many nearly equal ones is split again by the
+// bits of its (key, id) pairs; (4) kept mass per warp; the warp that holds the pick
+// walks its piece again.  Weights below 2^-24 (a billionth of a percent of the mass
+// each) get no bin: what top-p asks for nearly always ends before them, and if it
+// does not, they are one bin that is split by the same steps.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -42,11 +47,12 @@ namespace {
 constexpr int SM_THREADS = 512;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr int SM_BINS = 2048;
-constexpr int SM_CAP = 256;              // candidates ranked against each other directly
+constexpr int SM_CAP = SM_THREADS;        // candidates ranked against each other directly, one per thread
+constexpr int SM_TAIL = SM_BINS;          // the bin of everything beyond SM_RANGE
 constexpr int SM_MAX_CTAS = 8;
 constexpr int SM_MAX_V = 262144;         // 8 CTAs of 32768 keys
 constexpr int SM_MAX_PART = 65536;       // ids per CTA: sums of as many 16-bit limbs stay below 2^32
-constexpr float SM_RANGE = 62.f;         // x from here on is the last bin; weights below 2^-46 are zero
+constexpr float SM_RANGE = 24.f;         // x up to here has bins (64 to the unit) and exact weights
 constexpr int SM_STEPS = 128;            // table entries per octave
 constexpr float SM_GREEDY_T = 1e-5f;     // _sample_next_token's greedy border
 
@@ -65,7 +71,7 @@ struct SampleShared {
   unsigned n_cand[2];                    // rank 0; gathers alternate between the two lists
   u64 res_base, res_cut;
   int res_bin;
-  unsigned hist[3][SM_BINS];             // count, or 16-bit limbs of the mass
+  alignas(16) unsigned hist[3][SM_BINS];  // count, or 16-bit limbs of the mass
 };
 
 // floor(2^32 * 2^(-j / 128) * (1 - 2^-20))
@@ -114,13 +120,12 @@ struct Weigher {
   float mf, cf;
   bool top_inf;         // the largest logit is +inf: only its equals have weight
   const unsigned* tab;  // this lane's copy
-  // whether x is in range (else the element is in the last bin and has no weight)
-  __device__ __forceinline__ bool in_range(unsigned bits) const {
-    const float s = __uint_as_float(bits);
-    if (top_inf) return bits == 0x7f800000u;
-    return (mf - s) * cf <= SM_RANGE;    // not for NaN and -inf
+  // x in FP32; NaN or infinite for what has no weight
+  __device__ __forceinline__ float rough(unsigned bits) const {
+    if (top_inf) return bits == 0x7f800000u ? 0.f : INFINITY;
+    return (mf - __uint_as_float(bits)) * cf;
   }
-  // x >= 0 of an element in range
+  // x >= 0
   __device__ __forceinline__ double exponent(unsigned bits) const {
     return top_inf ? 0.0 : (m - widen(bits)) * c;
   }
@@ -129,8 +134,8 @@ struct Weigher {
     const double t = x + 1048576.0;      // 2^20: the last place is 2^-32
     return make_uint2((unsigned)__double2loint(t), (unsigned)__double2hiint(t) & 0xfffffu);
   }
-  // 1/32 wide bins of x
-  __device__ __forceinline__ int bin(uint2 x) const { return (int)__funnelshift_l(x.x, x.y, 5); }
+  // 1/64 wide bins of x
+  __device__ __forceinline__ int bin(uint2 x) const { return (int)__funnelshift_l(x.x, x.y, 6); }
   // 2^-x in units of 2^-45
   __device__ __forceinline__ u64 weight(uint2 x) const {
     const unsigned t = tab[(x.x >> 25) * 32];
@@ -141,14 +146,21 @@ struct Weigher {
     // its mantissa bits behind 2^-7 are q in units of 2^-30
     const unsigned qi = __float_as_uint(q + 0.0078125f) & 0x7fffffu;
     const unsigned w = t - __umulhi(t, qi << 2);
-    const int sh = 13 - (int)x.y;
+    const int sh = 13 - (int)x.y;        // x <= 25 here
     if (sh >= 0) return (u64)w << sh;
-    return sh < -32 ? 0ull : (u64)(((w >> (-sh - 1)) + 1u) >> 1);
+    return (u64)(((w >> (-sh - 1)) + 1u) >> 1);
   }
-  __device__ __forceinline__ u64 weight_of(unsigned key) const {
-    const unsigned bits = __float_as_uint(key_value(key));
-    return in_range(bits) ? weight(fixed(exponent(bits))) : 0ull;
+  // 2^-x in units of 2^-45 for rough x > SM_RANGE (0 for NaN and infinities): below 2^21, so that adding 2^23 rounds it
+  // to a whole number in the mantissa
+  __device__ __forceinline__ unsigned tail_weight(float y) const {
+    return y < 64.f ? __float_as_uint(exp2f(45.f - y) + 8388608.f) & 0x7fffffu : 0u;
   }
+  __device__ __forceinline__ u64 weight_of(unsigned bits) const {
+    const float y = rough(bits);
+    return y <= SM_RANGE ? weight(fixed(exponent(bits))) : (u64)tail_weight(y);
+  }
+  // the same by key
+  __device__ __forceinline__ u64 weight_of_key(unsigned key) const { return weight_of(__float_as_uint(key_value(key))); }
 };
 
 __device__ __forceinline__ u64 warp_sum64(u64 v) {
@@ -163,6 +175,13 @@ __device__ __forceinline__ u64 warp_max64(u64 v) {
     v = t > v ? t : v;
   }
   return v;
+}
+
+// the larger number, subnormal ones too (the compiler's own flag would flush them); a NaN loses
+__device__ __forceinline__ float max_exact(float a, float b) {
+  float r;
+  asm("max.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 // floor(x * total) for x in [0, 1): exact for every x >= 2^-40
@@ -292,7 +311,7 @@ __device__ u64 rank_candidates(Cluster& c, unsigned n, int mode, u64 target, con
   if (threadIdx.x == 0) sh->res_cut = 0ull;
   if (threadIdx.x < n) {
     mine = cand[threadIdx.x];
-    own = mode == FIND_COUNT ? 1ull : w.weight_of((unsigned)(mine >> 32));
+    own = mode == FIND_COUNT ? 1ull : w.weight_of_key((unsigned)(mine >> 32));
     sh->cand_w[threadIdx.x] = own;
   }
   __syncthreads();
@@ -306,19 +325,150 @@ __device__ u64 rank_candidates(Cluster& c, unsigned n, int mode, u64 target, con
   return sh->res_cut;
 }
 
+// The merged histogram's bin that holds `target` and what lies before it, the same in every CTA.  *total: of all bins.
+// With top_p > 0 the target is that part of *total + more (mass), and written back.  The bin is -1 if the target
+// lies behind all bins.
+__device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, u64& base_out, u64& total) {
+  SampleShared* sh = c.sh;
+  c.sync();
+  // this CTA sums its share of the bins over the cluster: thread t has PB consecutive ones
+  constexpr int Q = SM_BINS / SM_THREADS;
+  const int share = SM_BINS / c.S, b0 = c.rank * share, PB = (share + SM_THREADS - 1) / SM_THREADS;
+  u64 val[Q], sum = 0ull;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    val[q] = 0ull;
+    const int bl = threadIdx.x * PB + q;
+    if (q < PB && bl < share)
+      for (int r = 0; r < c.S; ++r) {
+        const SampleShared* p = c.peer(r);
+        val[q] += p->hist[0][b0 + bl];
+        if (mode == FIND_MASS) val[q] += ((u64)p->hist[1][b0 + bl] << 16) + ((u64)p->hist[2][b0 + bl] << 32);
+      }
+    sum += val[q];
+  }
+  u64 inc = sum;                         // prefix over the CTA's threads
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
+    if ((threadIdx.x & 31) >= o) inc += t;
+  }
+  more = warp_sum64(more);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 31) {
+    sh->wred[threadIdx.x >> 5] = inc;
+    sh->wred2[threadIdx.x >> 5] = more;
+  }
+  __syncthreads();
+  u64 base = 0ull, mine = 0ull;
+  more = 0ull;
+  for (int i = 0; i < SM_WARPS; ++i) {
+    if (i < (int)(threadIdx.x >> 5)) base += sh->wred[i];
+    mine += sh->wred[i];
+    more += sh->wred2[i];
+  }
+  if (threadIdx.x == 0) sh->res_bin = -1;
+  const int ph = c.exchange(Sel{mine, more});
+  total = 0ull;
+  more = 0ull;
+  for (int r = 0; r < c.S; ++r) {
+    if (r < c.rank) base += sh->xch[ph][r].a;
+    total += sh->xch[ph][r].a;
+    more += sh->xch[ph][r].b;
+  }
+  if (top_p > 0.f) target = part_of(top_p, total + more);
+  u64 at = base + inc - sum;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    if (at <= target && at + val[q] > target)
+      for (int r = 0; r < c.S; ++r) {
+        SampleShared* p = c.peer(r);
+        p->res_bin = b0 + threadIdx.x * PB + q;
+        p->res_base = at;
+      }
+    at += val[q];
+  }
+  c.sync();
+  base_out = sh->res_base;
+  return sh->res_bin;
+}
+
+__device__ __forceinline__ void add_mass(SampleShared* sh, int bin, u64 wt) {
+  const unsigned l0 = (unsigned)wt & 0xffffu, l1 = (unsigned)wt >> 16, l2 = (unsigned)(wt >> 32);
+  if (l0) atomicAdd(&sh->hist[0][bin], l0);
+  if (l1) atomicAdd(&sh->hist[1][bin], l1);
+  if (l2) atomicAdd(&sh->hist[2][bin], l2);
+}
+
+__device__ __forceinline__ void clear_hist(SampleShared* sh) {
+  uint4* h = reinterpret_cast<uint4*>(&sh->hist[0][0]);
+  for (int i = threadIdx.x; i < 3 * SM_BINS / 4; i += SM_THREADS) h[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+}
+
+// The pair of the n-th (from 0, by id) candidate with this key; there are more than n of them.
+__device__ u64 nth_equal(Cluster& c, const Row& row, unsigned key, u64 n) {
+  SampleShared* sh = c.sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned count = 0u;
+  row.each([&](const unsigned (&x)[8], int) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) count += order_key(x[e]) == key;
+    return true;
+  });
+  count = __reduce_add_sync(0xffffffffu, count);
+  __syncthreads();
+  if (lane == 0) sh->wred[warp] = count;
+  __syncthreads();
+  u64 below = 0ull, all = 0ull;
+  for (int i = 0; i < SM_WARPS; ++i) {
+    if (i < warp) below += sh->wred[i];
+    all += sh->wred[i];
+  }
+  const int ph = c.exchange(Sel{all, 0ull});
+  for (int r = 0; r < c.rank; ++r) below += sh->xch[ph][r].a;
+  if (below <= n && n < below + count) {   // one warp of the cluster
+    u64 at = below;
+    row.each([&](const unsigned (&x)[8], int id) {
+      unsigned mine = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mine += order_key(x[e]) == key;
+      unsigned inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+      }
+      const unsigned tile = __shfl_sync(0xffffffffu, inc, 31);
+      if (n >= at + tile) {
+        at += tile;
+        return true;
+      }
+      u64 run = at + inc - mine;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (order_key(x[e]) == key && run++ == n)
+          for (int r = 0; r < c.S; ++r) c.peer(r)->res_cut = pair_of(key, id + e);
+      return false;
+    });
+  }
+  c.sync();
+  return sh->res_cut;
+}
+
 // Last element of the kept prefix among the pairs >= cut: the first one, in the order, whose count or mass up
 // to and with it exceeds the target (count - 1, or top_p of the whole mass).  Returns `cut` if nothing does.
-__device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, int mode, u64 count_target, float top_p,
-                        u64 cut, unsigned n_eligible) {
+template <int MODE>
+__device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, u64 target, float top_p, u64 cut,
+                        unsigned n_eligible) {
   SampleShared* sh = c.sh;
   if (n_eligible <= SM_CAP) {            // few enough to rank at once
     const unsigned n = gather(c, row, [&](unsigned bits, int id) {
       const unsigned key = order_key(bits);
       return is_candidate(key) && pair_of(key, id) >= cut;
     });
-    u64 target = count_target;
-    if (mode == FIND_MASS) {
-      u64 v = threadIdx.x < n ? w.weight_of((unsigned)(sh->cand[c.list][threadIdx.x] >> 32)) : 0ull;
+    if (MODE == FIND_MASS) {
+      u64 v = threadIdx.x < n ? w.weight_of_key((unsigned)(sh->cand[c.list][threadIdx.x] >> 32)) : 0ull;
       v = warp_sum64(v);
       __syncthreads();
       if ((threadIdx.x & 31) == 0) sh->wred[threadIdx.x >> 5] = v;
@@ -327,125 +477,71 @@ __device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, int mode, 
       for (int i = 0; i < SM_WARPS; ++i) total += sh->wred[i];
       target = part_of(top_p, total);
     }
-    const u64 r = rank_candidates(c, n, mode, target, w);
+    const u64 r = rank_candidates(c, n, MODE, target, w);
     return r ? r : cut;
   }
-  // pass 0 bins by the exponent, later passes by the pair's bits in [lo, hi]
-  u64 lo = 0ull, hi = ~0ull, target = count_target;
-  int sh_bits = -1;
-  for (int pass = 0; pass < 10; ++pass) {
-    for (int i = threadIdx.x; i < 3 * SM_BINS; i += SM_THREADS) (&sh->hist[0][0])[i] = 0u;
-    __syncthreads();
+  clear_hist(sh);
+  u64 more = 0ull, base, total;
+  const unsigned cut_key = (unsigned)(cut >> 32);
+  row.each([&](const unsigned (&x)[8], int id) {
     unsigned tail = 0u;
-    row.each([&](const unsigned (&x)[8], int id) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bool in = w.in_range(x[e]);
-        int bin;
-        uint2 fx;
-        if (sh_bits >= 0 || cut != 0ull || !in) {   // anything but the first pass over a whole row
-          const unsigned key = order_key(x[e]);
-          const u64 pr = pair_of(key, id + e);
-          if (!is_candidate(key) || pr < cut || pr < lo || pr > hi) continue;
-          bin = sh_bits >= 0 ? (int)((hi - pr) >> sh_bits) : SM_BINS - 1;
-        }
-        if (in) {
-          fx = w.fixed(w.exponent(x[e]));
-          if (sh_bits < 0) bin = w.bin(fx);
-        }
-        if (mode == FIND_COUNT) {
-          if (sh_bits < 0 && !in)
-            ++tail;                      // the far tail is one bin: counted in registers
-          else
-            atomicAdd(&sh->hist[0][bin], 1u);
-        } else if (in) {
-          const u64 wt = w.weight(fx);
-          const unsigned l0 = (unsigned)wt & 0xffffu, l1 = (unsigned)wt >> 16, l2 = (unsigned)(wt >> 32);
-          if (l0) atomicAdd(&sh->hist[0][bin], l0);
-          if (l1) atomicAdd(&sh->hist[1][bin], l1);
-          if (l2) atomicAdd(&sh->hist[2][bin], l2);
-        }
+    for (int e = 0; e < 8; ++e) {
+      const float y = w.rough(x[e]);
+      if (cut_key) {                     // a cut from top-k
+        const unsigned key = order_key(x[e]);
+        if (key < cut_key || pair_of(key, id + e) < cut) continue;
       }
-      return true;
-    });
-    if (mode == FIND_COUNT) {
-      const unsigned t = __reduce_add_sync(0xffffffffu, tail);
-      if ((threadIdx.x & 31) == 0 && t) atomicAdd(&sh->hist[0][SM_BINS - 1], t);
+      if (y <= SM_RANGE) {
+        const uint2 fx = w.fixed(w.exponent(x[e]));
+        if (MODE == FIND_COUNT)
+          atomicAdd(&sh->hist[0][w.bin(fx)], 1u);
+        else
+          add_mass(sh, w.bin(fx), w.weight(fx));
+      } else if (MODE == FIND_MASS) {
+        tail += w.tail_weight(y);
+      }
     }
-    c.sync();
-    // this CTA sums its share of the bins over the cluster: thread t has PB consecutive ones
-    const int share = SM_BINS / c.S, b0 = c.rank * share;
-    const int PB = (share + SM_THREADS - 1) / SM_THREADS;
-    u64 val[SM_BINS / SM_THREADS], sum = 0ull;
-#pragma unroll
-    for (int q = 0; q < SM_BINS / SM_THREADS; ++q) {
-      val[q] = 0ull;
-      const int bl = threadIdx.x * PB + q;
-      if (q < PB && bl < share)
-        for (int r = 0; r < c.S; ++r) {
-          const SampleShared* p = c.peer(r);
-          val[q] += p->hist[0][b0 + bl];
-          if (mode == FIND_MASS) val[q] += ((u64)p->hist[1][b0 + bl] << 16) + ((u64)p->hist[2][b0 + bl] << 32);
-        }
-      sum += val[q];
-    }
-    // exclusive prefix over the CTA's threads
-    u64 inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
-      if ((threadIdx.x & 31) >= o) inc += t;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 31) sh->wred[threadIdx.x >> 5] = inc;
-    __syncthreads();
-    u64 base = 0ull, mine = 0ull;
-    for (int i = 0; i < SM_WARPS; ++i) {
-      if (i < (int)(threadIdx.x >> 5)) base += sh->wred[i];
-      mine += sh->wred[i];
-    }
-    if (threadIdx.x == 0) sh->res_bin = -1;
-    const int ph = c.exchange(Sel{mine, 0ull});
-    u64 total = 0ull;
-    for (int r = 0; r < c.S; ++r) {
-      if (r < c.rank) base += sh->xch[ph][r].a;
-      total += sh->xch[ph][r].a;
-    }
-    if (mode == FIND_MASS && pass == 0) target = part_of(top_p, total);
-    u64 at = base + inc - sum;
-#pragma unroll
-    for (int q = 0; q < SM_BINS / SM_THREADS; ++q) {
-      if (at <= target && at + val[q] > target)
-        for (int r = 0; r < c.S; ++r) {
-          SampleShared* p = c.peer(r);
-          p->res_bin = b0 + threadIdx.x * PB + q;
-          p->res_base = at;
-        }
-      at += val[q];
-    }
-    c.sync();
-    const int bin = sh->res_bin;
-    if (bin < 0) return cut;             // everything is within the target
-    target -= sh->res_base;
-    u64 mn = ~0ull, mx = 0ull;
-    const unsigned n = gather(c, row, [&](unsigned bits, int id) {
-      const bool in = w.in_range(bits);
-      if (sh_bits < 0 && (in ? w.bin(w.fixed(w.exponent(bits))) : SM_BINS - 1) != bin) return false;
-      const unsigned key = order_key(bits);
-      const u64 pr = pair_of(key, id);
-      if (!is_candidate(key) || pr < cut || pr < lo || pr > hi) return false;
-      if (sh_bits >= 0 && (int)((hi - pr) >> sh_bits) != bin) return false;
-      mn = pr < mn ? pr : mn;
-      mx = pr > mx ? pr : mx;
-      return true;
-    });
+    more += tail;
+    return true;
+  });
+  int bin = locate(c, MODE, MODE == FIND_MASS ? top_p : 0.f, more, target, base, total);
+  if (bin < 0) {
+    bin = SM_TAIL;
+    base = total;
+  }
+  target -= base;
+  // FP32's x is off by less than 2^-18 up to SM_RANGE: most elements are told apart from the bin by it
+  const float y0 = bin == SM_TAIL ? SM_RANGE : (float)bin * (1.f / 64.f) - 1e-5f;
+  const float y1 = bin == SM_TAIL ? INFINITY : (float)(bin + 1) * (1.f / 64.f) + 1e-5f;
+  u64 mn = ~0ull, mx = 0ull, lo = 0ull, hi = ~0ull;
+  auto take = [&](unsigned bits, int id, u64& pr) {   // a candidate within the cut and [lo, hi]
+    const unsigned key = order_key(bits);
+    pr = pair_of(key, id);
+    return is_candidate(key) && pr >= cut && pr >= lo && pr <= hi;
+  };
+  auto span = [&](u64 pr) {
+    mn = pr < mn ? pr : mn;
+    mx = pr > mx ? pr : mx;
+    return true;
+  };
+  unsigned n = gather(c, row, [&](unsigned bits, int id) {
+    const float y = w.rough(bits);
+    u64 pr;
+    if (bin == SM_TAIL) return !(y <= SM_RANGE) && take(bits, id, pr) && span(pr);
+    return y >= y0 && y <= y1 && y <= SM_RANGE && w.bin(w.fixed(w.exponent(bits))) == bin && take(bits, id, pr) &&
+           span(pr);
+  });
+  bool sure = bin != SM_TAIL;            // whether the bin is known to hold the cut
+  bool whole = true;                     // whether it holds all candidates of a key, or none
+  for (int pass = 0; pass < 10; ++pass) {
     if (n <= SM_CAP) {
-      const u64 r = rank_candidates(c, n, mode, target, w);
+      const u64 r = rank_candidates(c, n, MODE, target, w);
       return r ? r : cut;
     }
-    // split the bin again: the range of the pairs that are in it
     mx = warp_max64(mx);
     mn = ~warp_max64(~mn);
+    __syncthreads();
     if ((threadIdx.x & 31) == 0) {
       sh->wred[threadIdx.x >> 5] = mx;
       sh->wred2[threadIdx.x >> 5] = mn;
@@ -455,17 +551,57 @@ __device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, int mode, 
       mx = sh->wred[i] > mx ? sh->wred[i] : mx;
       mn = sh->wred2[i] < mn ? sh->wred2[i] : mn;
     }
-    const int p2 = c.exchange(Sel{mx, mn});
+    const int ph = c.exchange(Sel{mx, mn});
     for (int r = 0; r < c.S; ++r) {
-      mx = sh->xch[p2][r].a > mx ? sh->xch[p2][r].a : mx;
-      mn = sh->xch[p2][r].b < mn ? sh->xch[p2][r].b : mn;
+      mx = sh->xch[ph][r].a > mx ? sh->xch[ph][r].a : mx;
+      mn = sh->xch[ph][r].b < mn ? sh->xch[ph][r].b : mn;
     }
-    lo = mn;
-    hi = mx;
-    const int bits = 64 - __clzll((long long)(hi - lo));
-    sh_bits = bits > 11 ? bits - 11 : 0;   // (hi - lo) >> sh_bits < 2048
+    const unsigned k0 = (unsigned)(mn >> 32), k1 = (unsigned)(mx >> 32);
+    int sh_bits;
+    if (k0 == k1 && sure && whole && k0 != cut_key) {
+      // equal logits: the first ones by id are kept
+      const u64 each = MODE == FIND_COUNT ? 1ull : w.weight_of_key(k0);
+      return nth_equal(c, row, k0, target / each);
+    }
+    if (k0 != k1 && whole) {             // by keys, then (rarely) by ids
+      lo = pair_of(k0, 0xffffffffu);
+      hi = pair_of(k1, 0u);
+      sh_bits = 32 + max(0, 21 - __clz((int)(k1 - k0)));   // (k1 - k0) >> (sh_bits - 32) < 2048
+    } else {
+      lo = mn;
+      hi = mx;
+      sh_bits = max(0, 53 - __clzll((long long)(hi - lo)));
+      whole = false;
+    }
+    clear_hist(sh);
+    row.each([&](const unsigned (&x)[8], int id) {
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        unsigned xe = x[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) xe = e == k ? x[k] : xe;
+        u64 pr;
+        if (!take(xe, id + e, pr)) continue;
+        const int at = (int)((hi - pr) >> sh_bits);
+        if (MODE == FIND_COUNT)
+          atomicAdd(&sh->hist[0][at], 1u);
+        else
+          add_mass(sh, at, w.weight_of(xe));
+      }
+      return true;
+    });
+    bin = locate(c, MODE, 0.f, 0ull, target, base, total);
+    if (bin < 0) return cut;             // everything is within the target
+    sure = true;
+    target -= base;
+    mn = ~0ull;
+    mx = 0ull;
+    n = gather(c, row, [&](unsigned bits_e, int id) {
+      u64 pr;
+      return take(bits_e, id, pr) && (int)((hi - pr) >> sh_bits) == bin && span(pr);
+    });
   }
-  return cut;                              // not reached: every pass leaves 1/2048 of a range of 2^64 pairs
+  return cut;                            // not reached: a pass leaves 1/2048 of the range of keys, then of ids
 }
 
 template <bool F32>
@@ -493,23 +629,23 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   const int end = min((c.rank + 1) * part, (lim + 7) / 8), per = ((part + SM_WARPS - 1) / SM_WARPS + 31) & ~31;
   row.v0 = min(end, c.rank * part + warp * per);
   row.v1 = min(end, row.v0 + per);
-  u64 best = 0ull;
-  row.each([&](const unsigned (&x)[8], int id) {
+  float top = -INFINITY;
+  row.each([&](const unsigned (&x)[8], int) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned k = order_key(x[e]);
-      if (k > (unsigned)(best >> 32) && k <= kInfKey) best = pair_of(k, id + e);   // ids rise: the first stays
-    }
+    for (int e = 0; e < 8; ++e) top = max_exact(top, __uint_as_float(x[e]));   // NaN loses
     return true;
   });
-  best = warp_max64(best);
-  if (lane == 0) sh->wred[warp] = best;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max_exact(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) sh->wred[warp] = order_key(__float_as_uint(top));
   __syncthreads();
+  u64 best = 0ull;
   for (int i = 0; i < SM_WARPS; ++i) best = sh->wred[i] > best ? sh->wred[i] : best;
   c.wait();
   const int ph = c.exchange(Sel{best, 0ull});
   for (int r = 0; r < c.S; ++r) best = sh->xch[ph][r].a > best ? sh->xch[ph][r].a : best;
-  if (!is_candidate((unsigned)(best >> 32))) {   // nothing to choose from: an allowed id, as the greedy pick gives
+  const unsigned mkey = (unsigned)best;
+  if (!is_candidate(mkey)) {   // nothing to choose from: an allowed id, as the greedy pick gives
     if (c.rank == 0 && tid == 0) {
       ids[row_i] = (stop_free ? 6 : 2) % lim;
       if (kept) kept[row_i] = 0;
@@ -526,7 +662,6 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   const bool greedy = !(T > SM_GREEDY_T) || top_k == 1;
   if (greedy) T = 1.f;
   Weigher w;
-  const unsigned mkey = (unsigned)(best >> 32);
   w.mf = key_value(mkey);
   w.m = widen(__float_as_uint(w.mf));
   w.top_inf = mkey == kInfKey;
@@ -535,26 +670,32 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   w.tab = sh->tab + lane;
   u64 cut = 0ull;
   if (greedy) {
-    cut = best;
+    cut = nth_equal(c, row, mkey, 0ull);
   } else {
     unsigned eligible = (unsigned)lim;
     if (top_k > 0 && top_k < lim) {
-      cut = find_cut(c, row, w, FIND_COUNT, (u64)(top_k - 1), 0.f, cut, eligible);
+      cut = find_cut<FIND_COUNT>(c, row, w, (u64)(top_k - 1), 0.f, cut, eligible);
       eligible = (unsigned)top_k;
     }
-    if (top_p < 1.f) cut = find_cut(c, row, w, FIND_MASS, 0ull, top_p, cut, eligible);
+    if (top_p < 1.f) cut = find_cut<FIND_MASS>(c, row, w, 0ull, top_p, cut, eligible);
   }
   const double x_max = min_p > 0.f ? -log2((double)fminf(min_p, 1.f)) : INFINITY;
   // ---- kept mass per warp
   const unsigned cut_key = max((unsigned)(cut >> 32), 0x00800000u);
   auto weigh = [&](unsigned bits, int id, bool& in) -> u64 {
     const unsigned key = order_key(bits);
-    in = key >= cut_key && key <= kInfKey && pair_of(key, id) >= cut;
+    in = key >= cut_key && key <= kInfKey;
     if (!in) return 0ull;
-    const bool near = w.in_range(bits);
-    const double x = near ? w.exponent(bits) : 1e300;
+    in = pair_of(key, id) >= cut;
+    if (!in) return 0ull;
+    const float y = w.rough(bits);
+    if (!(y <= SM_RANGE)) {
+      in = x_max == INFINITY || (double)y <= x_max;   // min_p below 2^-24
+      return in ? (u64)w.tail_weight(y) : 0ull;
+    }
+    const double x = w.exponent(bits);
     in = x <= x_max;
-    return near && in ? w.weight(w.fixed(x)) : 0ull;
+    return in ? w.weight(w.fixed(x)) : 0ull;
   };
   u64 mass = 0ull;
   unsigned count = 0u;
