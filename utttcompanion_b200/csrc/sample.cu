@@ -48,6 +48,7 @@ constexpr int SM_THREADS = 512;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr int SM_BINS = 2048;
 constexpr int SM_CAP = SM_THREADS;        // candidates ranked against each other directly, one per thread
+constexpr int SM_RING = 4;               // 16-byte vectors on their way per lane
 constexpr int SM_TAIL = SM_BINS;          // the bin of everything beyond SM_RANGE
 constexpr int SM_MAX_CTAS = 8;
 constexpr int SM_MAX_V = 262144;         // 8 CTAs of 32768 keys
@@ -63,6 +64,7 @@ struct Sel {     // value exchanged between the CTAs of a cluster
 };
 
 struct SampleShared {
+  uint4 ring[SM_WARPS][SM_RING * 32];    // vectors on their way
   unsigned tab[SM_STEPS * 32];           // the table once per lane: no bank conflicts
   Sel xch[2][SM_MAX_CTAS];               // one slot per CTA, two phases
   u64 wred[SM_WARPS], wred2[SM_WARPS];
@@ -219,50 +221,68 @@ struct Cluster {
 
 enum { FIND_COUNT, FIND_MASS };
 
+// 8 logits from id i on, one by one (rows that do not start on 16 bytes, and the end of a row)
+struct Eight {
+  unsigned x[8];
+};
+template <bool F32>
+__device__ __noinline__ Eight load_scalar(const char* src, int i, int V) {
+  Eight r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int k = min(i + e, V - 1);     // what lies behind the row is masked by the caller
+    r.x[e] = F32 ? __ldg(reinterpret_cast<const unsigned*>(src) + k)
+                 : (unsigned)__ldg(reinterpret_cast<const unsigned short*>(src) + k) << 16;
+  }
+  return r;
+}
+
 // A row's piece of one warp: 8-logit vectors v0 .. v1 - 1, the lanes side by side.
+template <bool F32>
 struct Row {
   const char* src;        // the row
-  bool f32, vec;          // its type; whether it starts on 16 bytes
+  bool vec;               // whether it starts on 16 bytes
   int V, lim, stop_free;
   int v0, v1;
+  uint4* ring;            // the warp's places in shared memory
 
-  __device__ __forceinline__ void load(int v, uint4& a, uint4& b) const {
-    if (vec && v * 8 + 8 <= V) {
-      const uint4* p = reinterpret_cast<const uint4*>(src) + (size_t)v * (f32 ? 2 : 1);
-      a = __ldg(p);
-      if (f32) b = __ldg(p + 1);
-      return;
-    }
-    unsigned x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = min(v * 8 + e, V - 1);   // what lies behind the row is masked below
-      x[e] = f32 ? __ldg(reinterpret_cast<const unsigned*>(src) + i)
-                 : (unsigned)__ldg(reinterpret_cast<const unsigned short*>(src) + i);
-    }
-    if (f32) {
-      a = make_uint4(x[0], x[1], x[2], x[3]);
-      b = make_uint4(x[4], x[5], x[6], x[7]);
-    } else {
-      a = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
-    }
-  }
-  // f(bits[8], first id) for every vector of the piece, in step over the warp; ids that are never picked come as -inf
+  // f(bits[8], first id) for every vector of the piece, in step over the warp, until it returns false; ids that are
+  // never picked come as -inf.  Vectors arrive by cp.async, each lane's own ones in its own places, a few ahead.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
     const int lane = threadIdx.x & 31;
-    uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    if (v0 + lane < v1) load(v0 + lane, a, b);
+    constexpr int ahead = F32 ? SM_RING / 2 : SM_RING;
+    auto place = [&](int v) { return ring + ((v - v0) / 32 % ahead * (F32 ? 2 : 1)) * 32 + lane; };
+    auto fetch = [&](int v) {
+      if (vec && v < v1 && v * 8 + 8 <= V) {
+        const uint4* p = reinterpret_cast<const uint4*>(src) + (size_t)v * (F32 ? 2 : 1);
+        cp_async_16(place(v), p, true);
+        if (F32) cp_async_16(place(v) + 32, p + 1, true);
+      }
+      cp_async_commit();
+    };
+#pragma unroll 1
+    for (int k = 0; k < ahead - 1; ++k) fetch(v0 + lane + k * 32);
+#pragma unroll 1
     for (int t = v0; t < v1; t += 32) {
       const int v = t + lane;
+      fetch(v + (ahead - 1) * 32);
+      cp_async_wait<ahead - 1>();
       unsigned x[8];
-      if (f32) {
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+      if (vec && v * 8 + 8 <= V) {
+        const uint4 a = *place(v);       // (an old one where v is behind the piece)
+        if (F32) {
+          const uint4 b = place(v)[32];
+          x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+          x[0] = a.x << 16, x[1] = a.x & 0xffff0000u, x[2] = a.y << 16, x[3] = a.y & 0xffff0000u;
+          x[4] = a.z << 16, x[5] = a.z & 0xffff0000u, x[6] = a.w << 16, x[7] = a.w & 0xffff0000u;
+        }
       } else {
-        x[0] = a.x << 16, x[1] = a.x & 0xffff0000u, x[2] = a.y << 16, x[3] = a.y & 0xffff0000u;
-        x[4] = a.z << 16, x[5] = a.z & 0xffff0000u, x[6] = a.w << 16, x[7] = a.w & 0xffff0000u;
+        const Eight r = load_scalar<F32>(src, min(v, v1 - 1) * 8, V);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = r.x[e];
       }
-      if (v + 32 < v1) load(v + 32, a, b);
       if (v == 0 || v >= v1 || v * 8 + 8 > lim) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -270,8 +290,9 @@ struct Row {
           if (v >= v1 || id >= lim || id == 0 || id == 1 || id == 3 || (stop_free && id < 6)) x[e] = 0xff800000u;
         }
       }
-      if (!f(x, v * 8)) return;
+      if (!f(x, v * 8)) break;
     }
+    cp_async_wait<0>();                  // the places are free for the next walk
   }
 };
 
@@ -279,8 +300,8 @@ struct Row {
 // then holds a copy in cand[c.list] if they are at most SM_CAP.  Consecutive gathers use the two lists in turn, so
 // a CTA may start the next one while another still ranks this one's; the other list's counter is cleared between
 // this gather's two barriers, after its last reader and before its next writer.
-template <class InRange>
-__device__ unsigned gather(Cluster& c, const Row& row, InRange in_range) {
+template <bool F32, class InRange>
+__device__ unsigned gather(Cluster& c, const Row<F32>& row, InRange in_range) {
   SampleShared* lead = c.peer(0);
   const int q = c.list ^= 1;
   row.each([&](const unsigned (&x)[8], int id) {
@@ -407,7 +428,8 @@ __device__ __forceinline__ void clear_hist(SampleShared* sh) {
 }
 
 // The pair of the n-th (from 0, by id) candidate with this key; there are more than n of them.
-__device__ u64 nth_equal(Cluster& c, const Row& row, unsigned key, u64 n) {
+template <bool F32>
+__device__ u64 nth_equal(Cluster& c, const Row<F32>& row, unsigned key, u64 n) {
   SampleShared* sh = c.sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned count = 0u;
@@ -458,8 +480,8 @@ __device__ u64 nth_equal(Cluster& c, const Row& row, unsigned key, u64 n) {
 
 // Last element of the kept prefix among the pairs >= cut: the first one, in the order, whose count or mass up
 // to and with it exceeds the target (count - 1, or top_p of the whole mass).  Returns `cut` if nothing does.
-template <int MODE>
-__device__ u64 find_cut(Cluster& c, const Row& row, const Weigher& w, u64 target, float top_p, u64 cut,
+template <int MODE, bool F32>
+__device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 target, float top_p, u64 cut,
                         unsigned n_eligible) {
   SampleShared* sh = c.sh;
   if (n_eligible <= SM_CAP) {            // few enough to rank at once
@@ -619,13 +641,13 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   pdl_wait();
   pdl_trigger();
   // ---- the warp's piece of the row (`part` 8-logit vectors per CTA)
-  Row row;
+  Row<F32> row;
   row.src = reinterpret_cast<const char*>(logits) + (size_t)row_i * ld * (F32 ? 4 : 2);
-  row.f32 = F32;
   row.vec = (reinterpret_cast<uintptr_t>(row.src) & 15u) == 0;
   row.V = V;
   row.lim = lim;
   row.stop_free = stop_free;
+  row.ring = sh->ring[warp];
   const int end = min((c.rank + 1) * part, (lim + 7) / 8), per = ((part + SM_WARPS - 1) / SM_WARPS + 31) & ~31;
   row.v0 = min(end, c.rank * part + warp * per);
   row.v1 = min(end, row.v0 + per);

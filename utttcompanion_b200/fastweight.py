@@ -10,6 +10,7 @@ CPU tensors raise ``ValueError``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
 from typing import Dict, Optional, Tuple
@@ -49,6 +50,18 @@ def workspace(nbytes: int, device: torch.device, slot: int = 0) -> torch.Tensor:
 
 def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_same_device = contextlib.nullcontext()
+
+
+def _launch(device: torch.device):
+    """(context manager, raw current stream) for a launch on ``device``, whichever device is current.  A call
+    of a few microseconds on the GPU waits for its host side, so this avoids the usual objects where it can."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        return _same_device, torch._C._cuda_getCurrentRawStream(index)
+    return torch.cuda.device(device), torch.cuda.current_stream(device).cuda_stream
 
 
 def _require_cuda(*tensors):

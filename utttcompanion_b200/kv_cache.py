@@ -12,12 +12,12 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .fastweight import _require_cuda
+from .fastweight import _launch, _require_cuda
 from .tree import MAX_NODES, _int_rows
 
 
 def _check_rings(rings: torch.Tensor) -> None:
-    if rings.dim() != 6 or rings.shape[0] != 2 or rings.dtype != torch.bfloat16 or not rings.is_contiguous() \
+    if rings.dim() != 6 or rings.shape[0] != 2 or rings.dtype is not torch.bfloat16 or not rings.is_contiguous() \
             or 0 in rings.shape:
         raise ValueError("rings must be contiguous BF16 (2, layers, slots, n_kv, W, hd)")
 
@@ -42,10 +42,11 @@ def ring_commit(rings: torch.Tensor, tree_kv: torch.Tensor, pos: torch.Tensor, s
         return
     tree_stride, ring_stride = B * n_kv * N * hd, S * n_kv * W * hd
     t, r = tree_kv.data_ptr(), rings.data_ptr()
-    with torch.cuda.device(dev):
+    on, stream = _launch(dev)
+    with on:
         st = _lib.load().uttt_kv_ring_commit(L, B, N, n_kv, hd, W, S, t, t + 2 * L * tree_stride, tree_stride, r,
                                              r + 2 * L * ring_stride, ring_stride, *ptrs,
-                                             torch.cuda.current_stream(dev).cuda_stream)
+                                             stream)
     _lib.check(st, "uttt_kv_ring_commit")
 
 
@@ -65,8 +66,9 @@ def ring_fork(rings: torch.Tensor, src: Sequence[int], dst: Sequence[int],
     arr = C.c_int * n
     ring_stride, r = S * n_kv * W * hd, rings.data_ptr()
     dev = rings.device
-    with torch.cuda.device(dev):
+    on, stream = _launch(dev)
+    with on:
         st = _lib.load().uttt_kv_ring_fork(L, n, n_kv, hd, W, S, r, r + 2 * L * ring_stride, ring_stride, arr(*src),
                                            arr(*dst), None if end_pos is None else arr(*(min(e, W) for e in end_pos)),
-                                           torch.cuda.current_stream(dev).cuda_stream)
+                                           stream)
     _lib.check(st, "uttt_kv_ring_fork")

@@ -16,7 +16,7 @@ from typing import NamedTuple, Optional, Union
 import torch
 
 from . import _lib
-from .fastweight import _require_cuda
+from .fastweight import _launch, _require_cuda
 
 Setting = Union[None, int, float, torch.Tensor]
 
@@ -45,7 +45,7 @@ def check_settings(temperature: float = 1.0, top_k: Optional[int] = None, top_p:
 def _per_row(name: str, v: Setting, off, dtype: torch.dtype, rows: int, device: torch.device):
     """(device pointer or None, value for all rows)."""
     if isinstance(v, torch.Tensor):
-        if v.dtype != dtype or v.dim() != 1 or v.shape[0] != rows or not v.is_contiguous() or v.device != device:
+        if v.dtype is not dtype or v.shape != (rows,) or not v.is_contiguous() or v.device != device:
             raise ValueError(f"{name} per row must be a contiguous {dtype} tensor of {rows} on {device}")
         return v.data_ptr(), off
     return None, off if v is None else v
@@ -63,42 +63,45 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
     PAD / BOS / UNK and ids from ``active_limit`` on are never picked (nor ids 2, 4 and 5 when
     ``stop_free``), as by ``UtttB200.greedy``.  Runs on the current stream of the logits' device."""
     _require_cuda(logits, u, u_index)
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.shape[1] <= 6:
+    dev, f = logits.device, torch.float32
+    is_f32 = logits.dtype is f
+    if logits.dim() != 2 or not (is_f32 or logits.dtype is torch.bfloat16) or logits.shape[1] <= 6:
         raise ValueError("logits must be FP32 or BF16 (rows, V) with V > 6")
-    dev = logits.device
     rows, V = logits.shape
     if rows == 0:
-        return Sampled(torch.empty(0, dtype=torch.int32, device=dev), torch.empty(0, dtype=torch.int32, device=dev),
-                       torch.empty(0, device=dev))
-    if logits.stride(1) != 1 or (rows > 1 and logits.stride(0) < V):
+        return Sampled(*(torch.empty(0, dtype=t, device=dev) for t in (torch.int32, torch.int32, f)))
+    ld, step = logits.stride()
+    if step != 1 or (rows > 1 and ld < V):
         logits = logits.contiguous()
-    if u.dtype != torch.float32 or u.device != dev or u.shape[0] != rows or u.dim() not in (1, 2) \
-            or not u.is_contiguous() or u.numel() == 0:
+        ld = V
+    n_u = 1 if u.dim() == 1 else u.shape[-1]
+    if u.dtype is not f or u.dim() > 2 or u.shape[0] != rows or n_u == 0 or not u.is_contiguous() or u.device != dev:
         raise ValueError("u must be a contiguous FP32 (rows,) or (rows, n) tensor beside the logits")
-    if u_index is None and u.dim() == 2 and u.shape[1] != 1:
-        raise ValueError("u of several numbers a row needs u_index")
-    if u_index is not None and (u_index.dtype != torch.int32 or u_index.shape != (rows,) or u_index.device != dev
-                                or not u_index.is_contiguous()):
+    if u_index is None:
+        if n_u != 1:
+            raise ValueError("u of several numbers a row needs u_index")
+        index = None
+    elif u_index.dtype is not torch.int32 or u_index.shape != (rows,) or not u_index.is_contiguous() \
+            or u_index.device != dev:
         raise ValueError("u_index must be a contiguous int32 (rows,) tensor beside the logits")
-    check_settings(*(d if isinstance(v, torch.Tensor) else v
-                     for v, d in ((temperature, 1.0), (top_k, None), (top_p, None), (min_p, None))))
+    else:
+        index = u_index.data_ptr()
     limit = V if active_limit is None else int(active_limit)
     if limit <= 2:
         raise ValueError("Active vocabulary must include EOS")
-    f = torch.float32
-    opt = _lib.Sampling()
-    opt.temperature, opt.temperature_all = _per_row("temperature", temperature, 1.0, f, rows, dev)
-    opt.top_k, opt.top_k_all = _per_row("top_k", top_k, 0, torch.int32, rows, dev)
-    opt.top_p, opt.top_p_all = _per_row("top_p", top_p, 1.0, f, rows, dev)
-    opt.min_p, opt.min_p_all = _per_row("min_p", min_p, 0.0, f, rows, dev)
-    n_u = u.shape[1] if u.dim() == 2 else 1
-    ids, kept = torch.empty(2, rows, dtype=torch.int32, device=dev).unbind(0)
+    tp, t0 = _per_row("temperature", temperature, 1.0, f, rows, dev)
+    kp, k0 = _per_row("top_k", top_k, 0, torch.int32, rows, dev)
+    pp, p0 = _per_row("top_p", top_p, 1.0, f, rows, dev)
+    mp, m0 = _per_row("min_p", min_p, 0.0, f, rows, dev)
+    check_settings(t0, k0, p0, m0)
+    opt = _lib.Sampling(tp, kp, pp, mp, t0, int(k0), p0, m0)
+    ids = torch.empty(rows, dtype=torch.int32, device=dev)
+    kept = torch.empty(rows, dtype=torch.int32, device=dev)
     prob = torch.empty(rows, dtype=f, device=dev)
-    with torch.cuda.device(dev):
-        st = _lib.load().uttt_sample(rows, V, logits.data_ptr(), int(logits.dtype == f),
-                                     logits.stride(0) if rows > 1 else V, limit, int(stop_free), C.byref(opt),
-                                     u.data_ptr(), n_u, None if u_index is None else u_index.data_ptr(), n_u,
-                                     ids.data_ptr(), kept.data_ptr(), prob.data_ptr(),
-                                     torch.cuda.current_stream(dev).cuda_stream)
+    on, stream = _launch(dev)
+    with on:
+        st = _lib.load().uttt_sample(rows, V, logits.data_ptr(), is_f32, ld if rows > 1 else V, limit, bool(stop_free),
+                                     C.byref(opt), u.data_ptr(), n_u, index, n_u, ids.data_ptr(), kept.data_ptr(),
+                                     prob.data_ptr(), stream)
     _lib.check(st, "uttt_sample")
     return Sampled(ids, kept, prob)

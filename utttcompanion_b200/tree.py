@@ -13,7 +13,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .fastweight import _require_cuda
+from .fastweight import _launch, _require_cuda
 
 MAX_NODES = 64
 
@@ -30,7 +30,7 @@ def check_tree(parents: Sequence[int]) -> None:
 def _int_rows(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 {shape} tensor on {device}")
     return t.data_ptr()
 
@@ -53,43 +53,43 @@ def tree_attention(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, 
     if parents.dim() != 2 or k_ring.dim() != 4:
         raise ValueError("parents must be (B, N) and the rings (slots, n_kv, W, hd)")
     B, N = parents.shape
-    n_slots, n_kv, W, hd = k_ring.shape
-    if k_ring.dtype != bf or v_ring.dtype != bf or v_ring.shape != k_ring.shape or not k_ring.is_contiguous() \
-            or not v_ring.is_contiguous() or k_ring.device != dev or v_ring.device != dev:
+    n_slots, n_kv, W, hd = shape = k_ring.shape
+    if k_ring.dtype is not bf or v_ring.dtype is not bf or v_ring.shape != shape or not k_ring.is_contiguous() \
+            or not v_ring.is_contiguous() or k_ring.device != dev or v_ring.device != dev or 0 in shape:
         raise ValueError("the rings must be contiguous BF16 tensors of one shape beside qkv")
     if not 1 <= N <= MAX_NODES:
         raise ValueError(f"a drafted tree has 1 to {MAX_NODES} nodes")
-    if n_heads < 1 or n_heads % n_kv or qkv.dtype != bf or qkv.dim() != 2 or qkv.shape[0] != B * N \
-            or qkv.shape[1] < (n_heads + 2 * n_kv) * hd or qkv.stride(1) != 1:
+    q_dim = n_heads * hd
+    if n_heads < 1 or n_heads % n_kv or qkv.dtype is not bf or qkv.dim() != 2 or qkv.shape[0] != B * N \
+            or qkv.shape[1] < q_dim + 2 * n_kv * hd or qkv.stride(1) != 1:
         raise ValueError("qkv must be BF16 (B * N, (n_heads + 2 * n_kv) * hd) rows")
+    table = rope_cos.shape
     for t in (rope_cos, rope_sin):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != hd or not t.is_contiguous() or t.device != dev \
-                or t.shape[0] != rope_cos.shape[0] or t.shape[0] < 1:
+        if t.dtype is not torch.float32 or t.shape != table or len(table) != 2 or table[1] != hd or table[0] < 1 \
+                or not t.is_contiguous() or t.device != dev:
             raise ValueError("rope_cos and rope_sin must be contiguous FP32 (positions, hd) tables")
     if out is None:
-        out = torch.zeros(B * N, n_heads * hd, dtype=bf, device=dev)
-    elif out.dtype != bf or out.dim() != 2 or out.shape[0] != B * N or out.shape[1] != n_heads * hd \
-            or out.stride(1) != 1 or out.device != dev:
+        out = torch.zeros(B * N, q_dim, dtype=bf, device=dev)
+    elif out.dtype is not bf or out.shape != (B * N, q_dim) or out.stride(1) != 1 or out.device != dev:
         raise ValueError("out must be BF16 (B * N, n_heads * hd) rows")
-    if k_tree is None:
-        k_tree = torch.zeros(B, n_kv, N, hd, dtype=bf, device=dev)
-    if v_tree is None:
-        v_tree = torch.zeros(B, n_kv, N, hd, dtype=bf, device=dev)
+    kv_shape = (B, n_kv, N, hd)
+    k_tree = torch.zeros(kv_shape, dtype=bf, device=dev) if k_tree is None else k_tree
+    v_tree = torch.zeros(kv_shape, dtype=bf, device=dev) if v_tree is None else v_tree
     for t in (k_tree, v_tree):
-        if t.dtype != bf or t.shape != (B, n_kv, N, hd) or not t.is_contiguous() or t.device != dev:
+        if t.dtype is not bf or t.shape != kv_shape or not t.is_contiguous() or t.device != dev:
             raise ValueError("k_tree and v_tree must be contiguous BF16 (B, n_kv, N, hd)")
     args = (_int_rows("parents", parents, (B, N), dev), _int_rows("n_nodes", n_nodes, (B,), dev),
             _int_rows("pos", pos, (B,), dev), _int_rows("slots", slots, (B,), dev))
     if B == 0:
         return out, k_tree, v_tree
     many = B * N > 1
-    with torch.cuda.device(dev):
-        st = _lib.load().uttt_attn_tree(B, N, n_heads, n_kv, hd, W, n_slots, rope_cos.shape[0], qkv.data_ptr(),
+    on, stream = _launch(dev)
+    with on:
+        st = _lib.load().uttt_attn_tree(B, N, n_heads, n_kv, hd, W, n_slots, table[0], qkv.data_ptr(),
                                         qkv.stride(0) if many else qkv.shape[1], *args, k_ring.data_ptr(),
                                         v_ring.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
                                         k_tree.data_ptr(), v_tree.data_ptr(), out.data_ptr(),
-                                        out.stride(0) if many else out.shape[1],
-                                        torch.cuda.current_stream(dev).cuda_stream)
+                                        out.stride(0) if many else q_dim, stream)
     _lib.check(st, "uttt_attn_tree")
     return out, k_tree, v_tree
 
@@ -104,15 +104,17 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     _require_cuda(tokens, parents, picks, n_nodes)
     if tokens.dim() != 2 or not 1 <= tokens.shape[1] <= MAX_NODES:
         raise ValueError(f"tokens must be (B, N) with 1 to {MAX_NODES} nodes")
-    dev, shape = tokens.device, tuple(tokens.shape)
+    dev, shape = tokens.device, tokens.shape
     B, N = shape
     ptrs = (_int_rows("tokens", tokens, shape, dev), _int_rows("parents", parents, shape, dev),
             _int_rows("n_nodes", n_nodes, (B,), dev), _int_rows("picks", picks, shape, dev))
     path = torch.empty(B, N, dtype=torch.int32, device=dev)
-    n_path, following = torch.empty(2, B, dtype=torch.int32, device=dev).unbind(0)
+    n_path = torch.empty(B, dtype=torch.int32, device=dev)
+    following = torch.empty(B, dtype=torch.int32, device=dev)
     if B:
-        with torch.cuda.device(dev):
+        on, stream = _launch(dev)
+        with on:
             st = _lib.load().uttt_tree_accept(B, N, *ptrs, path.data_ptr(), n_path.data_ptr(), following.data_ptr(),
-                                              torch.cuda.current_stream(dev).cuda_stream)
+                                              stream)
         _lib.check(st, "uttt_tree_accept")
     return path, n_path, following
