@@ -117,20 +117,21 @@ __device__ __forceinline__ double widen(unsigned bits) {
                           (int)(bits << 29));
 }
 
+// Rows with +inf among their logits: only the infinities have weight (the others' is exp(-inf)).  +inf is taken as the
+// largest finite number and that one, in such a row, as the number below it, whose distance of 2^104 leaves no weight.
+constexpr float kMaxFinite = 3.402823466e+38f;
+__device__ __forceinline__ unsigned finite_top(unsigned bits) {
+  return bits == 0x7f800000u || bits == 0x7f7fffffu ? bits - 1u : bits;
+}
+
 struct Weigher {
   double m, c;          // largest logit, log2(e) / T
   float mf, cf;
-  bool top_inf;         // the largest logit is +inf: only its equals have weight
   const unsigned* tab;  // this lane's copy
-  // x in FP32; NaN or infinite for what has no weight
-  __device__ __forceinline__ float rough(unsigned bits) const {
-    if (top_inf) return bits == 0x7f800000u ? 0.f : INFINITY;
-    return (mf - __uint_as_float(bits)) * cf;
-  }
+  // x in FP32; NaN or infinite for NaN and -inf
+  __device__ __forceinline__ float rough(unsigned bits) const { return (mf - __uint_as_float(bits)) * cf; }
   // x >= 0
-  __device__ __forceinline__ double exponent(unsigned bits) const {
-    return top_inf ? 0.0 : (m - widen(bits)) * c;
-  }
+  __device__ __forceinline__ double exponent(unsigned bits) const { return (m - widen(bits)) * c; }
   // x as a whole number of 2^-32 (high word: integer part)
   __device__ __forceinline__ uint2 fixed(double x) const {
     const double t = x + 1048576.0;      // 2^20: the last place is 2^-32
@@ -242,6 +243,7 @@ template <bool F32>
 struct Row {
   const char* src;        // the row
   bool vec;               // whether it starts on 16 bytes
+  bool has_inf;           // whether its largest logit is +inf
   int V, lim, stop_free;
   int v0, v1;
   uint4* ring;            // the warp's places in shared memory
@@ -252,27 +254,37 @@ struct Row {
   __device__ __forceinline__ void each(F f) const {
     const int lane = threadIdx.x & 31;
     constexpr int ahead = F32 ? SM_RING / 2 : SM_RING;
-    auto place = [&](int v) { return ring + ((v - v0) / 32 % ahead * (F32 ? 2 : 1)) * 32 + lane; };
-    auto fetch = [&](int v) {
-      if (vec && v < v1 && v * 8 + 8 <= V) {
-        const uint4* p = reinterpret_cast<const uint4*>(src) + (size_t)v * (F32 ? 2 : 1);
-        cp_async_16(place(v), p, true);
-        if (F32) cp_async_16(place(v) + 32, p + 1, true);
+    constexpr int W = F32 ? 2 : 1;       // 16-byte pieces of a vector
+    uint4* const mine = ring + lane;
+    const uint4* next = reinterpret_cast<const uint4*>(src) + (size_t)(v0 + lane) * W;
+    const int full = vec ? min(v1, V / 8) : 0;   // vectors that can be fetched whole
+    int vf = v0 + lane;                  // the next one to fetch, into place sf
+    unsigned sf = 0;
+    auto fetch = [&]() {
+      if (vf < full) {
+        cp_async_16(mine + sf * (W * 32), next, true);
+        if (F32) cp_async_16(mine + sf * (W * 32) + 32, next + 1, true);
       }
       cp_async_commit();
+      next += 32 * W;
+      vf += 32;
+      sf = (sf + 1) & (ahead - 1);
     };
 #pragma unroll 1
-    for (int k = 0; k < ahead - 1; ++k) fetch(v0 + lane + k * 32);
+    for (int k = 0; k < ahead - 1; ++k) fetch();
+    unsigned sr = 0;
 #pragma unroll 1
     for (int t = v0; t < v1; t += 32) {
       const int v = t + lane;
-      fetch(v + (ahead - 1) * 32);
+      fetch();
       cp_async_wait<ahead - 1>();
       unsigned x[8];
-      if (vec && v * 8 + 8 <= V) {
-        const uint4 a = *place(v);       // (an old one where v is behind the piece)
+      const uint4* at = mine + sr * (W * 32);
+      sr = (sr + 1) & (ahead - 1);
+      if (v < full) {
+        const uint4 a = at[0];
         if (F32) {
-          const uint4 b = place(v)[32];
+          const uint4 b = at[32];
           x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
         } else {
           x[0] = a.x << 16, x[1] = a.x & 0xffff0000u, x[2] = a.y << 16, x[3] = a.y & 0xffff0000u;
@@ -282,6 +294,10 @@ struct Row {
         const Eight r = load_scalar<F32>(src, min(v, v1 - 1) * 8, V);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = r.x[e];
+      }
+      if (has_inf) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = finite_top(x[e]);
       }
       if (v == 0 || v >= v1 || v * 8 + 8 > lim) {
 #pragma unroll
@@ -296,21 +312,34 @@ struct Row {
   }
 };
 
-// Gather the pairs that f(bits) takes (of all CTAs) into rank 0's list; returns how many there are.  Every CTA
+__device__ __forceinline__ unsigned nth_of(const unsigned (&x)[8], int e) {
+  unsigned r = x[0];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) r = e == k ? x[k] : r;
+  return r;
+}
+
+// Gather the pairs that in_range(bits, id) takes (of all CTAs) into rank 0's list; returns how many there are.
+// near(bits) is a quick test that lets all of them pass and few others.  Every CTA
 // then holds a copy in cand[c.list] if they are at most SM_CAP.  Consecutive gathers use the two lists in turn, so
 // a CTA may start the next one while another still ranks this one's; the other list's counter is cleared between
 // this gather's two barriers, after its last reader and before its next writer.
-template <bool F32, class InRange>
-__device__ unsigned gather(Cluster& c, const Row<F32>& row, InRange in_range) {
+template <bool F32, class Near, class InRange>
+__device__ unsigned gather(Cluster& c, const Row<F32>& row, Near near, InRange in_range) {
   SampleShared* lead = c.peer(0);
   const int q = c.list ^= 1;
   row.each([&](const unsigned (&x)[8], int id) {
+    unsigned mask = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (in_range(x[e], id + e)) {
+    for (int e = 0; e < 8; ++e) mask |= near(x[e]) ? 1u << e : 0u;
+    for (; mask; mask &= mask - 1) {
+      const int e = __ffs((int)mask) - 1;
+      const unsigned xe = nth_of(x, e);
+      if (in_range(xe, id + e)) {
         const unsigned at = atomicAdd(&lead->n_cand[q], 1u);
-        if (at < SM_CAP) lead->cand[q][at] = pair_of(order_key(x[e]), id + e);
+        if (at < SM_CAP) lead->cand[q][at] = pair_of(order_key(xe), id + e);
       }
+    }
     return true;
   });
   c.sync();
@@ -338,8 +367,8 @@ __device__ u64 rank_candidates(Cluster& c, unsigned n, int mode, u64 target, con
   __syncthreads();
   if (threadIdx.x < n) {
     u64 before = 0ull;
-    for (unsigned j = 0; j < n; ++j)
-      if (cand[j] > mine) before += sh->cand_w[j];
+#pragma unroll 8
+    for (unsigned j = 0; j < n; ++j) before += cand[j] > mine ? sh->cand_w[j] : 0ull;
     if (before <= target && before + own > target) sh->res_cut = mine;
   }
   __syncthreads();
@@ -416,8 +445,8 @@ __device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, 
 
 __device__ __forceinline__ void add_mass(SampleShared* sh, int bin, u64 wt) {
   const unsigned l0 = (unsigned)wt & 0xffffu, l1 = (unsigned)wt >> 16, l2 = (unsigned)(wt >> 32);
-  if (l0) atomicAdd(&sh->hist[0][bin], l0);
-  if (l1) atomicAdd(&sh->hist[1][bin], l1);
+  atomicAdd(&sh->hist[0][bin], l0);
+  atomicAdd(&sh->hist[1][bin], l1);
   if (l2) atomicAdd(&sh->hist[2][bin], l2);
 }
 
@@ -427,9 +456,10 @@ __device__ __forceinline__ void clear_hist(SampleShared* sh) {
   __syncthreads();
 }
 
-// The pair of the n-th (from 0, by id) candidate with this key; there are more than n of them.
+// The pair of the n-th (from 0, by id) candidate with this key; there are more than n of them.  One exchange (on a
+// copy of c).
 template <bool F32>
-__device__ u64 nth_equal(Cluster& c, const Row<F32>& row, unsigned key, u64 n) {
+__device__ __noinline__ u64 nth_equal(Cluster c, const Row<F32> row, unsigned key, u64 n) {
   SampleShared* sh = c.sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned count = 0u;
@@ -485,10 +515,14 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
                         unsigned n_eligible) {
   SampleShared* sh = c.sh;
   if (n_eligible <= SM_CAP) {            // few enough to rank at once
-    const unsigned n = gather(c, row, [&](unsigned bits, int id) {
-      const unsigned key = order_key(bits);
-      return is_candidate(key) && pair_of(key, id) >= cut;
-    });
+    const unsigned cut_bits = __float_as_uint(key_value((unsigned)(cut >> 32)));
+    const float least = cut ? __uint_as_float(cut_bits) : -INFINITY;
+    const unsigned n = gather(
+        c, row, [&](unsigned bits) { return __uint_as_float(bits) >= least; },
+        [&](unsigned bits, int id) {
+          const unsigned key = order_key(bits);
+          return is_candidate(key) && pair_of(key, id) >= cut;
+        });
     if (MODE == FIND_MASS) {
       u64 v = threadIdx.x < n ? w.weight_of_key((unsigned)(sh->cand[c.list][threadIdx.x] >> 32)) : 0ull;
       v = warp_sum64(v);
@@ -547,13 +581,18 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
     mx = pr > mx ? pr : mx;
     return true;
   };
-  unsigned n = gather(c, row, [&](unsigned bits, int id) {
-    const float y = w.rough(bits);
-    u64 pr;
-    if (bin == SM_TAIL) return !(y <= SM_RANGE) && take(bits, id, pr) && span(pr);
-    return y >= y0 && y <= y1 && y <= SM_RANGE && w.bin(w.fixed(w.exponent(bits))) == bin && take(bits, id, pr) &&
-           span(pr);
-  });
+  unsigned n = gather(
+      c, row,
+      [&](unsigned bits) {
+        const float y = w.rough(bits);
+        return y >= y0 && y <= y1;
+      },
+      [&](unsigned bits, int id) {
+        const bool tail = !(w.rough(bits) <= SM_RANGE);
+        u64 pr;
+        if (bin == SM_TAIL ? !tail : tail || w.bin(w.fixed(w.exponent(bits))) != bin) return false;
+        return take(bits, id, pr) && span(pr);
+      });
   bool sure = bin != SM_TAIL;            // whether the bin is known to hold the cut
   bool whole = true;                     // whether it holds all candidates of a key, or none
   for (int pass = 0; pass < 10; ++pass) {
@@ -583,7 +622,9 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
     if (k0 == k1 && sure && whole && k0 != cut_key) {
       // equal logits: the first ones by id are kept
       const u64 each = MODE == FIND_COUNT ? 1ull : w.weight_of_key(k0);
-      return nth_equal(c, row, k0, target / each);
+      const u64 pr = nth_equal(c, row, k0, target / each);
+      c.phase ^= 1;                      // it exchanged once
+      return pr;
     }
     if (k0 != k1 && whole) {             // by keys, then (rarely) by ids
       lo = pair_of(k0, 0xffffffffu);
@@ -596,12 +637,17 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
       whole = false;
     }
     clear_hist(sh);
+    auto near_span = [&](unsigned bits_e) {
+      const unsigned key = order_key(bits_e);
+      return key >= (unsigned)(lo >> 32) && key <= (unsigned)(hi >> 32);
+    };
     row.each([&](const unsigned (&x)[8], int id) {
-#pragma unroll 1
-      for (int e = 0; e < 8; ++e) {
-        unsigned xe = x[0];
+      unsigned mask = 0u;
 #pragma unroll
-        for (int k = 1; k < 8; ++k) xe = e == k ? x[k] : xe;
+      for (int e = 0; e < 8; ++e) mask |= near_span(x[e]) ? 1u << e : 0u;
+      for (; mask; mask &= mask - 1) {
+        const int e = __ffs((int)mask) - 1;
+        const unsigned xe = nth_of(x, e);
         u64 pr;
         if (!take(xe, id + e, pr)) continue;
         const int at = (int)((hi - pr) >> sh_bits);
@@ -618,10 +664,11 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
     target -= base;
     mn = ~0ull;
     mx = 0ull;
-    n = gather(c, row, [&](unsigned bits_e, int id) {
-      u64 pr;
-      return take(bits_e, id, pr) && (int)((hi - pr) >> sh_bits) == bin && span(pr);
-    });
+    n = gather(
+        c, row, near_span, [&](unsigned bits_e, int id) {
+          u64 pr;
+          return take(bits_e, id, pr) && (int)((hi - pr) >> sh_bits) == bin && span(pr);
+        });
   }
   return cut;                            // not reached: a pass leaves 1/2048 of the range of keys, then of ids
 }
@@ -637,7 +684,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   const int row_i = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < 2) sh->n_cand[tid] = 0u;
   c.arrive();                            // peers write here only once every CTA of the cluster has started
-  for (int i = tid; i < SM_STEPS * 32; i += SM_THREADS) sh->tab[i] = kPow2[i >> 5];
+#pragma unroll
+  for (int k = 0; k < SM_STEPS / SM_WARPS; ++k) sh->tab[(k * SM_WARPS + warp) * 32 + lane] = kPow2[k * SM_WARPS + warp];
   pdl_wait();
   pdl_trigger();
   // ---- the warp's piece of the row (`part` 8-logit vectors per CTA)
@@ -645,6 +693,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   row.src = reinterpret_cast<const char*>(logits) + (size_t)row_i * ld * (F32 ? 4 : 2);
   row.vec = (reinterpret_cast<uintptr_t>(row.src) & 15u) == 0;
   row.V = V;
+  row.has_inf = false;
   row.lim = lim;
   row.stop_free = stop_free;
   row.ring = sh->ring[warp];
@@ -684,15 +733,16 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   const bool greedy = !(T > SM_GREEDY_T) || top_k == 1;
   if (greedy) T = 1.f;
   Weigher w;
-  w.mf = key_value(mkey);
+  row.has_inf = mkey == kInfKey;
+  w.mf = row.has_inf ? kMaxFinite : key_value(mkey);
   w.m = widen(__float_as_uint(w.mf));
-  w.top_inf = mkey == kInfKey;
   w.c = 1.4426950408889634074 / (double)T;
   w.cf = (float)w.c;
   w.tab = sh->tab + lane;
   u64 cut = 0ull;
   if (greedy) {
-    cut = nth_equal(c, row, mkey, 0ull);
+    cut = nth_equal(c, row, order_key(__float_as_uint(w.mf)), 0ull);
+    c.phase ^= 1;                        // it exchanged once
   } else {
     unsigned eligible = (unsigned)lim;
     if (top_k > 0 && top_k < lim) {
@@ -703,31 +753,35 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   }
   const double x_max = min_p > 0.f ? -log2((double)fminf(min_p, 1.f)) : INFINITY;
   // ---- kept mass per warp
-  const unsigned cut_key = max((unsigned)(cut >> 32), 0x00800000u);
-  auto weigh = [&](unsigned bits, int id, bool& in) -> u64 {
-    const unsigned key = order_key(bits);
-    in = key >= cut_key && key <= kInfKey;
-    if (!in) return 0ull;
-    in = pair_of(key, id) >= cut;
-    if (!in) return 0ull;
+  // FP32's x (good to 2^-22 of itself) tells all but the elements next to the cut apart from it; the keys decide there
+  // and beyond 64, where an overflow could stand for anything
+  const bool any_cut = cut != 0ull, any_min = x_max != INFINITY;
+  const float yc = w.rough(__float_as_uint(key_value((unsigned)(cut >> 32))));
+  const float y_hi = fminf(any_cut ? yc * 1.000001f + 1e-5f : INFINITY,
+                           any_min ? (float)x_max * 1.000001f + 1e-5f : INFINITY);
+  const float y_lo = any_cut ? fminf(yc * 0.999999f - 1e-5f, 64.f) : 64.f;
+  auto weigh = [&](unsigned bits, int id, unsigned& count) -> u64 {
     const float y = w.rough(bits);
-    if (!(y <= SM_RANGE)) {
-      in = x_max == INFINITY || (double)y <= x_max;   // min_p below 2^-24
-      return in ? (u64)w.tail_weight(y) : 0ull;
+    if (!(y <= y_hi)) return 0ull;
+    if (y > y_lo) {
+      const unsigned key = order_key(bits);
+      if (!is_candidate(key) || pair_of(key, id) < cut) return 0ull;
     }
-    const double x = w.exponent(bits);
-    in = x <= x_max;
-    return in ? w.weight(w.fixed(x)) : 0ull;
+    if (y <= SM_RANGE) {
+      const double x = w.exponent(bits);
+      if (any_min && x > x_max) return 0ull;
+      ++count;
+      return w.weight(w.fixed(x));
+    }
+    if (any_min && (double)y > x_max) return 0ull;   // (min_p below 2^-24)
+    ++count;
+    return (u64)w.tail_weight(y);
   };
   u64 mass = 0ull;
   unsigned count = 0u;
   row.each([&](const unsigned (&x)[8], int id) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      bool in;
-      mass += weigh(x[e], id + e, in);
-      count += in;
-    }
+    for (int e = 0; e < 8; ++e) mass += weigh(x[e], id + e, count);
     return true;
   });
   mass = warp_sum64(mass);
@@ -745,49 +799,64 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     cnt += sh->wred2[i];
   }
   const int p2 = c.exchange(Sel{all, cnt});
-  u64 total = 0ull, n_kept = 0ull;
+  u64 total = 0ull, n_kept = 0ull, all_below = 0ull;
   for (int r = 0; r < c.S; ++r) {
-    if (r < c.rank) below += sh->xch[p2][r].a;
+    if (r < c.rank) all_below += sh->xch[p2][r].a;
     total += sh->xch[p2][r].a;
     n_kept += sh->xch[p2][r].b;
   }
+  below += all_below;
   float uv = u[(size_t)row_i * u_ld + (u_index ? min(max(u_index[row_i], 0), u_len - 1) : 0)];
   uv = fminf(uv, 0.99999994f);           // the largest number below 1
   const u64 target = part_of(uv, total);
+  // The piece that holds the pick has at most SM_WARPS tiles of 32 vectors: each warp of its CTA weighs one again.
   if (below <= target && target < below + mass) {   // one warp of the cluster
-    u64 at = below;
-    row.each([&](const unsigned (&x)[8], int id) {
-      u64 wt[8], sum = 0ull;
+    if (lane == 0) {
+      sh->res_bin = warp;
+      sh->res_base = below;
+    }
+  } else if (tid == 0 && !(all_below <= target && target < all_below + all)) {
+    sh->res_bin = -1;
+  }
+  __syncthreads();
+  const int owner = sh->res_bin;
+  if (owner >= 0) {                      // the same for the whole CTA
+    const u64 piece = sh->res_base;
+    const int v0 = min(end, c.rank * part + owner * per), v1 = min(end, v0 + per);
+    row.v0 = min(v1, v0 + warp * 32);
+    row.v1 = min(v1, row.v0 + 32);
+    u64 wt[8], sum = 0ull;
+    int id0 = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) wt[e] = 0ull;
+    row.each([&](const unsigned (&x)[8], int id) {   // one vector a lane
+      unsigned unused = 0u;
+      id0 = id;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += wt[e] = weigh(x[e], id + e, unused);
+      return true;
+    });
+    u64 inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += t;
+    }
+    if (lane == 31) sh->wred[warp] = inc;
+    __syncthreads();
+    u64 run = piece + inc - sum;
+    for (int i = 0; i < warp; ++i) run += sh->wred[i];
+    if (run <= target && target < run + sum) {       // one lane
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        bool in;
-        sum += wt[e] = weigh(x[e], id + e, in);
-      }
-      u64 inc = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += t;
-      }
-      const u64 tile = __shfl_sync(0xffffffffu, inc, 31);
-      if (target >= at + tile) {
-        at += tile;
-        return true;
-      }
-      u64 run = at + inc - sum;
-      if (run <= target && target < run + sum) {   // one lane
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (run <= target && target < run + wt[e]) {
-            ids[row_i] = id + e;
-            if (kept) kept[row_i] = (int)n_kept;
-            if (prob) prob[row_i] = (float)((double)wt[e] / (double)total);
-          }
-          run += wt[e];
+        if (run <= target && target < run + wt[e]) {
+          ids[row_i] = id0 + e;
+          if (kept) kept[row_i] = (int)n_kept;
+          if (prob) prob[row_i] = (float)((double)wt[e] / (double)total);
         }
+        run += wt[e];
       }
-      return false;
-    });
+    }
   }
   c.sync();                              // no CTA leaves while a peer may still read or write its shared memory
 }
