@@ -136,3 +136,49 @@ def test_trees_at_their_limits():
     tree.check_tree([-1])
     tree.check_tree([-1] + [0] * 63)
     tree.check_tree([-1] + list(range(63)))
+
+
+# ------------------------------------------------------------------------------------------------ host logic
+def test_depths_and_pruning():
+    parents = [-1, 0, 1, 1, 3, 0]
+    depth = tree.depths(parents)
+    assert depth == [0, 1, 2, 2, 3, 1]
+    tokens, par, d = tree.prune([10, 11, 12, 13, 14, 15], parents, depth, 1)
+    assert (tokens, par, d) == ([10, 11, 15], [-1, 0, 0], [0, 1, 1])
+    assert tree.prune([10, 11], [-1, 0], [0, 1], 5) == ([10, 11], [-1, 0], [0, 1])
+    assert tree.prune([10, 11, 12], [-1, 0, 0], [0, 1, 1], 0) == ([10], [-1], [0])
+
+
+def test_prompt_lookup_drafts_what_followed_before():
+    draft = tree.PromptLookup(match=2, depth=3, nodes=5)
+    #      5 6 followed by 7 8 9 first and by 7 1 later: the later one first, merged
+    ids = [5, 6, 7, 8, 9, 5, 6, 7, 1, 2, 5, 6]
+    tokens, parents = draft(ids)
+    assert tokens == [7, 1, 2, 8, 9] and parents == [0, 1, 2, 1, 4]
+    tree.check_tree([-1, *parents])
+    assert tree.PromptLookup(match=2, depth=3, nodes=2)(ids) == ([7, 1], [0, 1])
+    assert draft([1, 2, 3]) == ([], [])
+    assert draft([4, 4, 4, 4])[0] == [4, 4]            # what follows may run into the end
+    assert draft([7]) == ([], [])
+    with pytest.raises(ValueError):
+        tree.PromptLookup(nodes=64)
+
+
+def test_reply_uniforms_are_repeatable_and_in_range():
+    a = sampling.reply_uniforms(1000, 5)
+    assert torch.equal(a, sampling.reply_uniforms(1000, 5)) and not torch.equal(a, sampling.reply_uniforms(1000, 6))
+    assert torch.equal(sampling.reply_uniforms(10, 5), a[:10])
+    assert float(a.min()) >= 0.0 and float(a.max()) < 1.0
+
+
+def test_sampling_rows_hold_each_rows_settings():
+    rows = sampling.SamplingRows(torch.device("cpu"), 3, 4)
+    rows.set(1, 0.7, 5, 0.9, 0.1, torch.tensor([0.25, 0.5]))
+    f = rows.first(2)
+    assert f["temperature"].tolist() == [0.0, pytest.approx(0.7)] and f["top_k"].tolist() == [0, 5]
+    assert f["top_p"].tolist() == [1.0, pytest.approx(0.9)] and f["u"][1].tolist() == [0.25, 0.5, 0.0, 0.0]
+    rows.set(1)
+    assert rows.temperature.tolist() == [0.0, 0.0, 0.0] and rows.top_p.tolist() == [1.0, 1.0, 1.0]
+    for bad in (dict(row=3), dict(row=0, top_p=0.0), dict(row=0, u=torch.zeros(5))):
+        with pytest.raises(ValueError):
+            rows.set(**bad)

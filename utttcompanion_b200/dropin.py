@@ -526,7 +526,8 @@ class uTTTPersonalizerB200:
     (the reference's ``engine.prompting.encode_chat_prompt``); the turn is then written on the
     reference's re-tokenised ``<|user|> ... <|assistant|> ...`` text (``personalizer.py:480-489``).
     Without a tokenizer ``prompt`` is a list of token ids and the write runs on prompt + reply ids.
-    Decoding is greedy (the north star's contract): ``temperature`` must be 0 or None.
+    Decoding is greedy unless the serving engine samples (``ServingEngine(max_sampled_tokens=...)``): without it
+    ``temperature`` must be 0 or None.
     With ``persona_dir`` every gated write is saved in the reference's persona-file format."""
 
     def __init__(self, serving, tokenizer=None, encode_prompt: Optional[Callable] = None,
@@ -564,8 +565,10 @@ class uTTTPersonalizerB200:
         max_tokens = self.default_max_new_tokens if max_new_tokens is None else max_new_tokens
         if type(max_tokens) is not int or not 1 <= max_tokens < cfg.max_seq_len:
             raise ValueError(f"max_new_tokens must be between 1 and {cfg.max_seq_len - 1}")
-        if temperature is not None and (not math.isfinite(temperature) or temperature > 1e-5 or temperature < 0):
-            raise ValueError("the B200 serving path decodes greedily: temperature must be 0")
+        samples = max_tokens <= getattr(self.serving, "max_sampled_tokens", 0)
+        if temperature is not None and (not math.isfinite(temperature) or temperature < 0
+                                        or (temperature > 1e-5 and not samples)):
+            raise ValueError("this serving engine decodes greedily: temperature must be 0")
         if top_p is not None and (not math.isfinite(top_p) or not 0.0 < top_p <= 1.0):
             raise ValueError("top_p must be finite and in (0, 1]")
         if seed is not None and (type(seed) is not int or not 0 <= seed < 2 ** 63):
@@ -604,8 +607,10 @@ class uTTTPersonalizerB200:
         max_tokens = self._check(max_new_tokens, temperature, top_p, seed)
         ids, write_ids = self._ids(prompt, max_tokens, history)
         events: List[dict] = []
+        settings = dict(temperature=temperature, top_p=top_p, seed=seed) if temperature and temperature > 1e-5 else {}
         t = self.serving.submit(user_id, ids, max_tokens, eos_token_id=EOS_ID, on_event=events.append,
-                                write_ids=write_ids)
+                                write_ids=write_ids, **settings)
+        seed = t.seed if settings else seed
         emitted: List[int] = []
         text_len = 0
         while True:

@@ -13,6 +13,10 @@ the GPU and runs the hot path with this package's kernels only:
   KV ring slot and position (the multi-persona decode the reference, which is
   batch-1, serialises per persona).
 * ``generate_greedy`` -- ``stream_generate`` at temperature 0.
+* ``tree_step`` / ``tree_commit`` / ``generate_drafted`` -- a tree of drafted tokens verified in one
+  packed step (the reference drafts along one line, ``model/uttt_model.py:1052-1179``).
+* ``sample`` / ``generate_replies`` -- sampled tokens (``_sample_next_token``, ``:1181-1235``) from given
+  random numbers; several replies of one prompt from forked KV rings.
 * ``test_time_update`` -- ``uTTTModel.test_time_update`` with the chunk-first
   shared schedule (``model/uttt_model.py:453-608``): all layers of a chunk read
   the chunk-start snapshot; their writes advance one cursor.
@@ -26,13 +30,14 @@ import ctypes as C
 import math
 from dataclasses import dataclass, field
 from types import SimpleNamespace
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
 from .fastweight import _stream, chunk_write, check_status, workspace
 from .readout import fast_readout
+from . import kv_cache, sampling, tree
 from .workloads import ModelConfig
 
 PAD_ID, BOS_ID, EOS_ID, UNK_ID, USER_ID, ASSISTANT_ID = 0, 1, 2, 3, 4, 5
@@ -158,9 +163,10 @@ class UtttB200:
         self.active_limit = SIMPLE_ACTIVE_VOCAB_LIMIT if cfg.vocab_size >= 24000 else cfg.vocab_size
         self.qkv_dim = (cfg.n_heads + 2 * cfg.n_kv_heads) * hd
         self.max_personas = max_personas
-        shape = (max_personas, cfg.n_kv_heads, cfg.sliding_window_size, hd)
-        self.k_ring = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(cfg.n_layers)]
-        self.v_ring = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(cfg.n_layers)]
+        # keys, then values, of every layer: one tensor, so that one launch can copy all of a persona's rings
+        self.rings = torch.zeros(2, cfg.n_layers, max_personas, cfg.n_kv_heads, cfg.sliding_window_size, hd,
+                                 dtype=torch.bfloat16, device=dev)
+        self.k_ring, self.v_ring = (list(r.unbind(0)) for r in self.rings)
 
     # ------------------------------------------------------------------ launch helpers
     def _st(self) -> int:
@@ -243,6 +249,13 @@ class UtttB200:
         _lib.check(self.lib.uttt_greedy_argmax(B, V, logits.data_ptr(), 1, V, self.active_limit, int(stop_free),
                                                ids.data_ptr(), top2.data_ptr(), self._st()), "uttt_greedy_argmax")
         return ids, top2
+
+    def sample(self, logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=None, top_p=None, min_p=None,
+               stop_free: bool = False, u_index: Optional[torch.Tensor] = None) -> "sampling.Sampled":
+        """Device pick at temperature > 0 from given uniform numbers (``sampling.sample``; the ids that
+        ``greedy`` never picks are never picked here)."""
+        return sampling.sample(logits, u, temperature, top_k, top_p, min_p, active_limit=self.active_limit,
+                               stop_free=stop_free, u_index=u_index)
 
     def read_copies(self, w_up, w_gate, w_down) -> Tuple[torch.Tensor, torch.Tensor]:
         """BF16 read copies of FP32 states (S, d, h) (``inference_read_weights``)."""
@@ -401,6 +414,10 @@ class UtttB200:
             kr[slot].index_copy_(1, idx, k[0].to(device=self.device, dtype=torch.bfloat16))
             vr[slot].index_copy_(1, idx, v[0].to(device=self.device, dtype=torch.bfloat16))
 
+    def fork_kv(self, src: Sequence[int], dst: Sequence[int], end_pos: Optional[Sequence[int]] = None) -> None:
+        """Copy slot ``src[i]``'s rings of all layers to slot ``dst[i]`` (``kv_cache.ring_fork``)."""
+        kv_cache.ring_fork(self.rings, src, dst, end_pos)
+
     def use_state_ln(self, ln_weight: torch.Tensor, ln_bias: torch.Tensor) -> None:
         """Make a persona state's readout LayerNorm affine the one the frozen path applies (in place,
         so captured decode graphs see it), rounded as the BF16 path applies it (:253-257)."""
@@ -462,6 +479,163 @@ class UtttB200:
                                       packed, down, zero)
             pos += 1
         return ids, margins, all_logits
+
+    # ------------------------------------------------------------------ drafted and sampled generation
+    def tree_step(self, tokens: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
+                  read_packed: torch.Tensor, read_down: torch.Tensor, state_index: torch.Tensor,
+                  n_nodes: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """One step over trees of drafted tokens: ``tokens`` and ``parents`` int32 (B, N), node 0 of a row being its
+        pending token, ``pos`` the positions in its ring so far.  Returns (logits (B, N, V) FP32 of BF16 values,
+        the nodes' keys and values (2, layers, B, n_kv, N, hd)); the rings stay as they are until
+        ``tree_commit``.  Logits behind a row's ``n_nodes`` mean nothing."""
+        cfg = self.cfg
+        if tokens.dim() != 2 or tokens.shape != parents.shape:
+            raise ValueError("tokens and parents must be (B, N)")
+        B, N = tokens.shape
+        d, hd, nh, nkv = cfg.d_model, cfg.head_dim, cfg.n_heads, cfg.n_kv_heads
+        dev = self.device
+
+        def i32(t):
+            return None if t is None else t.to(device=dev, dtype=torch.int32).contiguous()
+        parents, pos, slots, sidx, n_nodes = (i32(t) for t in (parents, pos, slots, state_index, n_nodes))
+        R = B * N
+        h = self._embed(tokens)
+        qkv = torch.empty(R, self.qkv_dim, dtype=torch.bfloat16, device=dev)
+        att = torch.zeros(R, d, dtype=torch.bfloat16, device=dev)      # rows without a node stay finite
+        kv = torch.zeros(2, len(self.layers), B, nkv, N, hd, dtype=torch.bfloat16, device=dev)
+        L = len(self.layers)
+        x = self._rmsnorm(h, self.layers[0].attn_norm)
+        for i, lay in enumerate(self.layers):
+            self._linear(x, lay.wqkv, [_seg(0, self.qkv_dim, _lib.SEG_STORE, qkv, self.qkv_dim)])
+            tree.tree_attention(qkv, parents, pos, slots, self.k_ring[i], self.v_ring[i], self.rope_cos,
+                                self.rope_sin, nh, n_nodes=n_nodes, out=att, k_tree=kv[0, i], v_tree=kv[1, i])
+            x2 = self._resid_linear(h, att, lay.wo, lay.uttt_norm)
+            q = self._q_proj(lay, x2)
+            r = self._readout(q.reshape(B, N, d), read_packed, read_down, sidx)
+            x = self._resid_linear(h, r.reshape(R, d), lay.w_o, self.layers[i + 1].attn_norm if i + 1 < L else self.norm)
+        return self._lm_head(x).reshape(B, N, -1), kv
+
+    def tree_commit(self, tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor, kv: torch.Tensor,
+                    pos: torch.Tensor, slots: torch.Tensor, n_nodes: Optional[torch.Tensor] = None
+                    ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Accept each row's path (``tree.tree_accept`` of int32 (B, N) device tensors) and put its keys and values
+        into the rings; returns (path, n_path, next pending token).  The row's ring then holds ``pos + n_path``
+        positions."""
+        path, n_path, following = tree.tree_accept(tokens, parents, picks, n_nodes)
+        kv_cache.ring_commit(self.rings, kv, pos, slots, path, n_path)
+        return path, n_path, following
+
+    def generate_drafted(self, prompt: torch.Tensor, state: FastState, n_tokens: int,
+                         draft: Callable[[List[int]], Tuple[Sequence[int], Sequence[int]]], slot: int = 0,
+                         stop_free: bool = True, eos_token_id: Optional[int] = None, temperature: float = 0.0,
+                         top_k: Optional[int] = None, top_p: Optional[float] = None, min_p: Optional[float] = None,
+                         u: Optional[torch.Tensor] = None) -> Tuple[List[int], int]:
+        """``generate_greedy`` (or, at temperature > 0, sampled generation from the numbers ``u`` (n_tokens,)) with
+        drafted tokens: ``draft(ids)`` proposes, after the prompt and the reply so far, a tree of tokens
+        (``tokens[i]`` at node i + 1, ``parents[i]`` < i + 1; node 0 is the last id), e.g. ``tree.PromptLookup()``.
+        Token t of the reply is the pick from its own logits with ``u[t]``, as without a draft, so drafts change how
+        many steps the reply takes, not the reply.  Returns (ids, steps).  After a stop inside an accepted path the
+        ring also holds the path's tokens behind it."""
+        sampling.check_settings(temperature, top_k, top_p, min_p)
+        sampled = temperature > 1e-5
+        if sampled and (u is None or u.numel() < n_tokens):
+            raise ValueError("sampled generation needs one number per token")
+        packed, down = self.read_copies(state.w_up, state.w_gate, state.w_down)
+        dev = self.device
+        u = u.to(device=dev, dtype=torch.float32).reshape(-1).contiguous() if sampled else None
+
+        def pick(logits, numbers):
+            if not sampled:
+                return self.greedy(logits, stop_free)[0]
+            return self.sample(logits, numbers, temperature, top_k, top_p, min_p, stop_free=stop_free).ids
+        logits = self.prefill(prompt, slot, packed, down, 0).unsqueeze(0)
+        pending = int(pick(logits, None if u is None else u[:1]).item())
+        seq, start = [int(i) for i in prompt.reshape(-1).tolist()], prompt.numel()
+        ids: List[int] = []
+        pos, steps = start, 0
+        row = _host_list([0], torch.int32, dev)
+        slot_t = _host_list([slot], torch.int32, dev)
+
+        def ended(tok: int) -> bool:       # stream_generate's stop rules (:1036-1050)
+            if not stop_free and tok in (USER_ID, ASSISTANT_ID):
+                return True
+            ids.append(tok)
+            return len(ids) >= n_tokens or (not stop_free and eos_token_id is not None and tok == eos_token_id)
+        done = n_tokens < 1 or ended(pending)
+        while not done:
+            drafted, above = draft(seq + ids)
+            tokens, parents = [ids[-1], *(int(t) for t in drafted)], [-1, *(int(p) for p in above)]
+            if len(tokens) != len(parents):
+                raise ValueError("a draft has one parent per token")
+            tree.check_tree(parents)
+            if min(tokens) < 0 or max(tokens) >= self.emb.shape[0]:
+                raise ValueError("token id outside the vocabulary")
+            depth = tree.depths(parents)
+            # no deeper than the reply can still grow, and than the RoPE table reaches
+            most = min(n_tokens - len(ids), self.n_pos - pos) - 1
+            if most < 0:
+                raise ValueError("reply longer than the RoPE table")
+            tokens, parents, depth = tree.prune(tokens, parents, depth, most)
+            tok_t, par_t = (_host_list([v], torch.int32, dev) for v in (tokens, parents))
+            pos_t = _host_list([pos], torch.int32, dev)
+            lg, kv = self.tree_step(tok_t, par_t, pos_t, slot_t, packed, down, row)
+            lg = lg.reshape(len(tokens), -1)
+            numbers = None
+            if sampled:
+                numbers = u[_host_list([len(ids) + k for k in depth], torch.long, dev)]
+            picks = pick(lg, numbers).reshape(1, -1)
+            path, n_path, following = self.tree_commit(tok_t, par_t, picks, kv, pos_t, slot_t)
+            steps += 1
+            taken = path[0, :int(n_path.item())].tolist()
+            pos += len(taken)
+            for tok in [tokens[i] for i in taken[1:]] + [int(following.item())]:
+                done = ended(tok)
+                if done:
+                    break
+        return ids, steps
+
+    def generate_replies(self, prompt: torch.Tensor, state: FastState, n_tokens: int, n_replies: int,
+                         temperature: float = 0.7, top_k: Optional[int] = None, top_p: Optional[float] = 0.9,
+                         min_p: Optional[float] = None, seed: int = 0, slots: Optional[Sequence[int]] = None,
+                         stop_free: bool = True, eos_token_id: Optional[int] = None) -> List[List[int]]:
+        """``n_replies`` sampled replies of one persona to one prompt: the prompt is prefilled once, its KV rings are
+        forked to one slot per reply (``slots``; default 0 .. n_replies - 1), and the replies decode as one packed
+        batch, each from its own random numbers (``sampling.reply_uniforms(n_tokens, seed + reply)``)."""
+        sampling.check_settings(temperature, top_k, top_p, min_p)
+        slots = list(range(n_replies)) if slots is None else [int(s) for s in slots]
+        if n_replies < 1 or len(slots) != n_replies or len(set(slots)) != n_replies or n_tokens < 1 \
+                or min(slots) < 0 or max(slots) >= self.max_personas:
+            raise ValueError("one KV slot of the engine per reply")
+        T = prompt.numel()
+        if T + n_tokens >= self.n_pos:
+            raise ValueError("reply longer than the RoPE table")
+        packed, down = self.read_copies(state.w_up, state.w_gate, state.w_down)
+        dev = self.device
+        u = torch.stack([sampling.reply_uniforms(n_tokens, seed + r) for r in range(n_replies)])
+        u = (u.pin_memory() if dev.type == "cuda" else u).to(dev, non_blocking=True)
+        logits = self.prefill(prompt, slots[0], packed, down, 0)
+        self.fork_kv([slots[0]] * (n_replies - 1), slots[1:], [T] * (n_replies - 1))
+        logits = logits.unsqueeze(0).expand(n_replies, -1).contiguous()
+        slot_t = _host_list(slots, torch.int32, dev)
+        zero = torch.zeros(n_replies, dtype=torch.int32, device=dev)
+        step = torch.zeros(n_replies, dtype=torch.int32, device=dev)
+        replies: List[List[int]] = [[] for _ in range(n_replies)]
+        live = [True] * n_replies
+        for t in range(n_tokens):
+            picks = self.sample(logits, u, temperature, top_k, top_p, min_p, stop_free=stop_free, u_index=step).ids
+            for r, tok in enumerate(picks.tolist()):
+                if not live[r]:
+                    continue
+                if not stop_free and tok in (USER_ID, ASSISTANT_ID):
+                    live[r] = False
+                    continue
+                replies[r].append(tok)
+                live[r] = stop_free or eos_token_id is None or tok != eos_token_id
+            if t + 1 == n_tokens or not any(live):
+                break
+            logits = self.decode_step(picks, step + T, slot_t, packed, down, zero)
+            step += 1
+        return replies
 
     def teacher_forced_logits(self, prompt: torch.Tensor, forced: Sequence[int], state: FastState,
                               slot: int = 0) -> List[torch.Tensor]:
@@ -662,9 +836,13 @@ class DecodeTable:
     (``advance``), so steps run back to back without the host.  The host starts a row with
     ``admit`` (after the turn's prefill) and reads the rows back asynchronously with
     ``snapshot`` / ``read``, one step behind, to stream tokens and retire finished turns.
-    Idle and finished rows are padding rows: KV slot ``pad_slot``, state -1."""
+    Idle and finished rows are padding rows: KV slot ``pad_slot``, state -1.
 
-    def __init__(self, device: torch.device, rows: int, pad_slot: int, stop_free: bool):
+    ``uniforms`` > 0: the rows also hold sampling settings and that many random numbers each
+    (``sampling.SamplingRows``), and a captured step over the table picks with ``uttt_sample``; rows at
+    temperature 0 pick greedily."""
+
+    def __init__(self, device: torch.device, rows: int, pad_slot: int, stop_free: bool, uniforms: int = 0):
         self.device = device
         self.rows = rows
         self.pad_slot = int(pad_slot)
@@ -679,6 +857,7 @@ class DecodeTable:
         self.eos = torch.full((rows,), -1, **i32)
         self.status = torch.full((rows,), _lib.ROW_IDLE, **i32)
         self.ring = torch.zeros(rows, _lib.ENGINE_RING, **i32)
+        self.sampling = sampling.SamplingRows(device, rows, uniforms) if uniforms else None
         self.lib = _lib.load()
         # two pinned host copies of (produced, status, ring), written alternately
         self._host = [(torch.empty(rows, dtype=torch.int32).pin_memory(),
@@ -772,7 +951,13 @@ class DecodeGraph:
 
     def _body(self):
         lg = self.engine.decode_step(self.tokens, self.pos, self.slots, self.read_packed, self.read_down, self.sidx)
-        ids, top2 = self.engine.greedy(lg, self.stop_free)
+        rows = None if self.table is None else self.table.sampling
+        if rows is None:
+            ids, top2 = self.engine.greedy(lg, self.stop_free)
+        else:      # reply token n of a row is picked with the row's number n
+            ids = self.engine.sample(lg, stop_free=self.stop_free, u_index=self.table.produced[:self.batch],
+                                     **rows.first(self.batch)).ids
+            top2 = None
         if self.table is not None:
             self.table.advance(ids, self.batch)
         return lg, ids, top2

@@ -42,6 +42,50 @@ def check_settings(temperature: float = 1.0, top_k: Optional[int] = None, top_p:
         raise ValueError("min_p must be finite and in [0, 1]")
 
 
+def reply_uniforms(n: int, seed: int) -> torch.Tensor:
+    """The ``n`` uniform numbers in [0, 1) of a reply with this seed (host FP32): token t is picked with number t."""
+    return torch.rand(n, generator=torch.Generator().manual_seed(seed), dtype=torch.float32)
+
+
+class SamplingRows:
+    """The sampling settings and random numbers of a packed batch's rows, in device memory, where captured steps
+    read them.  A row at temperature 0, as all are at first, picks greedily."""
+
+    def __init__(self, device: torch.device, rows: int, uniforms: int):
+        self.device = torch.device(device)
+        self.uniforms = int(uniforms)
+        self.temperature = torch.zeros(rows, device=device)
+        self.top_k = torch.zeros(rows, dtype=torch.int32, device=device)
+        self.top_p = torch.ones(rows, device=device)
+        self.min_p = torch.zeros(rows, device=device)
+        self.u = torch.zeros(rows, self.uniforms, device=device)
+
+    def set(self, row: int, temperature: float = 0.0, top_k: Optional[int] = None, top_p: Optional[float] = None,
+            min_p: Optional[float] = None, u: Optional[torch.Tensor] = None) -> None:
+        """Give ``row`` its settings and, at temperature > 0, its numbers (host FP32), on the current stream."""
+        check_settings(temperature, top_k, top_p, min_p)
+        if not 0 <= row < self.temperature.shape[0]:
+            raise ValueError("row outside the table")
+        if u is not None and u.numel() > self.uniforms:
+            raise ValueError(f"a row holds {self.uniforms} random numbers")
+
+        def put(dst: torch.Tensor, values: torch.Tensor) -> None:
+            if self.device.type == "cuda":
+                values = values.pin_memory()
+            dst.copy_(values, non_blocking=True)
+        put(self.temperature[row:row + 1], torch.tensor([float(temperature)]))
+        put(self.top_k[row:row + 1], torch.tensor([int(top_k or 0)], dtype=torch.int32))
+        put(self.top_p[row:row + 1], torch.tensor([1.0 if top_p is None else float(top_p)]))
+        put(self.min_p[row:row + 1], torch.tensor([float(min_p or 0.0)]))
+        if u is not None and u.numel():
+            put(self.u[row, :u.numel()], u.to(torch.float32).reshape(-1))
+
+    def first(self, n: int) -> dict:
+        """The arguments of ``sample`` for the first ``n`` rows."""
+        return dict(u=self.u[:n], temperature=self.temperature[:n], top_k=self.top_k[:n], top_p=self.top_p[:n],
+                    min_p=self.min_p[:n])
+
+
 def _per_row(name: str, v: Setting, off, dtype: torch.dtype, rows: int, device: torch.device):
     """(device pointer or None, value for all rows)."""
     if isinstance(v, torch.Tensor):

@@ -33,7 +33,7 @@ from typing import Any, Callable, Deque, Dict, Generator, List, Optional
 
 import torch
 
-from . import _lib
+from . import _lib, sampling
 from .fastweight import _stream, workspace
 from .model import EOS_ID, PAD_ID, DecodeGraph, DecodeTable, FastState, UtttB200, _host_list
 
@@ -209,15 +209,22 @@ class Turn:
     # front end passes the reference's re-tokenised "<|user|> ... <|assistant|> ..." turn
     # (engine/personalizer.py:480-489) here.
     write_ids: Optional[Callable[[List[int], List[int]], List[int]]] = None
+    # sampling settings (temperature 0: greedy) and the seed of the turn's random numbers
+    temperature: float = 0.0
+    top_k: Optional[int] = None
+    top_p: Optional[float] = None
+    min_p: Optional[float] = None
+    seed: Optional[int] = None
 
 
 class ServingEngine:
-    """Continuous batching of persona turns on one GPU (greedy decoding)."""
+    """Continuous batching of persona turns on one GPU (greedy decoding; with ``max_sampled_tokens`` also sampled)."""
 
     def __init__(self, engine: UtttB200, capacity: int, max_batch: int, surprise_threshold: float = 0.25,
                  elastic_anchor_lambda: float = 0.02, max_weight_drift_ratio: Optional[float] = 0.35,
                  online_ttt: bool = True, stop_free: bool = False, write_batch: int = 8,
-                 write_wait_s: float = 0.05, async_writes: bool = False, prefill_budget: int = 16384):
+                 write_wait_s: float = 0.05, async_writes: bool = False, prefill_budget: int = 16384,
+                 max_sampled_tokens: int = 0):
         """``prefill_budget``: turns admitted in one step are prefilled together (one batched prefill, the
         prompts packed one after another) up to this many prompt tokens.
         ``stop_free``: replies run to their ``max_new_tokens`` (role ids and EOS are masked
@@ -230,7 +237,10 @@ class ServingEngine:
         is done (and its user's next turn admitted) only after its write has landed.
         Off by default: both paths are HBM-bound, so overlapping them slows each, and
         on the 151M serve sweep at 32 req/s it raised the mean latency from 0.72 s to
-        3.1 s (writes between steps form fewer, larger batches)."""
+        3.1 s (writes between steps form fewer, larger batches).
+        ``max_sampled_tokens`` > 0: turns may ask for a temperature, for replies of up to that many tokens; every
+        captured step then picks with ``uttt_sample``, row by row with the turn's own settings and random
+        numbers, and turns without a temperature stay greedy."""
         self.engine = engine
         self._w0_norm2: Optional[List[float]] = None
         self.stop_free = stop_free
@@ -262,7 +272,9 @@ class ServingEngine:
         # host.  One captured step per batch bucket (1, 2, 4, ... max_batch) over the table's first rows: a
         # step runs the smallest bucket that holds every row in use; idle and finished rows are padding rows
         # (padding slot, no fast-weight state) and read no weights.
-        self.table = DecodeTable(engine.device, max_batch, self.arena.pad_slot, stop_free)
+        self.max_sampled_tokens = max(0, int(max_sampled_tokens))
+        more = {"uniforms": self.max_sampled_tokens} if self.max_sampled_tokens else {}
+        self.table = DecodeTable(engine.device, max_batch, self.arena.pad_slot, stop_free, **more)
         sizes, b = [], 1
         while b < max_batch:
             sizes.append(b)
@@ -287,13 +299,26 @@ class ServingEngine:
     # ------------------------------------------------------------------ API
     def submit(self, user_id: str, prompt_ids: List[int], max_new_tokens: int = 128,
                eos_token_id: Optional[int] = EOS_ID, on_event: Optional[Callable[[dict], None]] = None,
-               write_ids: Optional[Callable[[List[int], List[int]], List[int]]] = None) -> Turn:
+               write_ids: Optional[Callable[[List[int], List[int]], List[int]]] = None, temperature: float = 0.0,
+               top_k: Optional[int] = None, top_p: Optional[float] = None, min_p: Optional[float] = None,
+               seed: Optional[int] = None) -> Turn:
+        """Queue a turn.  At ``temperature`` > 0 (an engine with ``max_sampled_tokens``) reply token t is sampled
+        with number t of ``sampling.reply_uniforms(max_new_tokens, seed)``; without a seed one is drawn from
+        torch's global generator and kept in ``Turn.seed``."""
         if not prompt_ids:
             raise ValueError("empty prompt")
         if type(max_new_tokens) is not int or max_new_tokens < 1:
             raise ValueError("max_new_tokens must be a positive integer")
+        sampling.check_settings(temperature, top_k, top_p, min_p)
+        if temperature > 1e-5:
+            if max_new_tokens > self.max_sampled_tokens:
+                raise ValueError(f"this engine samples replies of up to {self.max_sampled_tokens} tokens "
+                                 "(max_sampled_tokens)")
+            if seed is None:
+                seed = int(torch.randint(2 ** 62, ()).item())
         t = Turn(str(user_id), list(prompt_ids), max_new_tokens, eos_token_id, on_event=on_event,
-                 write_ids=write_ids)
+                 write_ids=write_ids, temperature=float(temperature), top_k=top_k, top_p=top_p, min_p=min_p,
+                 seed=seed)
         self.waiting.append(t)
         return t
 
@@ -408,7 +433,7 @@ class ServingEngine:
         logits = e.prefill_batch([torch.tensor(t.prompt_ids, dtype=torch.long) for t in admitted],
                                  [t.slot for t in admitted], self.arena.read_packed, self.arena.read_down,
                                  [t.slot for t in admitted])
-        picks, _ = e.greedy(logits, stop_free=self.stop_free)
+        picks = self._first_picks(logits, admitted)
         for i, t in enumerate(admitted):
             self.table.admit(t.row, picks[i:i + 1], len(t.prompt_ids), t.slot, t.slot, t.max_new_tokens,
                              t.eos_token_id)
@@ -416,6 +441,20 @@ class ServingEngine:
         self.stats["prefill_s"] += time.perf_counter() - t0
         self.stats["prefill_tokens"] += tokens
         self.stats["prefill_batches"] += 1
+
+    def _first_picks(self, logits: torch.Tensor, admitted: List[Turn]) -> torch.Tensor:
+        """Reply token 0 of every admitted turn from its prompt's last logits; an engine that samples also gives the
+        turns' rows their settings and numbers for the steps to come."""
+        e = self.engine
+        if not self.max_sampled_tokens:
+            return e.greedy(logits, stop_free=self.stop_free)[0]
+        rows, here = self.table.sampling, sampling.SamplingRows(e.device, len(admitted), 1)
+        for i, t in enumerate(admitted):
+            s = dict(temperature=t.temperature, top_k=t.top_k, top_p=t.top_p, min_p=t.min_p)
+            u = sampling.reply_uniforms(t.max_new_tokens, t.seed) if t.temperature > 1e-5 else None
+            rows.set(t.row, u=u, **s)
+            here.set(i, u=None if u is None else u[:1], **s)
+        return e.sample(logits, stop_free=self.stop_free, **here.first(len(admitted))).ids
 
     def _harvest(self, buf: int, bucket: int, seq: int) -> None:
         """Take the results of decode step ``seq`` (snapshot ``buf``): the reply tokens each turn yielded

@@ -8,7 +8,7 @@ The reference drafts along one line (``model/uttt_model.py:1052-1179``).
 
 from __future__ import annotations
 
-from typing import Optional, Sequence, Tuple
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -25,6 +25,57 @@ def check_tree(parents: Sequence[int]) -> None:
         raise ValueError(f"a drafted tree has 1 to {MAX_NODES} nodes")
     if parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(parents) if i > 0):
         raise ValueError("node 0 is the root (parent -1) and a node's parent comes before it")
+
+
+def depths(parents: Sequence[int]) -> List[int]:
+    """How many ancestors each node of a host-side tree has."""
+    out: List[int] = []
+    for p in parents:
+        out.append(0 if p < 0 else out[p] + 1)
+    return out
+
+
+def prune(tokens: Sequence[int], parents: Sequence[int], depth: Sequence[int], most: int):
+    """(tokens, parents, depth) of the nodes at most ``most`` deep."""
+    keep = [i for i, d in enumerate(depth) if d <= most]
+    at = {i: k for k, i in enumerate(keep)}
+    return ([tokens[i] for i in keep], [-1 if parents[i] < 0 else at[parents[i]] for i in keep],
+            [depth[i] for i in keep])
+
+
+class PromptLookup:
+    """Drafts from the text itself: what followed earlier occurrences of the last few ids, the latest first, merged
+    into one tree.  An instance is a ``draft`` of ``UtttB200.generate_drafted``."""
+
+    def __init__(self, match: int = 2, depth: int = 8, nodes: int = 16):
+        """``match`` ids must agree (fewer at the start of a text); continuations of up to ``depth`` ids; at most
+        ``nodes`` drafted ids."""
+        if match < 1 or depth < 1 or not 1 <= nodes < MAX_NODES:
+            raise ValueError(f"match and depth must be positive and nodes between 1 and {MAX_NODES - 1}")
+        self.match, self.depth, self.nodes = match, depth, nodes
+
+    def __call__(self, ids: Sequence[int]) -> Tuple[List[int], List[int]]:
+        n = min(self.match, len(ids))
+        last = list(ids[-n:])
+        tokens: List[int] = []
+        parents: List[int] = []
+        child = {}
+        for at in range(len(ids) - n - 1, -1, -1):
+            if len(tokens) >= self.nodes:
+                break
+            if list(ids[at:at + n]) != last:
+                continue
+            node = 0
+            for tok in ids[at + n:at + n + self.depth]:
+                nxt = child.get((node, tok))
+                if nxt is None:
+                    if len(tokens) >= self.nodes:
+                        break
+                    tokens.append(int(tok))
+                    parents.append(node)
+                    nxt = child[(node, tok)] = len(tokens)
+                node = nxt
+        return tokens, parents
 
 
 def _int_rows(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[int]:
