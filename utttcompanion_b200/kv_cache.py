@@ -27,27 +27,29 @@ def ring_commit(rings: torch.Tensor, tree_kv: torch.Tensor, pos: torch.Tensor, s
     """Put an accepted path into the rings, in place: node ``path[b, t]`` of ``tree_kv`` BF16
     (2, layers, B, n_kv, N, hd) at position ``pos[b] + t`` of slot ``slots[b]``, t < ``n_path[b]``
     (int32 device tensors of ``tree.tree_accept``; the slots of a batch must differ)."""
-    _require_cuda(rings, tree_kv, pos, slots, path, n_path)
+    _require_cuda(rings)
     _check_rings(rings)
     _, L, S, n_kv, W, hd = rings.shape
-    dev = rings.device
-    if tree_kv.dim() != 6 or tree_kv.dtype != torch.bfloat16 or not tree_kv.is_contiguous() or tree_kv.device != dev:
+    index = rings.get_device()
+    if tree_kv.get_device() != index or tree_kv.dtype is not torch.bfloat16 or tree_kv.dim() != 6 \
+            or not tree_kv.is_contiguous():
         raise ValueError("tree_kv must be contiguous BF16 (2, layers, B, n_kv, N, hd) beside the rings")
-    B, N = tree_kv.shape[2], tree_kv.shape[4]
-    if tree_kv.shape != (2, L, B, n_kv, N, hd) or not 1 <= N <= MAX_NODES:
+    two, layers, B, heads, N, width = tree_kv.shape
+    if (two, layers, heads, width) != (2, L, n_kv, hd) or not 1 <= N <= MAX_NODES:
         raise ValueError("tree_kv does not fit the rings' layers and heads")
-    ptrs = (_int_rows("pos", pos, (B,), dev), _int_rows("slots", slots, (B,), dev),
-            _int_rows("path", path, (B, N), dev), _int_rows("n_path", n_path, (B,), dev))
+    rows = (B,)
+    ptrs = (_int_rows("pos", pos, rows, index), _int_rows("slots", slots, rows, index),
+            _int_rows("path", path, (B, N), index), _int_rows("n_path", n_path, rows, index))
     if B == 0:
         return
     tree_stride, ring_stride = B * n_kv * N * hd, S * n_kv * W * hd
     t, r = tree_kv.data_ptr(), rings.data_ptr()
-    on, stream = _launch(dev)
+    on, stream = _launch(rings.device)
     with on:
         st = _lib.load().uttt_kv_ring_commit(L, B, N, n_kv, hd, W, S, t, t + 2 * L * tree_stride, tree_stride, r,
-                                             r + 2 * L * ring_stride, ring_stride, *ptrs,
-                                             stream)
-    _lib.check(st, "uttt_kv_ring_commit")
+                                             r + 2 * L * ring_stride, ring_stride, *ptrs, stream)
+    if st:
+        _lib.check(st, "uttt_kv_ring_commit")
 
 
 def ring_fork(rings: torch.Tensor, src: Sequence[int], dst: Sequence[int],

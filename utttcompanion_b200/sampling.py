@@ -86,11 +86,11 @@ class SamplingRows:
                     min_p=self.min_p[:n])
 
 
-def _per_row(name: str, v: Setting, off, dtype: torch.dtype, rows: int, device: torch.device):
+def _per_row(name: str, v: Setting, off, dtype: torch.dtype, rows: int, index: int):
     """(device pointer or None, value for all rows)."""
     if isinstance(v, torch.Tensor):
-        if v.dtype is not dtype or v.shape != (rows,) or not v.is_contiguous() or v.device != device:
-            raise ValueError(f"{name} per row must be a contiguous {dtype} tensor of {rows} on {device}")
+        if v.get_device() != index or v.dtype is not dtype or v.shape != (rows,) or not v.is_contiguous():
+            raise ValueError(f"{name} per row must be a contiguous {dtype} tensor of {rows} on cuda:{index}")
         return v.data_ptr(), off
     return None, off if v is None else v
 
@@ -106,46 +106,49 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
     a temperature of at most 1e-5 picks greedily, ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0 are off.
     PAD / BOS / UNK and ids from ``active_limit`` on are never picked (nor ids 2, 4 and 5 when
     ``stop_free``), as by ``UtttB200.greedy``.  Runs on the current stream of the logits' device."""
-    _require_cuda(logits, u, u_index)
-    dev, f = logits.device, torch.float32
+    _require_cuda(logits, u)
+    f, index = torch.float32, logits.get_device()
     is_f32 = logits.dtype is f
-    if logits.dim() != 2 or not (is_f32 or logits.dtype is torch.bfloat16) or logits.shape[1] <= 6:
+    if logits.dim() != 2 or not (is_f32 or logits.dtype is torch.bfloat16):
         raise ValueError("logits must be FP32 or BF16 (rows, V) with V > 6")
     rows, V = logits.shape
+    if V <= 6:
+        raise ValueError("logits must be FP32 or BF16 (rows, V) with V > 6")
+    n_u = 1 if u.dim() == 1 else u.shape[-1]
+    if u.get_device() != index or u.dtype is not f or u.dim() > 2 or u.shape[0] != rows or not u.is_contiguous():
+        raise ValueError("u must be a contiguous FP32 (rows,) or (rows, n) tensor beside the logits")
     if rows == 0:
-        return Sampled(*(torch.empty(0, dtype=t, device=dev) for t in (torch.int32, torch.int32, f)))
+        return Sampled(*(torch.empty(0, dtype=t, device=logits.device) for t in (torch.int32, torch.int32, f)))
     ld, step = logits.stride()
     if step != 1 or (rows > 1 and ld < V):
         logits = logits.contiguous()
         ld = V
-    n_u = 1 if u.dim() == 1 else u.shape[-1]
-    if u.dtype is not f or u.dim() > 2 or u.shape[0] != rows or n_u == 0 or not u.is_contiguous() or u.device != dev:
-        raise ValueError("u must be a contiguous FP32 (rows,) or (rows, n) tensor beside the logits")
     if u_index is None:
+        at = None
         if n_u != 1:
             raise ValueError("u of several numbers a row needs u_index")
-        index = None
-    elif u_index.dtype is not torch.int32 or u_index.shape != (rows,) or not u_index.is_contiguous() \
-            or u_index.device != dev:
+    elif u_index.get_device() != index or u_index.dtype is not torch.int32 or u_index.shape != (rows,) \
+            or not u_index.is_contiguous() or n_u == 0:
         raise ValueError("u_index must be a contiguous int32 (rows,) tensor beside the logits")
     else:
-        index = u_index.data_ptr()
+        at = u_index.data_ptr()
     limit = V if active_limit is None else int(active_limit)
     if limit <= 2:
         raise ValueError("Active vocabulary must include EOS")
-    tp, t0 = _per_row("temperature", temperature, 1.0, f, rows, dev)
-    kp, k0 = _per_row("top_k", top_k, 0, torch.int32, rows, dev)
-    pp, p0 = _per_row("top_p", top_p, 1.0, f, rows, dev)
-    mp, m0 = _per_row("min_p", min_p, 0.0, f, rows, dev)
+    tp, t0 = _per_row("temperature", temperature, 1.0, f, rows, index)
+    kp, k0 = _per_row("top_k", top_k, 0, torch.int32, rows, index)
+    pp, p0 = _per_row("top_p", top_p, 1.0, f, rows, index)
+    mp, m0 = _per_row("min_p", min_p, 0.0, f, rows, index)
     check_settings(t0, k0, p0, m0)
     opt = _lib.Sampling(tp, kp, pp, mp, t0, int(k0), p0, m0)
-    ids = torch.empty(rows, dtype=torch.int32, device=dev)
-    kept = torch.empty(rows, dtype=torch.int32, device=dev)
-    prob = torch.empty(rows, dtype=f, device=dev)
-    on, stream = _launch(dev)
+    prob = torch.empty_like(u) if u.dim() == 1 else torch.empty(rows, dtype=f, device=u.device)
+    ids = torch.empty(rows, dtype=torch.int32, device=u.device)
+    kept = torch.empty_like(ids)
+    on, stream = _launch(u.device)
     with on:
         st = _lib.load().uttt_sample(rows, V, logits.data_ptr(), is_f32, ld if rows > 1 else V, limit, bool(stop_free),
-                                     C.byref(opt), u.data_ptr(), n_u, index, n_u, ids.data_ptr(), kept.data_ptr(),
+                                     C.byref(opt), u.data_ptr(), n_u, at, n_u, ids.data_ptr(), kept.data_ptr(),
                                      prob.data_ptr(), stream)
-    _lib.check(st, "uttt_sample")
+    if st:
+        _lib.check(st, "uttt_sample")
     return Sampled(ids, kept, prob)

@@ -78,11 +78,12 @@ class PromptLookup:
         return tokens, parents
 
 
-def _int_rows(name: str, t: Optional[torch.Tensor], shape, device) -> Optional[int]:
+def _int_rows(name: str, t: Optional[torch.Tensor], shape, index: int) -> Optional[int]:
+    """Address of a contiguous int32 tensor of this shape on CUDA device ``index`` (None for None)."""
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.shape != shape or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 {shape} tensor on {device}")
+    if t.get_device() != index or t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 {tuple(shape)} tensor on cuda:{index}")
     return t.data_ptr()
 
 
@@ -99,49 +100,56 @@ def tree_attention(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, 
     ``n_nodes`` int32 (B,): nodes of each row (default N).  ``out`` BF16 (B * N, n_heads * hd), rows any stride,
     ``k_tree`` / ``v_tree`` BF16 (B, n_kv, N, hd): taken if given, else new (zeros); what lies behind a row's last
     node is left as it was."""
-    _require_cuda(qkv, parents, pos, slots, k_ring, v_ring, rope_cos, rope_sin, n_nodes, out, k_tree, v_tree)
-    dev, bf = qkv.device, torch.bfloat16
+    _require_cuda(qkv, parents)
+    dev, bf, index = qkv.device, torch.bfloat16, qkv.get_device()
     if parents.dim() != 2 or k_ring.dim() != 4:
         raise ValueError("parents must be (B, N) and the rings (slots, n_kv, W, hd)")
     B, N = parents.shape
     n_slots, n_kv, W, hd = shape = k_ring.shape
-    if k_ring.dtype is not bf or v_ring.dtype is not bf or v_ring.shape != shape or not k_ring.is_contiguous() \
-            or not v_ring.is_contiguous() or k_ring.device != dev or v_ring.device != dev or 0 in shape:
-        raise ValueError("the rings must be contiguous BF16 tensors of one shape beside qkv")
+    for t in (k_ring, v_ring):
+        if t.get_device() != index or t.dtype is not bf or t.shape != shape or not t.is_contiguous() or 0 in shape:
+            raise ValueError("the rings must be contiguous BF16 tensors of one shape beside qkv")
     if not 1 <= N <= MAX_NODES:
         raise ValueError(f"a drafted tree has 1 to {MAX_NODES} nodes")
-    q_dim = n_heads * hd
-    if n_heads < 1 or n_heads % n_kv or qkv.dtype is not bf or qkv.dim() != 2 or qkv.shape[0] != B * N \
-            or qkv.shape[1] < q_dim + 2 * n_kv * hd or qkv.stride(1) != 1:
+    R, q_dim = B * N, n_heads * hd
+    if n_heads < 1 or n_heads % n_kv or qkv.dtype is not bf or qkv.dim() != 2 or qkv.shape[0] != R:
+        raise ValueError("qkv must be BF16 (B * N, (n_heads + 2 * n_kv) * hd) rows")
+    qkv_ld, step = qkv.stride()
+    if step != 1 or qkv.shape[1] < q_dim + 2 * n_kv * hd:
         raise ValueError("qkv must be BF16 (B * N, (n_heads + 2 * n_kv) * hd) rows")
     table = rope_cos.shape
     for t in (rope_cos, rope_sin):
-        if t.dtype is not torch.float32 or t.shape != table or len(table) != 2 or table[1] != hd or table[0] < 1 \
-                or not t.is_contiguous() or t.device != dev:
+        if t.get_device() != index or t.dtype is not torch.float32 or t.shape != table or not t.is_contiguous():
             raise ValueError("rope_cos and rope_sin must be contiguous FP32 (positions, hd) tables")
+    if len(table) != 2 or table[1] != hd or table[0] < 1:
+        raise ValueError("rope_cos and rope_sin must be contiguous FP32 (positions, hd) tables")
     if out is None:
-        out = torch.zeros(B * N, q_dim, dtype=bf, device=dev)
-    elif out.dtype is not bf or out.shape != (B * N, q_dim) or out.stride(1) != 1 or out.device != dev:
+        out = torch.zeros(R, q_dim, dtype=bf, device=dev)
+    elif out.get_device() != index or out.dtype is not bf or out.shape != (R, q_dim):
+        raise ValueError("out must be BF16 (B * N, n_heads * hd) rows")
+    out_ld, step = out.stride()
+    if step != 1 and R:
         raise ValueError("out must be BF16 (B * N, n_heads * hd) rows")
     kv_shape = (B, n_kv, N, hd)
     k_tree = torch.zeros(kv_shape, dtype=bf, device=dev) if k_tree is None else k_tree
     v_tree = torch.zeros(kv_shape, dtype=bf, device=dev) if v_tree is None else v_tree
     for t in (k_tree, v_tree):
-        if t.dtype is not bf or t.shape != kv_shape or not t.is_contiguous() or t.device != dev:
+        if t.get_device() != index or t.dtype is not bf or t.shape != kv_shape or not t.is_contiguous():
             raise ValueError("k_tree and v_tree must be contiguous BF16 (B, n_kv, N, hd)")
-    args = (_int_rows("parents", parents, (B, N), dev), _int_rows("n_nodes", n_nodes, (B,), dev),
-            _int_rows("pos", pos, (B,), dev), _int_rows("slots", slots, (B,), dev))
+    rows = (B,)
+    args = (_int_rows("parents", parents, (B, N), index), _int_rows("n_nodes", n_nodes, rows, index),
+            _int_rows("pos", pos, rows, index), _int_rows("slots", slots, rows, index))
     if B == 0:
         return out, k_tree, v_tree
-    many = B * N > 1
     on, stream = _launch(dev)
     with on:
         st = _lib.load().uttt_attn_tree(B, N, n_heads, n_kv, hd, W, n_slots, table[0], qkv.data_ptr(),
-                                        qkv.stride(0) if many else qkv.shape[1], *args, k_ring.data_ptr(),
+                                        qkv_ld if R > 1 else qkv.shape[1], *args, k_ring.data_ptr(),
                                         v_ring.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
                                         k_tree.data_ptr(), v_tree.data_ptr(), out.data_ptr(),
-                                        out.stride(0) if many else q_dim, stream)
-    _lib.check(st, "uttt_attn_tree")
+                                        out_ld if R > 1 else q_dim, stream)
+    if st:
+        _lib.check(st, "uttt_attn_tree")
     return out, k_tree, v_tree
 
 
@@ -152,20 +160,23 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     ``tokens``, ``parents``, ``picks`` int32 (B, N): each node's drafted token and parent, and the model's pick
     after it.  The path is node 0, then from each node on its lowest later child that holds the pick; -1 behind
     its last node, whose pick is ``next``."""
-    _require_cuda(tokens, parents, picks, n_nodes)
-    if tokens.dim() != 2 or not 1 <= tokens.shape[1] <= MAX_NODES:
-        raise ValueError(f"tokens must be (B, N) with 1 to {MAX_NODES} nodes")
-    dev, shape = tokens.device, tokens.shape
+    _require_cuda(tokens)
+    if tokens.dim() != 2:
+        raise ValueError("tokens must be (B, N)")
+    index, shape = tokens.get_device(), tokens.shape
     B, N = shape
-    ptrs = (_int_rows("tokens", tokens, shape, dev), _int_rows("parents", parents, shape, dev),
-            _int_rows("n_nodes", n_nodes, (B,), dev), _int_rows("picks", picks, shape, dev))
-    path = torch.empty(B, N, dtype=torch.int32, device=dev)
-    n_path = torch.empty(B, dtype=torch.int32, device=dev)
-    following = torch.empty(B, dtype=torch.int32, device=dev)
+    if not 1 <= N <= MAX_NODES:
+        raise ValueError(f"a drafted tree has 1 to {MAX_NODES} nodes")
+    ptrs = (_int_rows("tokens", tokens, shape, index), _int_rows("parents", parents, shape, index),
+            _int_rows("n_nodes", n_nodes, (B,), index), _int_rows("picks", picks, shape, index))
+    path = torch.empty_like(tokens)
+    n_path = torch.empty(B, dtype=torch.int32, device=tokens.device) if n_nodes is None else torch.empty_like(n_nodes)
+    following = torch.empty_like(n_path)
     if B:
-        on, stream = _launch(dev)
+        on, stream = _launch(tokens.device)
         with on:
             st = _lib.load().uttt_tree_accept(B, N, *ptrs, path.data_ptr(), n_path.data_ptr(), following.data_ptr(),
                                               stream)
-        _lib.check(st, "uttt_tree_accept")
+        if st:
+            _lib.check(st, "uttt_tree_accept")
     return path, n_path, following
