@@ -1,9 +1,9 @@
 """GPU: uttt_sample against the 64-bit rule, row by row.
 
 The pick and the number of kept ids must be equal.  A probability is one rounding to FP32 (2^-24 relative) of a
-quotient w / sum w of weights that are each off by at most 2^-29 of themselves (x by 2^-33, so 2^-33.5; the table entry
-by 2^-31; the polynomial by 2^-30.5, two roundings of a number below 2^-7.5; the product by 2^-31) and rounded to a whole
-number of 2^-45 of the largest: |error| <= (2^-24 + 2 * 2^-29) p + n 2^-46.
+quotient w / sum w of weights.  Each weight is a whole number of 2^-45 of the largest; from 2^-24 on it is off by at most
+2^-38 of itself before that rounding (the polynomial), below by 2^-19 (x of at most 64 from three FP32 roundings, 2^-24
+each, and 2^-x by 2^-22), which is 2^-43 of the largest.  So |error| <= (2^-24 + 2^-37 + n 2^-42) p + n 2^-46.
 """
 
 import math
@@ -26,7 +26,7 @@ def _check(x, u, ids, kept, prob, settings, limit=None, stop_free=False):
         s = {k: (v[r].item() if isinstance(v, torch.Tensor) else v) for k, v in settings.items() if v is not None}
         want = sample_row(x[r], u[r], limit=limit, stop_free=stop_free, **s)
         assert (ids[r], kept[r]) == want[:2], (r, s, ids[r], kept[r], want)
-        assert abs(prob[r] - want[2]) <= (2.0 ** -24 + 2.0 ** -28) * want[2] + x.shape[1] * 2.0 ** -46, (r, prob[r], want)
+        assert abs(prob[r] - want[2]) <= (2.0 ** -24 + 2.0 ** -37 + x.shape[1] * 2.0 ** -42) * want[2] + x.shape[1] * 2.0 ** -46, (r, prob[r], want)
 
 
 def _logits(rows, V, dtype, seed, std=2.0):

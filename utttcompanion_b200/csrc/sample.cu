@@ -12,16 +12,17 @@
 // is one cut element.  The pick is the lowest id i with (sum of kept w_j, j <= i)
 // > u * (sum of all kept w_j).
 //
-// Whole-number weights.  x_i is computed in 64 bits and taken to a whole number of
-// 2^-32; 2^-x_i comes from its integer part (a shift), the next 7 bits (a table of
-// 2^(-j/128)) and the rest (a cubic Taylor polynomial: the table-driven method of
-// Tang, ACM TOMS 15, 1989), as a whole number of 2^-45, good to 2^-29 of itself
-// (all carry one common factor, 1 - 2^-20, which keeps the table within 32 bits
-// and leaves every ratio alone).  Weights below 2^-24 take x and 2^-x from FP32
+// Whole-number weights.  x_i is computed in 64 bits and split into the nearest k / 128
+// and the rest; 2^-x_i comes from the integer part of k / 128 (the exponent), the
+// other 7 bits of k (a table of 2^(-j/128)) and the rest (a cubic Taylor polynomial:
+// the table-driven method of Tang, ACM TOMS 15, 1989), good to 2^-38 of itself and
+// rounded to a whole number of 2^-45.  Weights below 2^-24 take x and 2^-x from FP32
 // instead: off by 2^-19 of themselves, they are still good to 2^-43 of the largest.
-// So every sum of weights is an exact 64-bit
-// integer that does not depend on the order of the additions: histograms with
+// So every sum of weights is an exact integer (64-bit, or in a double while it is
+// below 2^53) that does not depend on the order of the additions: histograms with
 // atomics, splits over CTAs and any grid give the same cut and the same pick.
+// 64-bit floating point, because its pipe is idle: with the same steps in 32-bit
+// integers the half-rate integer pipe was 60 % busy and bound the kernel.
 //
 // Layout.  One cluster of S CTAs per row; each warp owns a contiguous piece of the
 // row and streams it in 16-byte loads, once per step (the row comes from HBM once
@@ -65,7 +66,7 @@ struct Sel {     // value exchanged between the CTAs of a cluster
 
 struct SampleShared {
   uint4 ring[SM_WARPS][SM_RING * 32];    // vectors on their way
-  unsigned tab[SM_STEPS * 32];           // the table once per lane: no bank conflicts
+  double tab[SM_STEPS * 16];             // the table 16 times: the lanes of a half-warp meet no bank conflicts
   Sel xch[2][SM_MAX_CTAS];               // one slot per CTA, two phases
   u64 wred[SM_WARPS], wred2[SM_WARPS];
   u64 cand[2][SM_CAP];                   // rank 0: gathered candidates; others: their copies of them
@@ -76,24 +77,40 @@ struct SampleShared {
   alignas(16) unsigned hist[3][SM_BINS];  // count, or 16-bit limbs of the mass
 };
 
-// floor(2^32 * 2^(-j / 128) * (1 - 2^-20))
-__device__ const unsigned kPow2[SM_STEPS] = {
-    0xfffff000u, 0xfe9e0172u, 0xfd3dfc39u, 0xfbdfddaeu, 0xfa83a333u, 0xf9294a28u, 0xf7d0cff5u, 0xf67a3204u,
-    0xf5256dc2u, 0xf3d280a1u, 0xf2816814u, 0xf1322194u, 0xefe4aa9du, 0xee9900aeu, 0xed4f2149u, 0xec0709f5u,
-    0xeac0b83bu, 0xe97c29a8u, 0xe8395bccu, 0xe6f84c3bu, 0xe5b8f88bu, 0xe47b5e58u, 0xe33f7b3eu, 0xe2054cdfu,
-    0xe0ccd0dfu, 0xdf9604e5u, 0xde60e69cu, 0xdd2d73b2u, 0xdbfba9d8u, 0xdacb86c2u, 0xd99d0828u, 0xd8702bc5u,
-    0xd744ef56u, 0xd61b509cu, 0xd4f34d5cu, 0xd3cce35cu, 0xd2a81067u, 0xd184d24au, 0xd06326d4u, 0xcf430bdau,
-    0xce247f32u, 0xcd077eb5u, 0xcbec0840u, 0xcad219b1u, 0xc9b9b0eau, 0xc8a2cbd2u, 0xc78d684fu, 0xc679844eu,
-    0xc5671dbau, 0xc4563286u, 0xc346c0a5u, 0xc238c60du, 0xc12c40b7u, 0xc0212e9fu, 0xbf178dc5u, 0xbe0f5c28u,
-    0xbd0897ceu, 0xbc033ebeu, 0xbaff4f02u, 0xb9fcc6a5u, 0xb8fba3b7u, 0xb7fbe44au, 0xb6fd8673u, 0xb6008848u,
-    0xb504e7e3u, 0xb40aa361u, 0xb311b8e1u, 0xb21a2684u, 0xb123ea6fu, 0xb02f02c8u, 0xaf3b6db9u, 0xae49296eu,
-    0xad583414u, 0xac688bdeu, 0xab7a2efeu, 0xaa8d1baau, 0xa9a1501au, 0xa8b6ca8bu, 0xa7cd8938u, 0xa6e58a61u,
-    0xa5fecc49u, 0xa5194d35u, 0xa4350b6au, 0xa3520533u, 0xa27038dcu, 0xa18fa4b1u, 0xa0b04704u, 0x9fd21e28u,
-    0x9ef52871u, 0x9e196437u, 0x9d3ecfd3u, 0x9c6569a1u, 0x9b8d3001u, 0x9ab62151u, 0x99e03bf5u, 0x990b7e51u,
-    0x9837e6ceu, 0x976573d3u, 0x969423cdu, 0x95c3f52au, 0x94f4e659u, 0x9426f5cdu, 0x935a21f9u, 0x928e6954u,
-    0x91c3ca57u, 0x90fa437cu, 0x9031d33fu, 0x8f6a7821u, 0x8ea430a1u, 0x8ddefb42u, 0x8d1ad689u, 0x8c57c0feu,
-    0x8b95b92au, 0x8ad4bd97u, 0x8a14ccd3u, 0x8955e56eu, 0x889805f7u, 0x87db2d02u, 0x871f5924u, 0x866488f5u,
-    0x85aabb0du, 0x84f1ee07u, 0x843a2080u, 0x83835116u, 0x82cd7e6bu, 0x8218a721u, 0x8164c9ddu, 0x80b1e544u,
+// 2^45 * 2^(-j / 128)
+__device__ const double kPow2[SM_STEPS] = {
+    0x1.0000000000000p+45, 0x1.fd3c22b8f71f1p+44, 0x1.fa7c1819e90d8p+44, 0x1.f7bfdad9cbe14p+44,
+    0x1.f50765b6e4540p+44, 0x1.f252b376bba97p+44, 0x1.efa1bee615a27p+44, 0x1.ecf482d8e67f1p+44,
+    0x1.ea4afa2a490dap+44, 0x1.e7a51fbc74c83p+44, 0x1.e502ee78b3ff6p+44, 0x1.e264614f5a129p+44,
+    0x1.dfc97337b9b5fp+44, 0x1.dd321f301b460p+44, 0x1.da9e603db3285p+44, 0x1.d80e316c98398p+44,
+    0x1.d5818dcfba487p+44, 0x1.d2f87080d89f2p+44, 0x1.d072d4a07897cp+44, 0x1.cdf0b555dc3fap+44,
+    0x1.cb720dcef9069p+44, 0x1.c8f6d9406e7b5p+44, 0x1.c67f12e57d14bp+44, 0x1.c40ab5fffd07ap+44,
+    0x1.c199bdd85529cp+44, 0x1.bf2c25bd71e09p+44, 0x1.bcc1e904bc1d2p+44, 0x1.ba5b030a1064ap+44,
+    0x1.b7f76f2fb5e47p+44, 0x1.b59728de5593ap+44, 0x1.b33a2b84f15fbp+44, 0x1.b0e07298db666p+44,
+    0x1.ae89f995ad3adp+44, 0x1.ac36bbfd3f37ap+44, 0x1.a9e6b5579fdbfp+44, 0x1.a799e1330b358p+44,
+    0x1.a5503b23e255dp+44, 0x1.a309bec4a2d33p+44, 0x1.a0c667b5de565p+44, 0x1.9e86319e32323p+44,
+    0x1.9c49182a3f090p+44, 0x1.9a0f170ca07bap+44, 0x1.97d829fde4e50p+44, 0x1.95a44cbc8520fp+44,
+    0x1.93737b0cdc5e5p+44, 0x1.9145b0b91ffc6p+44, 0x1.8f1ae99157736p+44, 0x1.8cf3216b5448cp+44,
+    0x1.8ace5422aa0dbp+44, 0x1.88ac7d98a6699p+44, 0x1.868d99b4492edp+44, 0x1.8471a4623c7adp+44,
+    0x1.82589994cce13p+44, 0x1.80427543e1a12p+44, 0x1.7e2f336cf4e62p+44, 0x1.7c1ed0130c132p+44,
+    0x1.7a11473eb0187p+44, 0x1.780694fde5d3fp+44, 0x1.75feb564267c9p+44, 0x1.73f9a48a58174p+44,
+    0x1.71f75e8ec5f74p+44, 0x1.6ff7df9519484p+44, 0x1.6dfb23c651a2fp+44, 0x1.6c012750bdabfp+44,
+    0x1.6a09e667f3bcdp+44, 0x1.68155d44ca973p+44, 0x1.6623882552225p+44, 0x1.6434634ccc320p+44,
+    0x1.6247eb03a5585p+44, 0x1.605e1b976dc09p+44, 0x1.5e76f15ad2148p+44, 0x1.5c9268a5946b7p+44,
+    0x1.5ab07dd485429p+44, 0x1.58d12d497c7fdp+44, 0x1.56f4736b527dap+44, 0x1.551a4ca5d920fp+44,
+    0x1.5342b569d4f82p+44, 0x1.516daa2cf6642p+44, 0x1.4f9b2769d2ca7p+44, 0x1.4dcb299fddd0dp+44,
+    0x1.4bfdad5362a27p+44, 0x1.4a32af0d7d3dep+44, 0x1.486a2b5c13cd0p+44, 0x1.46a41ed1d0057p+44,
+    0x1.44e086061892dp+44, 0x1.431f5d950a897p+44, 0x1.4160a21f72e2ap+44, 0x1.3fa4504ac801cp+44,
+    0x1.3dea64c123422p+44, 0x1.3c32dc313a8e5p+44, 0x1.3a7db34e59ff7p+44, 0x1.38cae6d05d866p+44,
+    0x1.371a7373aa9cbp+44, 0x1.356c55f929ff1p+44, 0x1.33c08b26416ffp+44, 0x1.32170fc4cd831p+44,
+    0x1.306fe0a31b715p+44, 0x1.2ecafa93e2f56p+44, 0x1.2d285a6e4030bp+44, 0x1.2b87fd0dad990p+44,
+    0x1.29e9df51fdee1p+44, 0x1.284dfe1f56381p+44, 0x1.26b4565e27cddp+44, 0x1.251ce4fb2a63fp+44,
+    0x1.2387a6e756238p+44, 0x1.21f49917ddc96p+44, 0x1.2063b88628cd6p+44, 0x1.1ed5022fcd91dp+44,
+    0x1.1d4873168b9aap+44, 0x1.1bbe084045cd4p+44, 0x1.1a35beb6fcb75p+44, 0x1.18af9388c8deap+44,
+    0x1.172b83c7d517bp+44, 0x1.15a98c8a58e51p+44, 0x1.1429aaea92de0p+44, 0x1.12abdc06c31ccp+44,
+    0x1.11301d0125b51p+44, 0x1.0fb66affed31bp+44, 0x1.0e3ec32d3d1a2p+44, 0x1.0cc922b7247f7p+44,
+    0x1.0b5586cf9890fp+44, 0x1.09e3ecac6f383p+44, 0x1.0874518759bc8p+44, 0x1.0706b29ddf6dep+44,
+    0x1.059b0d3158574p+44, 0x1.04315e86e7f85p+44, 0x1.02c9a3e778061p+44, 0x1.0163da9fb3335p+44,
 };
 
 // order-preserving key of a logit: larger logit, larger key.  Both zeros are one value.
@@ -110,13 +127,6 @@ __device__ __forceinline__ float key_value(unsigned k) {
 // (key, id) as one number: larger comes first in the order
 __device__ __forceinline__ u64 pair_of(unsigned key, unsigned id) { return ((u64)key << 32) | (0xffffffffu - id); }
 
-// a FP32 number as a double, without the slow conversion (subnormals come out as other numbers below 2^-126,
-// next to any logit that is not one itself as good as zero)
-__device__ __forceinline__ double widen(unsigned bits) {
-  return __hiloint2double((int)((bits & 0x80000000u) | (((bits & 0x7fffffffu) >> 3) + 0x38000000u)),
-                          (int)(bits << 29));
-}
-
 // Rows with +inf among their logits: only the infinities have weight (the others' is exp(-inf)).  +inf is taken as the
 // largest finite number and that one, in such a row, as the number below it, whose distance of 2^104 leaves no weight.
 constexpr float kMaxFinite = 3.402823466e+38f;
@@ -124,34 +134,34 @@ __device__ __forceinline__ unsigned finite_top(unsigned bits) {
   return bits == 0x7f800000u || bits == 0x7f7fffffu ? bits - 1u : bits;
 }
 
+// an integer in 0 .. 2^52 - 1 that was added to 2^52
+__device__ __forceinline__ u64 mantissa(double v) {
+  return ((u64)((unsigned)__double2hiint(v) & 0xfffffu) << 32) | (unsigned)__double2loint(v);
+}
+
 struct Weigher {
-  double m, c;          // largest logit, log2(e) / T
-  float mf, cf;
-  const unsigned* tab;  // this lane's copy
+  double m, c;          // largest logit, 128 log2(e) / T
+  float mf, cf;         // the same, but log2(e) / T
+  const double* tab;    // this lane's copy
   // x in FP32; NaN or infinite for NaN and -inf
   __device__ __forceinline__ float rough(unsigned bits) const { return (mf - __uint_as_float(bits)) * cf; }
-  // x >= 0
-  __device__ __forceinline__ double exponent(unsigned bits) const { return (m - widen(bits)) * c; }
-  // x as a whole number of 2^-32 (high word: integer part)
-  __device__ __forceinline__ uint2 fixed(double x) const {
-    const double t = x + 1048576.0;      // 2^20: the last place is 2^-32
-    return make_uint2((unsigned)__double2loint(t), (unsigned)__double2hiint(t) & 0xfffffu);
+  // m - s >= 0, exact but for one rounding to 53 bits
+  __device__ __forceinline__ double below(unsigned bits) const { return m - (double)__uint_as_float(bits); }
+  // k, the whole number next to 128 x, and the rest r
+  __device__ __forceinline__ int split(double d, double& r) const {
+    constexpr double magic = 6755399441055744.0;         // 1.5 * 2^52: the last place is 1
+    const double t = fma(d, c, magic);
+    r = fma(d, c, magic - t);
+    return __double2loint(t);
   }
-  // 1/64 wide bins of x
-  __device__ __forceinline__ int bin(uint2 x) const { return (int)__funnelshift_l(x.x, x.y, 6); }
-  // 2^-x in units of 2^-45
-  __device__ __forceinline__ u64 weight(uint2 x) const {
-    const unsigned t = tab[(x.x >> 25) * 32];
-    // q = 1 - 2^-r = r ln 2 - (r ln 2)^2 / 2 + (r ln 2)^3 / 6, r < 2^-7 (the next term is below 2^-34)
-    const float r = (float)(x.x & 0x1ffffffu);           // in units of 2^-32
-    constexpr float a1 = 1.61385904e-10f, a2 = 1.3022705e-20f, a3 = 7.0056034e-31f;
-    const float q = r * (a1 - r * (a2 - r * a3));
-    // its mantissa bits behind 2^-7 are q in units of 2^-30
-    const unsigned qi = __float_as_uint(q + 0.0078125f) & 0x7fffffu;
-    const unsigned w = t - __umulhi(t, qi << 2);
-    const int sh = 13 - (int)x.y;        // x <= 25 here
-    if (sh >= 0) return (u64)w << sh;
-    return (u64)(((w >> (-sh - 1)) + 1u) >> 1);
+  __device__ __forceinline__ int bin(int k) const { return k >> 1; }   // 64 to the unit
+  // 2^52 + 2^-x in units of 2^-45, rounded
+  __device__ __forceinline__ double weight52(int k, double r) const {
+    const double t = tab[(k & (SM_STEPS - 1)) * 16];
+    // 2^(-r / 128), |r| <= 1/2: the next term of the series is below 2^-38
+    const double p = fma(r, fma(r, fma(r, -2.646642144433097e-08, 1.4662262387640425e-05), -0.0054152123481245725), 1.0);
+    const double scaled = __hiloint2double(__double2hiint(t) - (k >> 7) * 0x100000, __double2loint(t));
+    return fma(scaled, p, 4503599627370496.0);
   }
   // 2^-x in units of 2^-45 for rough x > SM_RANGE (0 for NaN and infinities): below 2^21, so that adding 2^23 rounds it
   // to a whole number in the mantissa
@@ -160,7 +170,10 @@ struct Weigher {
   }
   __device__ __forceinline__ u64 weight_of(unsigned bits) const {
     const float y = rough(bits);
-    return y <= SM_RANGE ? weight(fixed(exponent(bits))) : (u64)tail_weight(y);
+    if (!(y <= SM_RANGE)) return (u64)tail_weight(y);
+    double r;
+    const int k = split(below(bits), r);
+    return mantissa(weight52(k, r));
   }
   // the same by key
   __device__ __forceinline__ u64 weight_of_key(unsigned key) const { return weight_of(__float_as_uint(key_value(key))); }
@@ -549,11 +562,12 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
         if (key < cut_key || pair_of(key, id + e) < cut) continue;
       }
       if (y <= SM_RANGE) {
-        const uint2 fx = w.fixed(w.exponent(x[e]));
+        double r;
+        const int k = w.split(w.below(x[e]), r);
         if (MODE == FIND_COUNT)
-          atomicAdd(&sh->hist[0][w.bin(fx)], 1u);
+          atomicAdd(&sh->hist[0][w.bin(k)], 1u);
         else
-          add_mass(sh, w.bin(fx), w.weight(fx));
+          add_mass(sh, w.bin(k), mantissa(w.weight52(k, r)));
       } else if (MODE == FIND_MASS) {
         tail += w.tail_weight(y);
       }
@@ -568,8 +582,9 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
   }
   target -= base;
   // FP32's x is off by less than 2^-18 up to SM_RANGE: most elements are told apart from the bin by it
-  const float y0 = bin == SM_TAIL ? SM_RANGE : (float)bin * (1.f / 64.f) - 1e-5f;
-  const float y1 = bin == SM_TAIL ? INFINITY : (float)(bin + 1) * (1.f / 64.f) + 1e-5f;
+  // (bin b has the x that round to 2 b / 128 or (2 b + 1) / 128)
+  const float y0 = bin == SM_TAIL ? SM_RANGE : ((float)bin - 0.25f) * (1.f / 64.f) - 1e-5f;
+  const float y1 = bin == SM_TAIL ? INFINITY : ((float)bin + 0.75f) * (1.f / 64.f) + 1e-5f;
   u64 mn = ~0ull, mx = 0ull, lo = 0ull, hi = ~0ull;
   auto take = [&](unsigned bits, int id, u64& pr) {   // a candidate within the cut and [lo, hi]
     const unsigned key = order_key(bits);
@@ -590,7 +605,8 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
       [&](unsigned bits, int id) {
         const bool tail = !(w.rough(bits) <= SM_RANGE);
         u64 pr;
-        if (bin == SM_TAIL ? !tail : tail || w.bin(w.fixed(w.exponent(bits))) != bin) return false;
+        double r;
+        if (bin == SM_TAIL ? !tail : tail || w.bin(w.split(w.below(bits), r)) != bin) return false;
         return take(bits, id, pr) && span(pr);
       });
   bool sure = bin != SM_TAIL;            // whether the bin is known to hold the cut
@@ -685,7 +701,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   if (tid < 2) sh->n_cand[tid] = 0u;
   c.arrive();                            // peers write here only once every CTA of the cluster has started
 #pragma unroll
-  for (int k = 0; k < SM_STEPS / SM_WARPS; ++k) sh->tab[(k * SM_WARPS + warp) * 32 + lane] = kPow2[k * SM_WARPS + warp];
+  for (int k = 0; k < SM_STEPS * 16 / SM_THREADS; ++k) sh->tab[k * SM_THREADS + tid] = kPow2[(k * SM_THREADS + tid) >> 4];
   pdl_wait();
   pdl_trigger();
   // ---- the warp's piece of the row (`part` 8-logit vectors per CTA)
@@ -735,10 +751,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   Weigher w;
   row.has_inf = mkey == kInfKey;
   w.mf = row.has_inf ? kMaxFinite : key_value(mkey);
-  w.m = widen(__float_as_uint(w.mf));
-  w.c = 1.4426950408889634074 / (double)T;
-  w.cf = (float)w.c;
-  w.tab = sh->tab + lane;
+  w.m = (double)w.mf;
+  w.c = 128.0 * 1.4426950408889634074 / (double)T;
+  w.cf = (float)(w.c / 128.0);
+  w.tab = sh->tab + (lane & 15);
   u64 cut = 0ull;
   if (greedy) {
     cut = nth_equal(c, row, order_key(__float_as_uint(w.mf)), 0ull);
@@ -751,39 +767,49 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     }
     if (top_p < 1.f) cut = find_cut<FIND_MASS>(c, row, w, 0ull, top_p, cut, eligible);
   }
-  const double x_max = min_p > 0.f ? -log2((double)fminf(min_p, 1.f)) : INFINITY;
+  const double x_max = min_p > 0.f ? -128.0 * log2((double)fminf(min_p, 1.f)) : INFINITY;   // of 128 x
   // ---- kept mass per warp
   // FP32's x (good to 2^-22 of itself) tells all but the elements next to the cut apart from it; the keys decide there
   // and beyond 64, where an overflow could stand for anything
   const bool any_cut = cut != 0ull, any_min = x_max != INFINITY;
   const float yc = w.rough(__float_as_uint(key_value((unsigned)(cut >> 32))));
   const float y_hi = fminf(any_cut ? yc * 1.000001f + 1e-5f : INFINITY,
-                           any_min ? (float)x_max * 1.000001f + 1e-5f : INFINITY);
+                           any_min ? (float)(x_max / 128.0) * 1.000001f + 1e-5f : INFINITY);
   const float y_lo = any_cut ? fminf(yc * 0.999999f - 1e-5f, 64.f) : 64.f;
-  auto weigh = [&](unsigned bits, int id, unsigned& count) -> u64 {
+  // whether an element is kept, and its weight (a whole number, as a double)
+  auto weigh = [&](unsigned bits, int id, double& wt) -> bool {
     const float y = w.rough(bits);
-    if (!(y <= y_hi)) return 0ull;
+    if (!(y <= y_hi)) return false;
     if (y > y_lo) {
       const unsigned key = order_key(bits);
-      if (!is_candidate(key) || pair_of(key, id) < cut) return 0ull;
+      if (!is_candidate(key) || pair_of(key, id) < cut) return false;
     }
     if (y <= SM_RANGE) {
-      const double x = w.exponent(bits);
-      if (any_min && x > x_max) return 0ull;
-      ++count;
-      return w.weight(w.fixed(x));
+      const double d = w.below(bits);
+      if (any_min && d * w.c > x_max) return false;
+      double r;
+      const int k = w.split(d, r);
+      wt = w.weight52(k, r) - 4503599627370496.0;
+      return true;
     }
-    if (any_min && (double)y > x_max) return 0ull;   // (min_p below 2^-24)
-    ++count;
-    return (u64)w.tail_weight(y);
+    if (any_min && (double)y * 128.0 > x_max) return false;   // (min_p below 2^-24)
+    wt = (double)w.tail_weight(y);
+    return true;
   };
-  u64 mass = 0ull;
+  double sum = 0.0;                      // at most 2^7 weights of 2^45: exact
   unsigned count = 0u;
   row.each([&](const unsigned (&x)[8], int id) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mass += weigh(x[e], id + e, count);
+    for (int e = 0; e < 8; ++e) {
+      double wt;
+      if (weigh(x[e], id + e, wt)) {
+        sum += wt;
+        ++count;
+      }
+    }
     return true;
   });
+  u64 mass = __double2ull_rn(sum);
   mass = warp_sum64(mass);
   count = __reduce_add_sync(0xffffffffu, count);
   __syncthreads();
@@ -825,18 +851,21 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     const int v0 = min(end, c.rank * part + owner * per), v1 = min(end, v0 + per);
     row.v0 = min(v1, v0 + warp * 32);
     row.v1 = min(v1, row.v0 + 32);
-    u64 wt[8], sum = 0ull;
+    u64 wt[8], own = 0ull;
     int id0 = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) wt[e] = 0ull;
     row.each([&](const unsigned (&x)[8], int id) {   // one vector a lane
-      unsigned unused = 0u;
       id0 = id;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += wt[e] = weigh(x[e], id + e, unused);
+      for (int e = 0; e < 8; ++e) {
+        double v;
+        wt[e] = weigh(x[e], id + e, v) ? mantissa(v + 4503599627370496.0) : 0ull;
+        own += wt[e];
+      }
       return true;
     });
-    u64 inc = sum;
+    u64 inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
@@ -844,9 +873,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     }
     if (lane == 31) sh->wred[warp] = inc;
     __syncthreads();
-    u64 run = piece + inc - sum;
+    u64 run = piece + inc - own;
     for (int i = 0; i < warp; ++i) run += sh->wred[i];
-    if (run <= target && target < run + sum) {       // one lane
+    if (run <= target && target < run + own) {       // one lane
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (run <= target && target < run + wt[e]) {
