@@ -723,6 +723,7 @@ int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 constexpr int TT_THREADS = 192;
 constexpr float TT_GROWTH = 8.f;         // log2 of the growth that a rescaling waits for
+constexpr int TT_POLY = 8;               // of a row's 32 pairs of weights in a tile, those that the FMA pipe computes
 
 template <int HD>
 struct TtLayout {
@@ -777,6 +778,56 @@ __device__ __forceinline__ bool elect_one() {
   return one != 0;
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// two FP32 numbers that one instruction works on
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_get(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two numbers x <= 16 without the special-function unit: x = n + f with n whole and |f| <= 1/2, 2^f by the
+// polynomial of degree 4 that fits its relative error best (below 2^-18, as much as P_hi + P_lo keep), n into the
+// exponent.  Below -126 the result is 0.  NaN and +inf stay what they are.
+__device__ __forceinline__ F2 f2_exp2(F2 x) {
+  float a, b, pa, pb;
+  f2_get(x, a, b);
+  const F2 xc = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const F2 magic = f2(12582912.f, 12582912.f);           // 1.5 * 2^23: the last place is 1
+  const F2 t = f2_add(xc, magic);
+  const F2 n = f2_add(t, f2(-12582912.f, -12582912.f));
+  const F2 f = f2_fma(n, f2(-1.f, -1.f), xc);
+  F2 q = f2_fma(f, f2(0.009560510516166687f, 0.009560510516166687f), f2(0.05591703951358795f, 0.05591703951358795f));
+  q = f2_fma(q, f, f2(0.24024981260299683f, 0.24024981260299683f));
+  q = f2_fma(q, f, f2(0.6931219696998596f, 0.6931219696998596f));
+  q = f2_fma(q, f, f2(0.9999991655349731f, 0.9999991655349731f));
+  float ta, tb;
+  f2_get(q, pa, pb);
+  f2_get(t, ta, tb);
+  pa = __int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23));
+  pb = __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23));
+  pa = a < -126.f ? 0.f : pa;
+  pb = b < -126.f ? 0.f : pb;
+  return f2(a <= 16.f ? pa : a * INFINITY, b <= 16.f ? pb : b * INFINITY);
+}
 
 // grid (S, n_kv * row blocks, B), cluster (S, 1, 1): CTA z takes tiles [nt * z / S, nt * (z + 1) / S) of the nt
 // tiles: tile 0 holds the drafted keys, tile t > 0 the ring's places 64 (t - 1) ..
@@ -963,12 +1014,15 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       const bool is_tree = t == 0;
       // keys that not every row sees: the tree's, the ring's behind the last valid place and around the window's
       // edge.  Values that must not reach the rows that do not see them leave the product (tree_values).
-      const u64 valid_keys = is_tree ? ~0ull : bit_range(0, nvalid - j0);
-      const u64 some = is_tree ? 0ull : hidden_places(j0, next, W, max_dep) & valid_keys;
+      const bool edge = !is_tree && (j0 + TR_KT > nvalid || (j0 <= next + max_dep && j0 + TR_KT > next) ||
+                                     j0 <= next - W + max_dep);
+      u64 seen = is_tree ? anc : ~0ull;
       // scores i are issued once values i - 2 have been used: after this wait v_full's phase can be told
       mbar_wait(&s_full[s], (i >> 1) & 1, nullptr);
       tc_fence_after();
-      if (some != 0ull || valid_keys != ~0ull) {
+      if (edge) {
+        const u64 valid_keys = bit_range(0, nvalid - j0), some = hidden_places(j0, next, W, max_dep) & valid_keys;
+        seen = valid_keys & ~hidden_places(j0, next, W, dep);
         mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
         auto at = [&](int r, int c) {
           return reinterpret_cast<uint4*>(sV + s * LY::TILE + (c >> 3) * 8192 + sw128_offset(r, (c & 7) * 16));
@@ -987,20 +1041,19 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         }
         fence_proxy_async_smem();
       }
-      const u64 seen = is_tree ? anc : valid_keys & ~hidden_places(j0, next, W, dep);
       float sv[64];
 #pragma unroll
       for (int c = 0; c < 64; c += 16)
         tmem_ld16(tmem + s * 64 + c + trow, *reinterpret_cast<float(*)[16]>(&sv[c]));
       tmem_wait_ld();
-      if (__any_sync(0xffffffffu, seen != ~0ull)) {
+      if (edge || is_tree) {
 #pragma unroll
         for (int c = 0; c < 64; ++c)
           if (!((c < 32 ? (uint32_t)seen : (uint32_t)(seen >> 32)) >> (c & 31) & 1u)) sv[c] = -INFINITY;
       }
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], sv[c]);
+      for (int c = 0; c < 64; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], sv[c], sv[c + 1]);
       const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
       const bool grow = mt > m + TT_GROWTH || m == -INFINITY;
       if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
@@ -1022,22 +1075,40 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       }
       if (grow) m = mt;
       const float ref = m == -INFINITY ? 0.f : m;   // nothing seen yet: every weight below is 0
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      // the special-function unit computes 16 powers a cycle on an SM, 512 cycles for a tile of 128 rows: a quarter of
+      // them goes to the FMA pipe
+      F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+      const F2 sc = f2(a.scale_log2, a.scale_log2), off = f2(-ref, -ref), minus = f2(-1.f, -1.f);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = exp2f(fmaf(sv[h * 32 + 2 * e], a.scale_log2, -ref));
-          const float y = exp2f(fmaf(sv[h * 32 + 2 * e + 1], a.scale_log2, -ref));
-          sum[e & 3] += x + y;
+          F2 p = f2_fma(f2(sv[h * 32 + 2 * e], sv[h * 32 + 2 * e + 1]), sc, off);
+          float x, y;
+          if (e % (32 / TT_POLY) == 0) {
+            p = f2_exp2(p);
+            f2_get(p, x, y);
+          } else {
+            f2_get(p, x, y);
+            x = exp2f(x);
+            y = exp2f(y);
+            p = f2(x, y);
+          }
+          sum[e & 1] = f2_add(sum[e & 1], p);
           hi[e] = pack_bf16x2(x, y);
-          lo[e] = pack_bf16x2(x - bf16_lo(hi[e]), y - bf16_hi(hi[e]));
+          p = f2_fma(f2(bf16_lo(hi[e]), bf16_hi(hi[e])), minus, p);
+          f2_get(p, x, y);
+          lo[e] = pack_bf16x2(x, y);
         }
         tmem_st16(tmem + s * 64 + h * 16 + trow, hi);
         tmem_st16(tmem + s * 64 + 32 + h * 16 + trow, lo);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      {
+        float x, y;
+        f2_get(f2_add(sum[0], sum[1]), x, y);
+        l += x + y;
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[s]);
