@@ -10,19 +10,19 @@
 // nodes' RoPE'd keys and values go to k_tree / v_tree, and uttt_kv_ring_commit
 // copies an accepted path into the ring.  RoPE rounds as the decode kernel does.
 //
-// Kernel.  The rep query heads of a KV head and the nodes stack into the rows of
-// one matrix product (row = node * rep + head), so a ring is read once for all
-// of them.  One CTA takes up to 128 rows and streams its share of the keys
-// through shared memory in 64-key tiles (cp.async, three tiles in flight); the
-// drafted keys are the last tile, RoPE'd in place.  WM warps stack along the rows (16
-// each) and WK along the keys of a tile, so that a few rows still use every warp;
-// each keeps its running maximum, sum and unnormalised output in registers.  With
-// few rows in the batch a cluster of S CTAs splits the keys.  The partials meet in
-// (distributed) shared memory at the end.
-// The products run on mma.sync (16 x 8 x 16): at 16 to 128 rows a CTA is bound by
-// the ring's bytes (a ring of 512 x 128 keys and values is 256 KB for 2 * 2 * 64 *
-// 512 * 128 operations at 64 rows), a tcgen05 tile would hold mostly padding at the
-// usual 16 to 64 rows and leave the softmax of a row to a single thread.
+// Kernels.  The rep query heads of a KV head and the nodes stack into the rows of
+// one matrix product (row = node * rep + head), so a ring is read once for all of
+// them.  One CTA takes up to 128 rows and streams its share of the keys through
+// shared memory in 64-key tiles; the drafted keys, RoPE'd on the way, are the
+// first one.  Per row it keeps the running maximum and sum of the softmax and the
+// unnormalised output.  With few rows in the batch a cluster of S CTAs splits the
+// keys and joins its partials in distributed shared memory.
+//   head dim 64, 128   attn_tree_tc_kernel: tcgen05, S and O in TMEM, TMA tiles;
+//   head dim 32        attn_tree_kernel: mma.sync (16 x 8 x 16), cp.async tiles
+//                      (a row is half of the 128-byte swizzle the others use).
+// mma.sync for few rows of the larger heads was measured and dropped: 64 rows of
+// 8 nodes at the 1.58B heads (32 rows a CTA) 40.4 us against 31.6 us here, 4 nodes
+// (16 rows) 31.0 against 31.6, 32 rows of 5 nodes at 12/4 heads 14.2 against 12.8.
 // The probabilities enter the second product as two BF16 parts, P_hi = bf16(P) and
 // P_lo = bf16(P - P_hi) (about 16 significant bits, as the prefill kernel does);
 // scores, statistics and sums are FP32.
@@ -42,7 +42,7 @@ constexpr int TR_MAX_REP = 8;
 __device__ __forceinline__ float bfr(float x) { return __bfloat162float(__float2bfloat16(x)); }
 
 constexpr int TR_KT = 64;                // keys per tile (and the most nodes of a tree)
-constexpr int TR_NS = 3;                 // tiles in flight
+constexpr int TR_NS = 3;                 // tiles in flight (head dim 32)
 
 typedef unsigned long long u64;
 
@@ -90,6 +90,8 @@ struct TreeArgs {
   int qkv_ld, N, n_kv, rep, W, n_slots, n_pos, out_ld;
   float scale_log2;                      // log2(e) / sqrt(hd)
   int vec_in, vec_out;                   // whether rows of qkv (with the tables) and of out start on 16 bytes
+  int b0;                                // the first row of the launch
+  int joins;                             // whether the launch is the rest of the one before it
 };
 
 // bits lo .. lo + len - 1, as far as they lie in 0 .. 63
@@ -356,6 +358,8 @@ inline int tree_split(long long ctas, int tiles, int per_sm, int head, int join)
   return best;
 }
 
+// Head dim 32.  WM warps stack along the rows (16 each) and WK along the keys of a tile, so that a few rows still
+// use every warp; three tiles are in flight.
 // grid (S, n_kv * row blocks, B), cluster (S, 1, 1): CTA z takes tiles [nt * z / S, nt * (z + 1) / S) of the nt
 // 64-key tiles: tile 0 holds the drafted keys, tile t > 0 the ring's places 64 (t - 1) ..
 template <int HD, int WM>
@@ -709,7 +713,7 @@ int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// The same on tcgen05, for many rows (head dim 64 or 128).
+// The same on tcgen05 (head dim 64 and 128).
 //
 // One CTA takes 128 rows (TMEM lanes).  Tile by tile: S = Q K^T into one of two
 // TMEM buffers; the thread that owns a row reads its 64 scores, keeps the running
@@ -723,7 +727,6 @@ int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
 // ---------------------------------------------------------------------------
 constexpr int TT_THREADS = 192;
 constexpr float TT_GROWTH = 8.f;         // log2 of the growth that a rescaling waits for
-constexpr int TT_POLY = 8;               // of a row's 32 pairs of weights in a tile, those that the FMA pipe computes
 
 template <int HD>
 struct TtLayout {
@@ -804,31 +807,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of two numbers x <= 16 without the special-function unit: x = n + f with n whole and |f| <= 1/2, 2^f by the
-// polynomial of degree 4 that fits its relative error best (below 2^-18, as much as P_hi + P_lo keep), n into the
-// exponent.  Below -126 the result is 0.  NaN and +inf stay what they are.
-__device__ __forceinline__ F2 f2_exp2(F2 x) {
-  float a, b, pa, pb;
-  f2_get(x, a, b);
-  const F2 xc = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const F2 magic = f2(12582912.f, 12582912.f);           // 1.5 * 2^23: the last place is 1
-  const F2 t = f2_add(xc, magic);
-  const F2 n = f2_add(t, f2(-12582912.f, -12582912.f));
-  const F2 f = f2_fma(n, f2(-1.f, -1.f), xc);
-  F2 q = f2_fma(f, f2(0.009560510516166687f, 0.009560510516166687f), f2(0.05591703951358795f, 0.05591703951358795f));
-  q = f2_fma(q, f, f2(0.24024981260299683f, 0.24024981260299683f));
-  q = f2_fma(q, f, f2(0.6931219696998596f, 0.6931219696998596f));
-  q = f2_fma(q, f, f2(0.9999991655349731f, 0.9999991655349731f));
-  float ta, tb;
-  f2_get(q, pa, pb);
-  f2_get(t, ta, tb);
-  pa = __int_as_float(__float_as_int(pa) + (__float_as_int(ta) << 23));
-  pb = __int_as_float(__float_as_int(pb) + (__float_as_int(tb) << 23));
-  pa = a < -126.f ? 0.f : pa;
-  pb = b < -126.f ? 0.f : pb;
-  return f2(a <= 16.f ? pa : a * INFINITY, b <= 16.f ? pb : b * INFINITY);
-}
-
 // grid (S, n_kv * row blocks, B), cluster (S, 1, 1): CTA z takes tiles [nt * z / S, nt * (z + 1) / S) of the nt
 // tiles: tile 0 holds the drafted keys, tile t > 0 the ring's places 64 (t - 1) ..
 template <int HD>
@@ -848,17 +826,22 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sQ = base, *sK = base + LY::K0, *sV = base + LY::V0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int S = gridDim.x, z = blockIdx.x, b = blockIdx.z;
+  const int S = gridDim.x, z = blockIdx.x, b = a.b0 + blockIdx.z;
   const int g = blockIdx.y % a.n_kv, row0 = blockIdx.y / a.n_kv * 128;
   const int N = a.N, rep = a.rep, W = a.W;
-  pdl_wait();
+  // A launch that joins the one before it starts as soon as that one's CTAs have: they waited for what came before
+  // both.  It ends after that one instead, so that what comes next waits for both.
+  if (!a.joins) pdl_wait();
   pdl_trigger();
   const int ti = tid - 64;               // warps 2-5: 0 .. 127
   const int par_i = ti >= 0 && ti < N ? a.parents[(size_t)b * N + ti] : -1;
   const int n = a.n_nodes ? min(a.n_nodes[b], N) : N;
   const int p0 = a.pos[b], sl = a.slot[b];
   const int rows = n * rep;
-  if (row0 >= rows || sl < 0 || sl >= a.n_slots || p0 < 0) return;   // the same in the whole cluster
+  if (row0 >= rows || sl < 0 || sl >= a.n_slots || p0 < 0) {   // the same in the whole cluster
+    if (a.joins) pdl_wait();
+    return;
+  }
   const int nvalid = min(p0, W), nt = (nvalid + TR_KT - 1) / TR_KT + 1;
   const int t_lo = (int)((long long)nt * z / S), t_hi = (int)((long long)nt * (z + 1) / S), cnt = t_hi - t_lo;
   const bool has_tree = t_lo == 0 && cnt > 0;
@@ -1075,8 +1058,9 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       }
       if (grow) m = mt;
       const float ref = m == -INFINITY ? 0.f : m;   // nothing seen yet: every weight below is 0
-      // the special-function unit computes 16 powers a cycle on an SM, 512 cycles for a tile of 128 rows: a quarter of
-      // them goes to the FMA pipe
+      // The special-function unit computes 16 powers a cycle on an SM, 512 cycles for a tile of 128 rows.  (Powers by
+      // polynomials on the FMA pipe made the tile slower: an eighth of them by 1 %, a quarter by 5 %, half by 17 %;
+      // a warp of its own per scheduler is bound by what it issues.)
       F2 sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
       const F2 sc = f2(a.scale_log2, a.scale_log2), off = f2(-ref, -ref), minus = f2(-1.f, -1.f);
 #pragma unroll
@@ -1086,15 +1070,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         for (int e = 0; e < 16; ++e) {
           F2 p = f2_fma(f2(sv[h * 32 + 2 * e], sv[h * 32 + 2 * e + 1]), sc, off);
           float x, y;
-          if (e % (32 / TT_POLY) == 0) {
-            p = f2_exp2(p);
-            f2_get(p, x, y);
-          } else {
-            f2_get(p, x, y);
-            x = exp2f(x);
-            y = exp2f(y);
-            p = f2(x, y);
-          }
+          f2_get(p, x, y);
+          x = exp2f(x);
+          y = exp2f(y);
+          p = f2(x, y);
           sum[e & 1] = f2_add(sum[e & 1], p);
           hi[e] = pack_bf16x2(x, y);
           p = f2_fma(f2(bf16_lo(hi[e]), bf16_hi(hi[e])), minus, p);
@@ -1176,7 +1155,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, 256);
-  if (S == 1) return;
+  if (S == 1) {
+    if (a.joins) pdl_wait();
+    return;
+  }
   cg::this_cluster().sync();             // all rows have arrived; nothing remote after this
   const Joiner jn{reinterpret_cast<float*>(base), ml_s, S, 128 / S, LY::OLD};
   const int live = min(128, rows - row0);
@@ -1185,6 +1167,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
     const float L = jn.join(i / CH, i % CH * 8, v);
     store_out(a, b, g, row0 + z + i / CH * S, i % CH * 8, HD, v, 1.f / L);
   }
+  if (a.joins) pdl_wait();
 }
 
 template <int HD>
@@ -1204,32 +1187,47 @@ int launch_tree_tc(const TreeArgs& a, int B, cudaStream_t st) {
   UTTT_TRY(make_tmap_bf16(&tmV, a.vring, 3, dims, str, box));
   const int blocks = (a.N * a.rep + 127) / 128;
   UTTT_REQUIRE((long long)a.n_kv * blocks <= 65535, UTTT_ERR_UNSUPPORTED);
-  const int S = tree_split((long long)B * a.n_kv * blocks, (a.W + TR_KT - 1) / TR_KT + 1, 2, 4, 1);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(S, a.n_kv * blocks, B);
-  cfg.blockDim = dim3(TT_THREADS);
-  cfg.dynamicSmemBytes = LY::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = S;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1] = pdl_attribute();
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, attn_tree_tc_kernel<HD>, tmK, tmV, a) != cudaSuccess) return launch_status();
-  return launch_status();
+  auto launch = [&](int b0, int n, int S, int joins) {
+    TreeArgs part = a;
+    part.b0 = b0;
+    part.joins = joins;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S, a.n_kv * blocks, n);
+    cfg.blockDim = dim3(TT_THREADS);
+    cfg.dynamicSmemBytes = LY::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = S;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    at[1] = pdl_attribute();
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, attn_tree_tc_kernel<HD>, tmK, tmV, part) != cudaSuccess) return launch_status();
+    return launch_status();
+  };
+  const int tiles = (a.W + TR_KT - 1) / TR_KT + 1, per = a.n_kv * blocks, slots = 2 * num_sms();
+  const int S = tree_split((long long)B * per, tiles, 2, 4, 1);
+  // A last wave with few CTAs would take as long as a full one: its rows are a launch of their own, split over
+  // clusters, that fills the SMs which the full waves leave (64 rows of 16 nodes at the 1.58B heads, 320 CTAs on 296
+  // places, window 512: 32.5 us in one launch, 22 us for the 59 rows of one wave).
+  const int full = S == 1 ? (int)((long long)B * per / slots * slots / per) : 0, rest = B - full;
+  if (full > 0 && rest > 0 && (long long)rest * per * 2 <= slots) {
+    UTTT_TRY(launch(0, full, 1, 0));
+    return launch(full, rest, tree_split((long long)rest * per, tiles, 2, 4, 1), 1);
+  }
+  return launch(0, B, S, 0);
 }
 
 template <int HD>
 int launch_tree_rows(const TreeArgs& a, int B, cudaStream_t st) {
-  const int rows = a.N * a.rep;
-  if (rows <= 16) return launch_tree<HD, 1>(a, B, st);
-  if (rows <= 32) return launch_tree<HD, 2>(a, B, st);
   if constexpr (HD >= 64) {
     return launch_tree_tc<HD>(a, B, st);
   } else {
+    const int rows = a.N * a.rep;
+    if (rows <= 16) return launch_tree<HD, 1>(a, B, st);
+    if (rows <= 32) return launch_tree<HD, 2>(a, B, st);
     if (rows <= 64) return launch_tree<HD, 4>(a, B, st);
     return launch_tree<HD, 8>(a, B, st);
   }
@@ -1317,6 +1315,7 @@ extern "C" int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W
   a.scale_log2 = 1.4426950408889634f / sqrtf((float)hd);
   a.vec_in = at16(qkv) && qkv_ld % 8 == 0 && at16(rope_cos) && at16(rope_sin);
   a.vec_out = at16(out) && out_ld % 8 == 0;
+  a.b0 = a.joins = 0;
   if (hd == 32) return launch_tree_rows<32>(a, B, st);
   if (hd == 64) return launch_tree_rows<64>(a, B, st);
   return launch_tree_rows<128>(a, B, st);
