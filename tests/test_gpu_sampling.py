@@ -76,6 +76,37 @@ def test_settings_per_row():
     _check(x, u, *sampling.sample(x, u, **st), {**st, "top_k": st["top_k"].clamp_min(0)})
 
 
+@pytest.mark.parametrize("V", [300, 9000])
+def test_device_values_out_of_range(V):
+    """Per-row values that the host checks would refuse: each has a meaning, none an effect beyond its row."""
+    nan, inf = float("nan"), float("inf")
+    st = dict(temperature=[nan, -1.0, 0.8, 0.8, 0.8, 0.8, 0.8, 0.8], top_k=[0, 0, -5, 0, 20, 0, 0, 2 ** 31 - 1],
+              top_p=[1, 1, 0.9, 0.0, -1.0, nan, 7.0, 0.9], min_p=[0, 0, 0, 0, 0, nan, 3.0, -1.0])
+    means = dict(temperature=[0, 0] + [0.8] * 6, top_k=[0, 0, 0, 1, 1, 0, 0, 0], top_p=[1, 1, 0.9, 1, 1, 1, 1, 0.9],
+                 min_p=[0, 0, 0, 0, 0, 0, 1.0, 0])
+    x, u = _logits(8, V, torch.float32, 14)
+
+    def tensors(d):
+        return {k: torch.tensor(v, device=DEV, dtype=torch.int32 if k == "top_k" else torch.float32)
+                for k, v in d.items()}
+    _check(x, u, *sampling.sample(x, u, **tensors(st)), tensors(means))
+    for given, used in ((-1.0, 0.0), (1.0, 0.99999994), (inf, 0.99999994), (nan, 0.99999994)):
+        got = sampling.sample(x, torch.full((8,), given, device=DEV), top_p=0.9)
+        _check(x, torch.full((8,), used, device=DEV), *got, dict(top_p=0.9))
+
+
+@pytest.mark.parametrize("V", [700, 40000])
+@pytest.mark.parametrize("settings", [
+    dict(top_k=400), dict(top_k=512), dict(top_k=513, top_p=0.8), dict(top_p=0.9999), dict(top_p=0.5, min_p=0.2),
+    dict(top_k=100, top_p=0.999999, min_p=1e-9), dict(temperature=0.1, top_p=0.99), dict(temperature=9.0, top_k=64),
+])
+@pytest.mark.parametrize("std", [0.0, 0.01, 6.0])
+def test_few_and_many_candidates_down_to_the_cut(V, settings, std):
+    x, u = _logits(4, V, torch.float32, 15, std)
+    x[2] = x[2].round()                            # many equals
+    _check(x, u, *sampling.sample(x, u, **settings), settings)
+
+
 def _special(V, dtype):
     """Rows whose values go to the edges of the type."""
     low = torch.finfo(dtype).min

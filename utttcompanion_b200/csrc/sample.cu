@@ -72,7 +72,7 @@ struct SampleShared {
   u64 cand[2][SM_CAP];                   // rank 0: gathered candidates; others: their copies of them
   u64 cand_w[SM_CAP];
   unsigned n_cand[2];                    // rank 0; gathers alternate between the two lists
-  u64 res_base, res_cut;
+  u64 res_base, res_held, res_cut;
   int res_bin;
   alignas(16) unsigned hist[3][SM_BINS];  // count, or 16-bit limbs of the mass
 };
@@ -388,10 +388,11 @@ __device__ u64 rank_candidates(Cluster& c, unsigned n, int mode, u64 target, con
   return sh->res_cut;
 }
 
-// The merged histogram's bin that holds `target` and what lies before it, the same in every CTA.  *total: of all bins.
-// With top_p > 0 the target is that part of *total + more (mass), and written back.  The bin is -1 if the target
+// The merged histogram's bin that holds `target`, what lies before it and what is in it, the same in every CTA; `total`:
+// of all bins.  With top_p > 0 the target is that part of total + more (mass), and written back.  The bin is -1 if the target
 // lies behind all bins.
-__device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, u64& base_out, u64& total) {
+__device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, u64& base_out, u64& held,
+                      u64& total) {
   SampleShared* sh = c.sh;
   c.sync();
   // this CTA sums its share of the bins over the cluster: thread t has PB consecutive ones
@@ -448,11 +449,13 @@ __device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, 
         SampleShared* p = c.peer(r);
         p->res_bin = b0 + threadIdx.x * PB + q;
         p->res_base = at;
+        p->res_held = val[q];
       }
     at += val[q];
   }
   c.sync();
   base_out = sh->res_base;
+  held = sh->res_held;
   return sh->res_bin;
 }
 
@@ -523,9 +526,11 @@ __device__ __noinline__ u64 nth_equal(Cluster c, const Row<F32> row, unsigned ke
 
 // Last element of the kept prefix among the pairs >= cut: the first one, in the order, whose count or mass up
 // to and with it exceeds the target (count - 1, or top_p of the whole mass).  Returns `cut` if nothing does.
+// Where the candidates down to the cut are few and `cut` is 0, they are gathered as a whole instead: `listed` says how
+// many are in the list (0: there is none, and the cut is returned), `target` what they must not exceed.
 template <int MODE, bool F32>
-__device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 target, float top_p, u64 cut,
-                        unsigned n_eligible) {
+__device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64& target, float top_p, u64 cut,
+                        unsigned n_eligible, unsigned& listed) {
   SampleShared* sh = c.sh;
   if (n_eligible <= SM_CAP) {            // few enough to rank at once
     const unsigned cut_bits = __float_as_uint(key_value((unsigned)(cut >> 32)));
@@ -545,6 +550,10 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
       u64 total = 0ull;
       for (int i = 0; i < SM_WARPS; ++i) total += sh->wred[i];
       target = part_of(top_p, total);
+    }
+    if (cut == 0ull) {
+      listed = n;
+      return 0ull;
     }
     const u64 r = rank_candidates(c, n, MODE, target, w);
     return r ? r : cut;
@@ -575,10 +584,25 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
     more += tail;
     return true;
   });
-  int bin = locate(c, MODE, MODE == FIND_MASS ? top_p : 0.f, more, target, base, total);
+  u64 held;
+  int bin = locate(c, MODE, MODE == FIND_MASS ? top_p : 0.f, more, target, base, held, total);
   if (bin < 0) {
     bin = SM_TAIL;
     base = total;
+  }
+  if (bin != SM_TAIL && cut == 0ull) {
+    // an upper bound of the candidates down to this bin's end: each weighs at least 2^-x there
+    const u64 least = MODE == FIND_COUNT ? 1ull : (u64)exp2(45.0 - ((double)bin + 0.8) / 64.0);
+    if (base + held <= (u64)SM_CAP * least) {
+      const float y2 = ((float)bin + 0.75f) * (1.f / 64.f) + 1e-5f;
+      listed = gather(
+          c, row, [&](unsigned bits) { return w.rough(bits) <= y2; },
+          [&](unsigned bits, int) {
+            double r;
+            return w.rough(bits) <= SM_RANGE && w.bin(w.split(w.below(bits), r)) <= bin;
+          });
+      return 0ull;
+    }
   }
   target -= base;
   // FP32's x is off by less than 2^-18 up to SM_RANGE: most elements are told apart from the bin by it
@@ -674,7 +698,7 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
       }
       return true;
     });
-    bin = locate(c, MODE, 0.f, 0ull, target, base, total);
+    bin = locate(c, MODE, 0.f, 0ull, target, base, held, total);
     if (bin < 0) return cut;             // everything is within the target
     sure = true;
     target -= base;
@@ -687,6 +711,80 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64 t
         });
   }
   return cut;                            // not reached: a pass leaves 1/2048 of the range of keys, then of ids
+}
+
+// Everything that is left where the row's first candidates in the order are in the list (n of them): ranks, the three
+// cuts and the pick.  `mass_limit`: what top-p allows before an element; with top_k it is worked out here.  Every CTA
+// does the same; the first one writes.
+__device__ __noinline__ void finish_list(Cluster c, const Weigher w, unsigned n, int top_k, float top_p, u64 mass_limit,
+                                         double x_max, float u, int row_i, int* ids, int* kept, float* prob) {
+  SampleShared* sh = c.sh;
+  const u64* cand = sh->cand[c.list];
+  const int tid = threadIdx.x;
+  u64 mine = 0ull, own = 0ull;
+  bool in = tid < (int)n;
+  __syncthreads();
+  if (in) {
+    mine = cand[tid];
+    own = w.weight_of_key((unsigned)(mine >> 32));
+    sh->cand_w[tid] = own;
+  }
+  __syncthreads();
+  unsigned rank = 0u;
+  u64 before = 0ull;
+  if (in) {
+#pragma unroll 8
+    for (unsigned j = 0; j < n; ++j) {
+      const bool first = cand[j] > mine;
+      rank += first;
+      before += first ? sh->cand_w[j] : 0ull;
+    }
+  }
+  auto total_of = [&](u64 v, unsigned k, unsigned& count) -> u64 {   // sums of v and k over the threads
+    v = warp_sum64(v);
+    k = __reduce_add_sync(0xffffffffu, k);
+    __syncthreads();
+    if ((tid & 31) == 0) {
+      sh->wred[tid >> 5] = v;
+      sh->wred2[tid >> 5] = k;
+    }
+    __syncthreads();
+    v = 0ull;
+    count = 0u;
+    for (int i = 0; i < SM_WARPS; ++i) {
+      v += sh->wred[i];
+      count += (unsigned)sh->wred2[i];
+    }
+    return v;
+  };
+  unsigned count;
+  if (top_k > 0) {
+    in = in && rank < (unsigned)top_k;
+    const u64 mass = total_of(in ? own : 0ull, 0u, count);
+    mass_limit = part_of(top_p, mass);
+  }
+  if (top_p < 1.f) in = in && before <= mass_limit;
+  const unsigned bits = __float_as_uint(key_value((unsigned)(mine >> 32)));
+  if (x_max != INFINITY) {
+    const float y = w.rough(bits);
+    in = in && (y <= SM_RANGE ? w.below(bits) * w.c : (double)y * 128.0) <= x_max;
+  }
+  const u64 total = total_of(in ? own : 0ull, in, count);
+  if (tid < (int)n) sh->cand_w[tid] = in ? own : 0ull;
+  __syncthreads();
+  if (c.rank == 0 && in) {
+    const u64 target = part_of(u, total);
+    const unsigned id = 0xffffffffu - (unsigned)mine;
+    u64 at = 0ull;                       // mass of the kept ids below this one
+#pragma unroll 8
+    for (unsigned j = 0; j < n; ++j) at += 0xffffffffu - (unsigned)cand[j] < id ? sh->cand_w[j] : 0ull;
+    if (at <= target && target < at + own) {
+      ids[row_i] = (int)id;
+      if (kept) kept[row_i] = (int)count;
+      if (prob) prob[row_i] = (float)((double)own / (double)total);
+    }
+  }
+  c.sync();                              // no CTA leaves while a peer may still read or write its shared memory
 }
 
 template <bool F32>
@@ -755,19 +853,32 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   w.c = 128.0 * 1.4426950408889634074 / (double)T;
   w.cf = (float)(w.c / 128.0);
   w.tab = sh->tab + (lane & 15);
+  const double x_max = min_p > 0.f ? -128.0 * log2((double)fminf(min_p, 1.f)) : INFINITY;   // of 128 x
+  float uv = u[(size_t)row_i * u_ld + (u_index ? min(max(u_index[row_i], 0), u_len - 1) : 0)];
+  uv = fminf(uv, 0.99999994f);           // the largest number below 1
   u64 cut = 0ull;
   if (greedy) {
     cut = nth_equal(c, row, order_key(__float_as_uint(w.mf)), 0ull);
     c.phase ^= 1;                        // it exchanged once
   } else {
-    unsigned eligible = (unsigned)lim;
+    unsigned eligible = (unsigned)lim, listed = 0u;
+    u64 target = (u64)max(top_k - 1, 0);
+    int k_left = 0;                      // what is left for the list to apply
     if (top_k > 0 && top_k < lim) {
-      cut = find_cut<FIND_COUNT>(c, row, w, (u64)(top_k - 1), 0.f, cut, eligible);
+      cut = find_cut<FIND_COUNT>(c, row, w, target, 0.f, cut, eligible, listed);
       eligible = (unsigned)top_k;
+      k_left = top_k;
     }
-    if (top_p < 1.f) cut = find_cut<FIND_MASS>(c, row, w, 0ull, top_p, cut, eligible);
+    if (listed == 0u && top_p < 1.f) {
+      target = 0ull;                     // (stays 0 for top_p <= 0: the first element alone)
+      cut = find_cut<FIND_MASS>(c, row, w, target, top_p, cut, eligible, listed);
+      k_left = 0;
+    }
+    if (listed != 0u) {                  // the same in every CTA
+      finish_list(c, w, listed, k_left, top_p, target, x_max, uv, row_i, ids, kept, prob);
+      return;
+    }
   }
-  const double x_max = min_p > 0.f ? -128.0 * log2((double)fminf(min_p, 1.f)) : INFINITY;   // of 128 x
   // ---- kept mass per warp
   // FP32's x (good to 2^-22 of itself) tells all but the elements next to the cut apart from it; the keys decide there
   // and beyond 64, where an overflow could stand for anything
@@ -832,8 +943,6 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     n_kept += sh->xch[p2][r].b;
   }
   below += all_below;
-  float uv = u[(size_t)row_i * u_ld + (u_index ? min(max(u_index[row_i], 0), u_len - 1) : 0)];
-  uv = fminf(uv, 0.99999994f);           // the largest number below 1
   const u64 target = part_of(uv, total);
   // The piece that holds the pick has at most SM_WARPS tiles of 32 vectors: each warp of its CTA weighs one again.
   if (below <= target && target < below + mass) {   // one warp of the cluster
