@@ -149,6 +149,23 @@ def test_values_at_the_edges(V, dtype, settings):
         _check(x, u, *sampling.sample(x, u, **settings), settings)
 
 
+@pytest.mark.parametrize("temperature", [1.01e-5, 1e29, 1e31, 2e37, 3.4e38])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_temperatures_and_logits_over_the_whole_range(dtype, temperature):
+    """Differences of logits beyond the largest FP32 number, and temperatures whose inverse FP32 does not hold."""
+    V, top = 5000, torch.finfo(dtype).max
+    x, u = _logits(6, V, dtype, 16)
+    x[1] *= top / 64
+    x[2] = torch.linspace(-1.0, 1.0, V, device=DEV).to(dtype) * top
+    x[3, 9:12] = torch.inf
+    x[3, 12:15] = top                                                 # no weight beside an infinity
+    x[4, :] = -top
+    x[4, 6:20] = top
+    x[5, ::2] = -torch.inf
+    for st in (dict(), dict(top_p=0.6), dict(top_k=1700, min_p=0.2), dict(top_k=9, top_p=0.8)):
+        _check(x, u, *sampling.sample(x, u, temperature=temperature, **st), dict(temperature=temperature, **st))
+
+
 def test_strides_alignment_and_u_index():
     x, _ = _logits(6, 1003, torch.bfloat16, 6)
     big = torch.full((6, 1100), 50.0, device=DEV, dtype=torch.bfloat16)
@@ -215,7 +232,9 @@ def test_no_rows_and_refusals():
     for bad in (dict(logits=x.double()), dict(u=u[:1]), dict(u=u.double()), dict(logits=x[:, :6]),
                 dict(top_k=torch.ones(2, device=DEV)), dict(top_p=torch.ones(3, device=DEV)),
                 dict(u=torch.rand(2, 3, device=DEV)), dict(u_index=torch.zeros(2, device=DEV)),
-                dict(active_limit=2), dict(temperature=-1.0), dict(u=u.cpu())):
+                dict(active_limit=2), dict(active_limit=-2 ** 32 + 9), dict(temperature=-1.0), dict(u=u.cpu()),
+                dict(logits=x[:1, :1].expand(2, 2 ** 32 + 64)), dict(logits=x[:1].expand(2 ** 16, 100))):
         a = {**dict(logits=x, u=u), **bad}
         with pytest.raises(ValueError):
             sampling.sample(a.pop("logits"), a.pop("u"), **a)
+    _check(x, u, *sampling.sample(x, u, active_limit=2 ** 32 + 5), {})   # no more than there are

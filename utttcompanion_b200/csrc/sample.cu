@@ -141,10 +141,11 @@ __device__ __forceinline__ u64 mantissa(double v) {
 
 struct Weigher {
   double m, c;          // largest logit, 128 log2(e) / T
-  float mf, cf;         // the same, but log2(e) / T
+  float scale, ms, cs;  // a power of 2, m times it, and log2(e) / T divided by it
   const double* tab;    // this lane's copy
-  // x in FP32; NaN or infinite for NaN and -inf
-  __device__ __forceinline__ float rough(unsigned bits) const { return (mf - __uint_as_float(bits)) * cf; }
+  // x in FP32; NaN or infinite for NaN and -inf.  Scaled, so that m - s does not overflow: by 1/2, and by 2^-100 at
+  // temperatures above 10^30, which would flush log2(e) / T to zero
+  __device__ __forceinline__ float rough(unsigned bits) const { return fmaf(__uint_as_float(bits), -scale, ms) * cs; }
   // m - s >= 0, exact but for one rounding to 53 bits
   __device__ __forceinline__ double below(unsigned bits) const { return m - (double)__uint_as_float(bits); }
   // k, the whole number next to 128 x, and the rest r
@@ -845,20 +846,22 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   const float top_p = opt.top_p ? opt.top_p[row_i] : opt.top_p_all;
   const float min_p = opt.min_p ? opt.min_p[row_i] : opt.min_p_all;
   const bool greedy = !(T > SM_GREEDY_T) || top_k == 1;
-  if (greedy) T = 1.f;
   Weigher w;
   row.has_inf = mkey == kInfKey;
-  w.mf = row.has_inf ? kMaxFinite : key_value(mkey);
-  w.m = (double)w.mf;
+  if (greedy || row.has_inf) T = 1.f;    // (whatever the temperature, only the infinities have weight)
+  const float top_logit = row.has_inf ? kMaxFinite : key_value(mkey);
+  w.m = (double)top_logit;
   w.c = 128.0 * 1.4426950408889634074 / (double)T;
-  w.cf = (float)(w.c / 128.0);
+  w.scale = T > 1e30f ? 0x1p-100f : 0.5f;
+  w.ms = top_logit * w.scale;
+  w.cs = (float)(w.c / 128.0 / (double)w.scale);
   w.tab = sh->tab + (lane & 15);
   const double x_max = min_p > 0.f ? -128.0 * log2((double)fminf(min_p, 1.f)) : INFINITY;   // of 128 x
   float uv = u[(size_t)row_i * u_ld + (u_index ? min(max(u_index[row_i], 0), u_len - 1) : 0)];
   uv = fminf(uv, 0.99999994f);           // the largest number below 1
   u64 cut = 0ull;
   if (greedy) {
-    cut = nth_equal(c, row, order_key(__float_as_uint(w.mf)), 0ull);
+    cut = nth_equal(c, row, order_key(__float_as_uint(top_logit)), 0ull);
     c.phase ^= 1;                        // it exchanged once
   } else {
     unsigned eligible = (unsigned)lim, listed = 0u;

@@ -19,6 +19,7 @@ from . import _lib
 from .fastweight import _launch, _require_cuda
 
 Setting = Union[None, int, float, torch.Tensor]
+MAX_VOCAB = 262144
 
 
 class Sampled(NamedTuple):
@@ -112,8 +113,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
     if logits.dim() != 2 or not (is_f32 or logits.dtype is torch.bfloat16):
         raise ValueError("logits must be FP32 or BF16 (rows, V) with V > 6")
     rows, V = logits.shape
-    if V <= 6:
-        raise ValueError("logits must be FP32 or BF16 (rows, V) with V > 6")
+    if not 6 < V <= MAX_VOCAB:
+        raise ValueError(f"logits must be FP32 or BF16 (rows, V) with 6 < V <= {MAX_VOCAB}")
     n_u = 1 if u.dim() == 1 else u.shape[-1]
     if u.get_device() != index or u.dtype is not f or u.dim() > 2 or u.shape[0] != rows or not u.is_contiguous():
         raise ValueError("u must be a contiguous FP32 (rows,) or (rows, n) tensor beside the logits")
@@ -132,7 +133,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
         raise ValueError("u_index must be a contiguous int32 (rows,) tensor beside the logits")
     else:
         at = u_index.data_ptr()
-    limit = V if active_limit is None else int(active_limit)
+    limit = V if active_limit is None else min(V, int(active_limit))
     if limit <= 2:
         raise ValueError("Active vocabulary must include EOS")
     tp, t0 = _per_row("temperature", temperature, 1.0, f, rows, index)
