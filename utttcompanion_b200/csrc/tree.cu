@@ -42,7 +42,8 @@ constexpr int TR_MAX_REP = 8;
 __device__ __forceinline__ float bfr(float x) { return __bfloat162float(__float2bfloat16(x)); }
 
 constexpr int TR_KT = 64;                // keys per tile (and the most nodes of a tree)
-constexpr int TR_NS = 3;                 // tiles in flight (head dim 32)
+constexpr int TR_HD = 32;                // head dim of the mma.sync kernel ...
+constexpr int TR_NS = 3;                 // ... and its tiles in flight
 
 typedef unsigned long long u64;
 
@@ -65,12 +66,9 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// byte offset of 16-byte chunk c of row r in a tile of HD-element rows; the XOR spreads the 8 rows of an
+// byte offset of 16-byte chunk c of row r in a tile of 32-element rows; the XOR spreads the 8 rows of an
 // ldmatrix over all banks
-template <int HD>
-__device__ __forceinline__ uint32_t tile_off(int r, int c) {
-  return (uint32_t)(r * HD * 2 + ((HD >= 64 ? c ^ (r & 7) : c ^ ((r >> 1) & 3)) << 4));
-}
+__device__ __forceinline__ uint32_t tile_off(int r, int c) { return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); }
 
 __device__ __forceinline__ bool has_nonfinite(uint32_t v) {   // either BF16 half
   return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u;
@@ -332,12 +330,12 @@ __device__ __forceinline__ void store_out(const TreeArgs& a, int b, int g, int r
   }
 }
 
-template <int HD, int WM>
+template <int WM>
 __host__ __device__ constexpr int tree_threads() { return 32 * (WM < 4 ? 4 : WM); }
 // the tiles; at the end the warps' partials and, behind them, the rows that the cluster sends
-template <int HD, int WM>
+template <int WM>
 constexpr int tree_smem() {
-  constexpr int tiles = TR_NS * 2 * TR_KT * HD * 2, ends = (tree_threads<HD, WM>() / 32 + WM) * 16 * (HD + 4) * 4;
+  constexpr int tiles = TR_NS * 2 * TR_KT * TR_HD * 2, ends = (tree_threads<WM>() / 32 + WM) * 16 * (TR_HD + 4) * 4;
   return tiles > ends ? tiles : ends;
 }
 
@@ -362,9 +360,9 @@ inline int tree_split(long long ctas, int tiles, int per_sm, int head, int join)
 // use every warp; three tiles are in flight.
 // grid (S, n_kv * row blocks, B), cluster (S, 1, 1): CTA z takes tiles [nt * z / S, nt * (z + 1) / S) of the nt
 // 64-key tiles: tile 0 holds the drafted keys, tile t > 0 the ring's places 64 (t - 1) ..
-template <int HD, int WM>
-__global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const TreeArgs a) {
-  constexpr int THREADS = tree_threads<HD, WM>(), NW = THREADS / 32, WK = NW / WM;
+template <int WM>
+__global__ void __launch_bounds__(tree_threads<WM>()) attn_tree_kernel(const TreeArgs a) {
+  constexpr int HD = TR_HD, THREADS = tree_threads<WM>(), NW = THREADS / 32, WK = NW / WM;
   constexpr int RB = 16 * WM;            // rows of the CTA
   constexpr int KW = TR_KT / WK;         // keys of a tile per warp
   constexpr int SUB = KW < 32 ? KW : 32;  // keys between two updates of the running maximum
@@ -399,8 +397,8 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
       const int r = i / CH, c = i % CH, j = (t - 1) * TR_KT + r;
       const bool ok = j < nvalid;
       const size_t o = ring0 + (size_t)(ok ? j : 0) * HD + c * 8;
-      cp_async_16(ks + tile_off<HD>(r, c), a.kring + o, ok);
-      cp_async_16(ks + TILE + tile_off<HD>(r, c), a.vring + o, ok);
+      cp_async_16(ks + tile_off(r, c), a.kring + o, ok);
+      cp_async_16(ks + TILE + tile_off(r, c), a.vring + o, ok);
     }
   };
 #pragma unroll
@@ -447,14 +445,14 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
   uint8_t* sQ = smem + (TR_NS - 1) * 2 * TILE;
   rope_nodes<HD>(
       tid, THREADS, n, b, g, p0, row0, RB, has_tree, a, &bad_tree, [&](int node) { return depth_s[node]; },
-      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(sQ + tile_off<HD>(r, c)) = v; },
-      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(smem + tile_off<HD>(r, c)) = v; },
-      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(smem + TILE + tile_off<HD>(r, c)) = v; });
+      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(sQ + tile_off(r, c)) = v; },
+      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(smem + tile_off(r, c)) = v; },
+      [&](int r, int c, uint4 v) { *reinterpret_cast<uint4*>(smem + TILE + tile_off(r, c)) = v; });
   __syncthreads();
   uint32_t qf[HD / 16][4];
 #pragma unroll
   for (int k = 0; k < HD / 16; ++k)
-    ldsm4(qf[k], smem_u32(sQ) + tile_off<HD>(wm * 16 + (lane & 15), 2 * k + (lane >> 4)));
+    ldsm4(qf[k], smem_u32(sQ) + tile_off(wm * 16 + (lane & 15), 2 * k + (lane >> 4)));
 
   // ---- this thread's two rows (lane / 4 and + 8 of its warp's 16)
   int dep[2];
@@ -497,7 +495,7 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
           if (tid == 0) bad_keys = 0ull;
           __syncthreads();
           finite_values<HD>(tid, THREADS, some & valid, &bad_keys, [&](int r, int c) {
-            return reinterpret_cast<uint4*>(ks + TILE + tile_off<HD>(r, c));
+            return reinterpret_cast<uint4*>(ks + TILE + tile_off(r, c));
           });
           __syncthreads();
           bad = bad_keys;
@@ -519,7 +517,7 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
 #pragma unroll
         for (int i = 0; i < SUB / 16; ++i) {
           uint32_t kf[4];
-          ldsm4(kf, ka + tile_off<HD>(kb + i * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+          ldsm4(kf, ka + tile_off(kb + i * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
           mma16816(s[2 * i], qf[k], kf[0], kf[1]);
           mma16816(s[2 * i + 1], qf[k], kf[2], kf[3]);
         }
@@ -579,7 +577,7 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
 #pragma unroll
         for (int cc = 0; cc < HD / 16; ++cc) {
           uint32_t vf[4];
-          ldsm4_t(vf, va + tile_off<HD>(kb + i * 16 + (lane & 15), 2 * cc + (lane >> 4)));
+          ldsm4_t(vf, va + tile_off(kb + i * 16 + (lane & 15), 2 * cc + (lane >> 4)));
           mma16816(o[2 * cc], ph[i], vf[0], vf[1]);
           mma16816(o[2 * cc + 1], ph[i], vf[2], vf[3]);
           mma16816(o[2 * cc], pl[i], vf[0], vf[1]);
@@ -685,20 +683,20 @@ __global__ void __launch_bounds__(tree_threads<HD, WM>()) attn_tree_kernel(const
   }
 }
 
-template <int HD, int WM>
+template <int WM>
 int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
   static DeviceOnce attr;
   UTTT_TRY(run_once_per_device(attr, [] {
-    return cuda_status(cudaFuncSetAttribute(attn_tree_kernel<HD, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            tree_smem<HD, WM>()));
+    return cuda_status(cudaFuncSetAttribute(attn_tree_kernel<WM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            tree_smem<WM>()));
   }));
   const int blocks = (a.N * a.rep + 16 * WM - 1) / (16 * WM);
   UTTT_REQUIRE((long long)a.n_kv * blocks <= 65535, UTTT_ERR_UNSUPPORTED);
   const int S = tree_split((long long)B * a.n_kv * blocks, (a.W + TR_KT - 1) / TR_KT + 1, WM == 8 ? 1 : 2, 4, 1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(S, a.n_kv * blocks, B);
-  cfg.blockDim = dim3(tree_threads<HD, WM>());
-  cfg.dynamicSmemBytes = tree_smem<HD, WM>();
+  cfg.blockDim = dim3(tree_threads<WM>());
+  cfg.dynamicSmemBytes = tree_smem<WM>();
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -708,7 +706,7 @@ int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
   at[1] = pdl_attribute();
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, attn_tree_kernel<HD, WM>, a) != cudaSuccess) return launch_status();
+  if (cudaLaunchKernelEx(&cfg, attn_tree_kernel<WM>, a) != cudaSuccess) return launch_status();
   return launch_status();
 }
 
@@ -996,7 +994,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       const int t = t_lo + i, s = i & 1, j0 = (t - 1) * TR_KT;
       const bool is_tree = t == 0;
       // keys that not every row sees: the tree's, the ring's behind the last valid place and around the window's
-      // edge.  Values that must not reach the rows that do not see them leave the product (tree_values).
+      // edge.  Values that must not reach the rows that do not see them leave the product (finite_values).
       const bool edge = !is_tree && (j0 + TR_KT > nvalid || (j0 <= next + max_dep && j0 + TR_KT > next) ||
                                      j0 <= next - W + max_dep);
       u64 seen = is_tree ? anc : ~0ull;
@@ -1220,19 +1218,6 @@ int launch_tree_tc(const TreeArgs& a, int B, cudaStream_t st) {
   return launch(0, B, S, 0);
 }
 
-template <int HD>
-int launch_tree_rows(const TreeArgs& a, int B, cudaStream_t st) {
-  if constexpr (HD >= 64) {
-    return launch_tree_tc<HD>(a, B, st);
-  } else {
-    const int rows = a.N * a.rep;
-    if (rows <= 16) return launch_tree<HD, 1>(a, B, st);
-    if (rows <= 32) return launch_tree<HD, 2>(a, B, st);
-    if (rows <= 64) return launch_tree<HD, 4>(a, B, st);
-    return launch_tree<HD, 8>(a, B, st);
-  }
-}
-
 // One warp per row; lane l holds nodes l and l + 32.  From node 0 on, the path goes to the lowest later child
 // whose token is the pick after its parent.
 __global__ void tree_accept_kernel(int B, int N, const int* __restrict__ tokens, const int* __restrict__ parents,
@@ -1316,9 +1301,13 @@ extern "C" int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W
   a.vec_in = at16(qkv) && qkv_ld % 8 == 0 && at16(rope_cos) && at16(rope_sin);
   a.vec_out = at16(out) && out_ld % 8 == 0;
   a.b0 = a.joins = 0;
-  if (hd == 32) return launch_tree_rows<32>(a, B, st);
-  if (hd == 64) return launch_tree_rows<64>(a, B, st);
-  return launch_tree_rows<128>(a, B, st);
+  if (hd == 128) return launch_tree_tc<128>(a, B, st);
+  if (hd == 64) return launch_tree_tc<64>(a, B, st);
+  const int rows = N * a.rep;
+  if (rows <= 16) return launch_tree<1>(a, B, st);
+  if (rows <= 32) return launch_tree<2>(a, B, st);
+  if (rows <= 64) return launch_tree<4>(a, B, st);
+  return launch_tree<8>(a, B, st);
 }
 
 extern "C" int uttt_tree_accept(int B, int N, const int* tokens, const int* parents, const int* n_nodes,
