@@ -373,8 +373,10 @@ int uttt_kv_ring_fill(int B, int L, int end_pos, int n_kv, int hd, int W, const 
  *   out     BF16 rows (B * N, out_ld), heads concatenated
  * Nothing is written for the nodes behind a row's last, nor for rows with a slot
  * outside [0, n_slots) or a negative position.  Nothing that a node does not see
- * reaches it, whatever its bits.  hd in {32, 64, 128}, n_heads / n_kv <= 8,
- * N <= 64.  No workspace.
+ * reaches it, whatever its bits (a NaN or an infinity that it does see makes its
+ * output NaN or infinite).  hd in {32, 64, 128}, n_heads / n_kv <= 8, N <= 64;
+ * rings, k_tree and v_tree 16-byte aligned (UTTT_ERR_UNSUPPORTED otherwise), qkv,
+ * out and the tables at any address and row stride.  No workspace.
  */
 int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos, const void* qkv,
                    int qkv_ld, const int* parents, const int* n_nodes, const int* pos, const int* slot,

@@ -137,6 +137,7 @@ def test_drafted_generation_limits_and_refusals():
     one, steps = eng.generate_drafted(prompt, st, 1, tree.PromptLookup())
     assert len(one) == 1 and steps == 0
     assert eng.generate_drafted(prompt, st, 0, tree.PromptLookup())[0] == []
+    assert eng.generate_drafted(prompt, st, 0, tree.PromptLookup(), temperature=0.5, u=torch.zeros(0))[0] == []
     three, _ = eng.generate_drafted(prompt, st, 3, lambda ids: (list(range(6, 26)), list(range(20))))
     assert len(three) == 3
     for bad in (lambda ids: ([7], []), lambda ids: ([7], [1]), lambda ids: ([512], [0]), lambda ids: ([-1], [0]),
@@ -225,7 +226,7 @@ def test_serving_samples_each_turn_with_its_own_settings():
     srv.run()
     _check_reply(eng, torch.tensor(prompts[0]), st, again.reply, slot=4)
     for bad in (dict(max_new_tokens=25, temperature=0.5), dict(temperature=float("nan")), dict(top_p=2.0),
-                dict(min_p=-1.0)):
+                dict(min_p=-1.0), dict(temperature=0.5, seed=-1), dict(temperature=0.5, seed=2 ** 63)):
         with pytest.raises(ValueError):
             srv.submit("x", prompts[0], **{"max_new_tokens": 8, **bad})
     with pytest.raises(ValueError):

@@ -208,6 +208,12 @@ def test_attention_refusals():
         _run(c, 4, out=torch.zeros(8, 255, dtype=torch.bfloat16, device=DEV))
     with pytest.raises(ValueError):
         _run(c, 4, k_tree=torch.zeros(2, 2, 5, 64, dtype=torch.bfloat16, device=DEV))
+    c = _case(1, 2, 4, 2, 64, 32, [1], seed=10)
+    far = torch.empty(2 ** 31 + 512, dtype=torch.bfloat16, device=DEV)      # rows 2^31 elements apart
+    with pytest.raises(ValueError):
+        _run({**c, "qkv": far.as_strided((2, 512), (2 ** 31, 1))}, 4)
+    with pytest.raises(ValueError):
+        _run(c, 4, out=far.as_strided((2, 256), (2 ** 31, 1)))
 
 
 # ------------------------------------------------------------------------------------------------ accepted path
@@ -302,9 +308,12 @@ def test_fork_many_pairs_and_refusals():
     kv_cache.ring_fork(rings, [], [])
     kv_cache.ring_fork(rings, [3], [3])
     now = rings.clone()
-    for src, dst in (([0, 1], [1, 0]), ([0], [600]), ([-1], [2]), ([0, 1], [5, 5])):
+    for src, dst in (([0, 1], [1, 0]), ([0], [600]), ([-1], [2]), ([0, 1], [5, 5]), ([2 ** 32], [1]),
+                     ([0], [2 ** 32 + 1])):
         with pytest.raises(ValueError):
             kv_cache.ring_fork(rings, src, dst)
     with pytest.raises(ValueError):
         kv_cache.ring_fork(rings[:, :, ::2], [0], [1])
+    with pytest.raises(ValueError):
+        kv_cache.ring_fork(rings, [0], [1], [-2 ** 33])
     assert torch.equal(rings, now)

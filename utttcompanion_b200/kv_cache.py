@@ -65,6 +65,8 @@ def ring_fork(rings: torch.Tensor, src: Sequence[int], dst: Sequence[int],
         raise ValueError("src, dst and end_pos must have one entry per pair")
     if n == 0:
         return
+    if min(src) < 0 or max(src) >= S or min(dst) < 0 or max(dst) >= S or (end_pos is not None and min(end_pos) < 0):
+        raise ValueError("slot out of range, or a negative position")
     arr = C.c_int * n
     ring_stride, r = S * n_kv * W * hd, rings.data_ptr()
     dev = rings.device

@@ -540,6 +540,8 @@ class UtttB200:
         sampled = temperature > 1e-5
         if sampled and (u is None or u.numel() < n_tokens):
             raise ValueError("sampled generation needs one number per token")
+        if n_tokens < 1:
+            return [], 0
         packed, down = self.read_copies(state.w_up, state.w_gate, state.w_down)
         dev = self.device
         u = u.to(device=dev, dtype=torch.float32).reshape(-1).contiguous() if sampled else None
@@ -561,7 +563,7 @@ class UtttB200:
                 return True
             ids.append(tok)
             return len(ids) >= n_tokens or (not stop_free and eos_token_id is not None and tok == eos_token_id)
-        done = n_tokens < 1 or ended(pending)
+        done = ended(pending)
         while not done:
             drafted, above = draft(seq + ids)
             tokens, parents = [ids[-1], *(int(t) for t in drafted)], [-1, *(int(p) for p in above)]
@@ -607,8 +609,8 @@ class UtttB200:
                 or min(slots) < 0 or max(slots) >= self.max_personas:
             raise ValueError("one KV slot of the engine per reply")
         T = prompt.numel()
-        if T + n_tokens >= self.n_pos:
-            raise ValueError("reply longer than the RoPE table")
+        if T < 1 or T + n_tokens >= self.n_pos:
+            raise ValueError("empty prompt, or a reply longer than the RoPE table")
         packed, down = self.read_copies(state.w_up, state.w_gate, state.w_down)
         dev = self.device
         u = torch.stack([sampling.reply_uniforms(n_tokens, seed + r) for r in range(n_replies)])

@@ -314,6 +314,8 @@ class ServingEngine:
             if max_new_tokens > self.max_sampled_tokens:
                 raise ValueError(f"this engine samples replies of up to {self.max_sampled_tokens} tokens "
                                  "(max_sampled_tokens)")
+            if seed is not None and (type(seed) is not int or not 0 <= seed < 2 ** 63):
+                raise ValueError("seed must be an integer from 0 to 2**63 - 1")
             if seed is None:
                 seed = int(torch.randint(2 ** 62, ()).item())
         t = Turn(str(user_id), list(prompt_ids), max_new_tokens, eos_token_id, on_event=on_event,

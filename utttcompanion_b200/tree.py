@@ -16,6 +16,7 @@ from . import _lib
 from .fastweight import _launch, _require_cuda
 
 MAX_NODES = 64
+MAX_LD = 2 ** 31                     # elements from one row to the next
 
 
 def check_tree(parents: Sequence[int]) -> None:
@@ -115,7 +116,7 @@ def tree_attention(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, 
     if n_heads < 1 or n_heads % n_kv or qkv.dtype is not bf or qkv.dim() != 2 or qkv.shape[0] != R:
         raise ValueError("qkv must be BF16 (B * N, (n_heads + 2 * n_kv) * hd) rows")
     qkv_ld, step = qkv.stride()
-    if step != 1 or qkv.shape[1] < q_dim + 2 * n_kv * hd:
+    if step != 1 or qkv.shape[1] < q_dim + 2 * n_kv * hd or qkv_ld >= MAX_LD:
         raise ValueError("qkv must be BF16 (B * N, (n_heads + 2 * n_kv) * hd) rows")
     table = rope_cos.shape
     for t in (rope_cos, rope_sin):
@@ -128,7 +129,7 @@ def tree_attention(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, 
     elif out.get_device() != index or out.dtype is not bf or out.shape != (R, q_dim):
         raise ValueError("out must be BF16 (B * N, n_heads * hd) rows")
     out_ld, step = out.stride()
-    if step != 1 and R:
+    if (step != 1 or out_ld >= MAX_LD) and R:
         raise ValueError("out must be BF16 (B * N, n_heads * hd) rows")
     kv_shape = (B, n_kv, N, hd)
     k_tree = torch.zeros(kv_shape, dtype=bf, device=dev) if k_tree is None else k_tree
