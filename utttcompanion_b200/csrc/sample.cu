@@ -69,12 +69,14 @@ struct SampleShared {
   double tab[SM_STEPS * 16];             // the table 16 times: the lanes of a half-warp meet no bank conflicts
   Sel xch[2][SM_MAX_CTAS];               // one slot per CTA, two phases
   u64 wred[SM_WARPS], wred2[SM_WARPS];
-  u64 cand[2][SM_CAP];                   // rank 0: gathered candidates; others: their copies of them
-  u64 cand_w[SM_CAP];
-  unsigned n_cand[2];                    // rank 0; gathers alternate between the two lists
+  u64 found[2][SM_CAP];                  // this CTA's gathered candidates; gathers alternate between the two lists
+  u64 cand[SM_CAP], cand_w[SM_CAP];      // the whole cluster's, and their weights
+  unsigned n_found[2];
   u64 res_base, res_held, res_cut;
   int res_bin;
+  u64 more[SM_MAX_CTAS * SM_WARPS];      // what every warp of the cluster has beyond the bins
   alignas(16) unsigned hist[3][SM_BINS];  // count, or 16-bit limbs of the mass
+  alignas(16) u64 merged[SM_BINS];       // the cluster's histogram
 };
 
 // 2^45 * 2^(-j / 128)
@@ -194,11 +196,35 @@ __device__ __forceinline__ u64 warp_max64(u64 v) {
   return v;
 }
 
-// the larger number, subnormal ones too (the compiler's own flag would flush them); a NaN loses
-__device__ __forceinline__ float max_exact(float a, float b) {
+// the largest number, subnormal ones too (the compiler's own flag would flush them); a NaN loses
+__device__ __forceinline__ float max_exact(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// Sums over the CTA's warps of two numbers that every lane of a warp has, and the first one's over the warps before
+// this one.  Each warp adds its 16 numbers by shuffles: read one by one they are 16 warps' worth of issue slots.
+struct Sums {
+  u64 a, b, a_below;
+};
+__device__ __forceinline__ Sums block_sums(SampleShared* sh, u64 a, u64 b) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = lane & (SM_WARPS - 1);
+  __syncthreads();
+  if (lane == 0) {
+    sh->wred[warp] = a;
+    sh->wred2[warp] = b;
+  }
+  __syncthreads();
+  Sums s{sh->wred[w], sh->wred2[w], 0ull};
+  if (w < warp) s.a_below = s.a;
+#pragma unroll
+  for (int o = SM_WARPS / 2; o > 0; o >>= 1) {
+    s.a += __shfl_xor_sync(0xffffffffu, s.a, o);
+    s.b += __shfl_xor_sync(0xffffffffu, s.b, o);
+    s.a_below += __shfl_xor_sync(0xffffffffu, s.a_below, o);
+  }
+  return s;
 }
 
 // floor(x * total) for x in [0, 1): exact for every x >= 2^-40
@@ -210,7 +236,7 @@ __device__ __forceinline__ u64 part_of(float x, u64 total) {
 struct Cluster {
   cg::cluster_group cl;
   SampleShared* sh;
-  int rank, S, phase, list;
+  int rank, S, phase, list;              // list: of the last gather
   __device__ __forceinline__ SampleShared* peer(int r) { return S == 1 ? sh : cl.map_shared_rank(sh, r); }
   __device__ __forceinline__ void sync() {
     if (S == 1)
@@ -231,6 +257,23 @@ struct Cluster {
     if ((int)threadIdx.x < S) peer(threadIdx.x)->xch[ph][rank] = v;   // v is the same in every thread
     sync();
     return ph;
+  }
+  // sums of what the CTAs gave, and the first one's over the CTAs before this one
+  __device__ __forceinline__ Sums sums(int ph) const {
+    const int r = threadIdx.x & (SM_MAX_CTAS - 1);
+    Sums s{0ull, 0ull, 0ull};
+    if (r < S) {
+      s.a = sh->xch[ph][r].a;
+      s.b = sh->xch[ph][r].b;
+      if (r < rank) s.a_below = s.a;
+    }
+#pragma unroll
+    for (int o = SM_MAX_CTAS / 2; o > 0; o >>= 1) {
+      s.a += __shfl_xor_sync(0xffffffffu, s.a, o);
+      s.b += __shfl_xor_sync(0xffffffffu, s.b, o);
+      s.a_below += __shfl_xor_sync(0xffffffffu, s.a_below, o);
+    }
+    return s;
   }
 };
 
@@ -258,12 +301,14 @@ struct Row {
   const char* src;        // the row
   bool vec;               // whether it starts on 16 bytes
   bool has_inf;           // whether its largest logit is +inf
+  bool kept;              // whether the whole piece is in the ring, from an earlier walk
   int V, lim, stop_free;
   int v0, v1;
   uint4* ring;            // the warp's places in shared memory
 
   // f(bits[8], first id) for every vector of the piece, in step over the warp, until it returns false; ids that are
-  // never picked come as -inf.  Vectors arrive by cp.async, each lane's own ones in its own places, a few ahead.
+  // never picked come as -inf.  Vectors arrive by cp.async, each lane's own ones in its own places, a few ahead; a
+  // piece of no more vectors than places stays there for the walks after the first.
   template <class F>
   __device__ __forceinline__ void each(F f) const {
     const int lane = threadIdx.x & 31;
@@ -284,14 +329,18 @@ struct Row {
       vf += 32;
       sf = (sf + 1) & (ahead - 1);
     };
+    if (!kept) {
 #pragma unroll 1
-    for (int k = 0; k < ahead - 1; ++k) fetch();
+      for (int k = 0; k < ahead - 1; ++k) fetch();
+    }
     unsigned sr = 0;
 #pragma unroll 1
     for (int t = v0; t < v1; t += 32) {
       const int v = t + lane;
-      fetch();
-      cp_async_wait<ahead - 1>();
+      if (!kept) {
+        fetch();
+        cp_async_wait<ahead - 1>();
+      }
       unsigned x[8];
       const uint4* at = mine + sr * (W * 32);
       sr = (sr + 1) & (ahead - 1);
@@ -333,14 +382,14 @@ __device__ __forceinline__ unsigned nth_of(const unsigned (&x)[8], int e) {
   return r;
 }
 
-// Gather the pairs that in_range(bits, id) takes (of all CTAs) into rank 0's list; returns how many there are.
-// near(bits) is a quick test that lets all of them pass and few others.  Every CTA
-// then holds a copy in cand[c.list] if they are at most SM_CAP.  Consecutive gathers use the two lists in turn, so
-// a CTA may start the next one while another still ranks this one's; the other list's counter is cleared between
-// this gather's two barriers, after its last reader and before its next writer.
+// Gather the pairs that in_range(bits, id) takes, of all CTAs; returns how many there are.  near(bits) is a quick test
+// that lets all of them pass and few others.  Every CTA gathers its own in a list and, if they are at most SM_CAP in
+// all, copies the cluster's lists into cand.  Consecutive gathers use the two lists in turn, so a CTA may start the next
+// one while another still copies; the other list's counter is cleared behind this gather's barrier, after its last
+// reader and before its next writer.
 template <bool F32, class Near, class InRange>
 __device__ unsigned gather(Cluster& c, const Row<F32>& row, Near near, InRange in_range) {
-  SampleShared* lead = c.peer(0);
+  SampleShared* sh = c.sh;
   const int q = c.list ^= 1;
   row.each([&](const unsigned (&x)[8], int id) {
     unsigned mask = 0u;
@@ -350,18 +399,27 @@ __device__ unsigned gather(Cluster& c, const Row<F32>& row, Near near, InRange i
       const int e = __ffs((int)mask) - 1;
       const unsigned xe = nth_of(x, e);
       if (in_range(xe, id + e)) {
-        const unsigned at = atomicAdd(&lead->n_cand[q], 1u);
-        if (at < SM_CAP) lead->cand[q][at] = pair_of(order_key(xe), id + e);
+        const unsigned at = atomicAdd(&sh->n_found[q], 1u);
+        if (at < SM_CAP) sh->found[q][at] = pair_of(order_key(xe), id + e);
       }
     }
     return true;
   });
   c.sync();
-  const unsigned n = lead->n_cand[q];
-  if (n <= SM_CAP && c.rank != 0)
-    for (unsigned i = threadIdx.x; i < n; i += SM_THREADS) c.sh->cand[q][i] = lead->cand[q][i];
-  if (c.rank == 0 && threadIdx.x == 0) c.sh->n_cand[q ^ 1] = 0u;
-  c.sync();
+  unsigned n = 0u, from = 0u, mine = 0u;   // cand[threadIdx.x] is number `mine` of CTA `from`
+#pragma unroll
+  for (int r = 0; r < SM_MAX_CTAS; ++r)
+    if (r < c.S) {
+      const unsigned k = c.peer(r)->n_found[q];
+      if (threadIdx.x >= n) {
+        from = r;
+        mine = threadIdx.x - n;
+      }
+      n += k;
+    }
+  if (threadIdx.x < n && n <= SM_CAP) sh->cand[threadIdx.x] = c.peer(from)->found[q][mine];
+  if (threadIdx.x == 0) sh->n_found[q ^ 1] = 0u;
+  __syncthreads();
   return n;
 }
 
@@ -369,7 +427,7 @@ __device__ unsigned gather(Cluster& c, const Row<F32>& row, Near near, InRange i
 // Every CTA computes the same.  0 if there is none.
 __device__ u64 rank_candidates(Cluster& c, unsigned n, int mode, u64 target, const Weigher& w) {
   SampleShared* sh = c.sh;
-  const u64* cand = sh->cand[c.list];
+  const u64* cand = sh->cand;
   u64 mine = 0ull, own = 0ull;
   __syncthreads();
   if (threadIdx.x == 0) sh->res_cut = 0ull;
@@ -389,72 +447,96 @@ __device__ u64 rank_candidates(Cluster& c, unsigned n, int mode, u64 target, con
   return sh->res_cut;
 }
 
-// The merged histogram's bin that holds `target`, what lies before it and what is in it, the same in every CTA; `total`:
-// of all bins.  With top_p > 0 the target is that part of total + more (mass), and written back.  The bin is -1 if the target
-// lies behind all bins.
+// This CTA's share of the bins, added up over a cluster of S and sent to all of it.  All loads are in flight together
+// (under a test of S each waited for the one before it: 6500 cycles for 8 CTAs).
+template <int S>
+__device__ __forceinline__ void merge_bins(Cluster& c, int mode) {
+  SampleShared* p[S];
+#pragma unroll
+  for (int r = 0; r < S; ++r) p[r] = c.cl.map_shared_rank(c.sh, r);
+  for (int i = threadIdx.x; i < SM_BINS / S; i += SM_THREADS) {
+    const int bin = c.rank * (SM_BINS / S) + i;
+    unsigned h0[S], h1[S], h2[S];
+#pragma unroll
+    for (int r = 0; r < S; ++r) h0[r] = p[r]->hist[0][bin];
+    u64 v = 0ull;
+    if (mode == FIND_MASS) {
+#pragma unroll
+      for (int r = 0; r < S; ++r) {
+        h1[r] = p[r]->hist[1][bin];
+        h2[r] = p[r]->hist[2][bin];
+      }
+#pragma unroll
+      for (int r = 0; r < S; ++r) v += ((u64)h1[r] << 16) + ((u64)h2[r] << 32);
+    }
+#pragma unroll
+    for (int r = 0; r < S; ++r) v += h0[r];
+#pragma unroll
+    for (int r = 0; r < S; ++r) p[r]->merged[bin] = v;
+  }
+}
+
+// The cluster's histogram's bin that holds `target`, what lies before it and what is in it, the same in every CTA;
+// `total`: of all bins.  With top_p > 0 the target is that part of total + more (mass), and written back.  The bin is -1
+// if the target lies behind all bins.  Every CTA adds up its share of the bins over the cluster and sends the sums to
+// all, who then look for the bin each: two cluster barriers, and remote loads that are in flight together.
 __device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, u64& base_out, u64& held,
                       u64& total) {
   SampleShared* sh = c.sh;
-  c.sync();
-  // this CTA sums its share of the bins over the cluster: thread t has PB consecutive ones
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int Q = SM_BINS / SM_THREADS;
-  const int share = SM_BINS / c.S, b0 = c.rank * share, PB = (share + SM_THREADS - 1) / SM_THREADS;
-  u64 val[Q], sum = 0ull;
+  u64 val[Q];
+  more = warp_sum64(more);
+  c.sync();
+  if (c.S == 1) {
+    const uint4 h0 = reinterpret_cast<const uint4*>(sh->hist[0])[tid];
+    val[0] = h0.x, val[1] = h0.y, val[2] = h0.z, val[3] = h0.w;
+    if (mode == FIND_MASS) {
+      const uint4 h1 = reinterpret_cast<const uint4*>(sh->hist[1])[tid], h2 = reinterpret_cast<const uint4*>(sh->hist[2])[tid];
+      val[0] += ((u64)h1.x << 16) + ((u64)h2.x << 32), val[1] += ((u64)h1.y << 16) + ((u64)h2.y << 32);
+      val[2] += ((u64)h1.z << 16) + ((u64)h2.z << 32), val[3] += ((u64)h1.w << 16) + ((u64)h2.w << 32);
+    }
+  } else {
+    if (c.S == 2) merge_bins<2>(c, mode);
+    if (c.S == 4) merge_bins<4>(c, mode);
+    if (c.S == 8) merge_bins<8>(c, mode);
+    if (lane < c.S) c.peer(lane)->more[c.rank * SM_WARPS + warp] = more;
+    c.sync();
+    const ulonglong2* m = reinterpret_cast<const ulonglong2*>(sh->merged) + tid * (Q / 2);
 #pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    val[q] = 0ull;
-    const int bl = threadIdx.x * PB + q;
-    if (q < PB && bl < share)
-      for (int r = 0; r < c.S; ++r) {
-        const SampleShared* p = c.peer(r);
-        val[q] += p->hist[0][b0 + bl];
-        if (mode == FIND_MASS) val[q] += ((u64)p->hist[1][b0 + bl] << 16) + ((u64)p->hist[2][b0 + bl] << 32);
-      }
-    sum += val[q];
+    for (int q = 0; q < Q; q += 2) {
+      val[q] = m[q / 2].x;
+      val[q + 1] = m[q / 2].y;
+    }
+    more = 0ull;
+    for (int i = lane; i < c.S * SM_WARPS; i += 32) more += sh->more[i];
+    more = warp_sum64(more);
   }
-  u64 inc = sum;                         // prefix over the CTA's threads
+  u64 sum = 0ull;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) sum += val[q];
+  u64 inc = sum;                         // prefix over the threads
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
-    if ((threadIdx.x & 31) >= o) inc += t;
+    if (lane >= o) inc += t;
   }
-  more = warp_sum64(more);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 31) {
-    sh->wred[threadIdx.x >> 5] = inc;
-    sh->wred2[threadIdx.x >> 5] = more;
-  }
-  __syncthreads();
-  u64 base = 0ull, mine = 0ull;
-  more = 0ull;
-  for (int i = 0; i < SM_WARPS; ++i) {
-    if (i < (int)(threadIdx.x >> 5)) base += sh->wred[i];
-    mine += sh->wred[i];
-    more += sh->wred2[i];
-  }
-  if (threadIdx.x == 0) sh->res_bin = -1;
-  const int ph = c.exchange(Sel{mine, more});
-  total = 0ull;
-  more = 0ull;
-  for (int r = 0; r < c.S; ++r) {
-    if (r < c.rank) base += sh->xch[ph][r].a;
-    total += sh->xch[ph][r].a;
-    more += sh->xch[ph][r].b;
-  }
+  if (tid == 0) sh->res_bin = -1;
+  const Sums s = block_sums(sh, __shfl_sync(0xffffffffu, inc, 31), more);
+  total = s.a;
+  if (c.S == 1) more = s.b;
   if (top_p > 0.f) target = part_of(top_p, total + more);
-  u64 at = base + inc - sum;
+  u64 at = s.a_below + inc - sum;
 #pragma unroll
   for (int q = 0; q < Q; ++q) {
-    if (at <= target && at + val[q] > target)
-      for (int r = 0; r < c.S; ++r) {
-        SampleShared* p = c.peer(r);
-        p->res_bin = b0 + threadIdx.x * PB + q;
-        p->res_base = at;
-        p->res_held = val[q];
-      }
+    if (at <= target && at + val[q] > target) {
+      sh->res_bin = tid * Q + q;
+      sh->res_base = at;
+      sh->res_held = val[q];
+    }
     at += val[q];
   }
-  c.sync();
+  __syncthreads();
   base_out = sh->res_base;
   held = sh->res_held;
   return sh->res_bin;
@@ -478,7 +560,7 @@ __device__ __forceinline__ void clear_hist(SampleShared* sh) {
 template <bool F32>
 __device__ __noinline__ u64 nth_equal(Cluster c, const Row<F32> row, unsigned key, u64 n) {
   SampleShared* sh = c.sh;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   unsigned count = 0u;
   row.each([&](const unsigned (&x)[8], int) {
 #pragma unroll
@@ -486,16 +568,8 @@ __device__ __noinline__ u64 nth_equal(Cluster c, const Row<F32> row, unsigned ke
     return true;
   });
   count = __reduce_add_sync(0xffffffffu, count);
-  __syncthreads();
-  if (lane == 0) sh->wred[warp] = count;
-  __syncthreads();
-  u64 below = 0ull, all = 0ull;
-  for (int i = 0; i < SM_WARPS; ++i) {
-    if (i < warp) below += sh->wred[i];
-    all += sh->wred[i];
-  }
-  const int ph = c.exchange(Sel{all, 0ull});
-  for (int r = 0; r < c.rank; ++r) below += sh->xch[ph][r].a;
+  const Sums in = block_sums(sh, count, 0ull);
+  const u64 below = in.a_below + c.sums(c.exchange(Sel{in.a, 0ull})).a_below;
   if (below <= n && n < below + count) {   // one warp of the cluster
     u64 at = below;
     row.each([&](const unsigned (&x)[8], int id) {
@@ -543,14 +617,8 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64& 
           return is_candidate(key) && pair_of(key, id) >= cut;
         });
     if (MODE == FIND_MASS) {
-      u64 v = threadIdx.x < n ? w.weight_of_key((unsigned)(sh->cand[c.list][threadIdx.x] >> 32)) : 0ull;
-      v = warp_sum64(v);
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) sh->wred[threadIdx.x >> 5] = v;
-      __syncthreads();
-      u64 total = 0ull;
-      for (int i = 0; i < SM_WARPS; ++i) total += sh->wred[i];
-      target = part_of(top_p, total);
+      const u64 v = threadIdx.x < n ? w.weight_of_key((unsigned)(sh->cand[threadIdx.x] >> 32)) : 0ull;
+      target = part_of(top_p, block_sums(sh, warp_sum64(v), 0ull).a);
     }
     if (cut == 0ull) {
       listed = n;
@@ -720,7 +788,7 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64& 
 __device__ __noinline__ void finish_list(Cluster c, const Weigher w, unsigned n, int top_k, float top_p, u64 mass_limit,
                                          double x_max, float u, int row_i, int* ids, int* kept, float* prob) {
   SampleShared* sh = c.sh;
-  const u64* cand = sh->cand[c.list];
+  const u64* cand = sh->cand;
   const int tid = threadIdx.x;
   u64 mine = 0ull, own = 0ull;
   bool in = tid < (int)n;
@@ -742,21 +810,9 @@ __device__ __noinline__ void finish_list(Cluster c, const Weigher w, unsigned n,
     }
   }
   auto total_of = [&](u64 v, unsigned k, unsigned& count) -> u64 {   // sums of v and k over the threads
-    v = warp_sum64(v);
-    k = __reduce_add_sync(0xffffffffu, k);
-    __syncthreads();
-    if ((tid & 31) == 0) {
-      sh->wred[tid >> 5] = v;
-      sh->wred2[tid >> 5] = k;
-    }
-    __syncthreads();
-    v = 0ull;
-    count = 0u;
-    for (int i = 0; i < SM_WARPS; ++i) {
-      v += sh->wred[i];
-      count += (unsigned)sh->wred2[i];
-    }
-    return v;
+    const Sums t = block_sums(sh, warp_sum64(v), __reduce_add_sync(0xffffffffu, k));
+    count = (unsigned)t.b;
+    return t.a;
   };
   unsigned count;
   if (top_k > 0) {
@@ -797,18 +853,25 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   SampleShared* sh = reinterpret_cast<SampleShared*>(smem);
   Cluster c{cg::this_cluster(), sh, (int)blockIdx.x, (int)gridDim.x, 0, 0};
   const int row_i = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid < 2) sh->n_cand[tid] = 0u;
+  if (tid < 2) sh->n_found[tid] = 0u;
   c.arrive();                            // peers write here only once every CTA of the cluster has started
+  double pow2[SM_STEPS * 16 / SM_THREADS];   // on their way during the first walk
 #pragma unroll
-  for (int k = 0; k < SM_STEPS * 16 / SM_THREADS; ++k) sh->tab[k * SM_THREADS + tid] = kPow2[(k * SM_THREADS + tid) >> 4];
+  for (int k = 0; k < SM_STEPS * 16 / SM_THREADS; ++k) pow2[k] = kPow2[(k * SM_THREADS + tid) >> 4];
   pdl_wait();
   pdl_trigger();
+  // ---- settings of the row
+  float T = opt.temperature ? opt.temperature[row_i] : opt.temperature_all;
+  const int top_k = opt.top_k ? opt.top_k[row_i] : opt.top_k_all;
+  const float top_p = opt.top_p ? opt.top_p[row_i] : opt.top_p_all;
+  const float min_p = opt.min_p ? opt.min_p[row_i] : opt.min_p_all;
+  float uv = u[(size_t)row_i * u_ld + (u_index ? min(max(u_index[row_i], 0), u_len - 1) : 0)];
   // ---- the warp's piece of the row (`part` 8-logit vectors per CTA)
   Row<F32> row;
   row.src = reinterpret_cast<const char*>(logits) + (size_t)row_i * ld * (F32 ? 4 : 2);
   row.vec = (reinterpret_cast<uintptr_t>(row.src) & 15u) == 0;
   row.V = V;
-  row.has_inf = false;
+  row.has_inf = row.kept = false;
   row.lim = lim;
   row.stop_free = stop_free;
   row.ring = sh->ring[warp];
@@ -818,19 +881,19 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   float top = -INFINITY;
   row.each([&](const unsigned (&x)[8], int) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_exact(top, __uint_as_float(x[e]));   // NaN loses
+    for (int e = 0; e < 8; e += 2) top = max_exact(top, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
     return true;
   });
+  row.kept = row.v1 - row.v0 <= 32 * (F32 ? SM_RING / 2 : SM_RING);
+  unsigned mkey = __reduce_max_sync(0xffffffffu, order_key(__float_as_uint(top)));
+  if (lane == 0) sh->wred[warp] = mkey;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_exact(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) sh->wred[warp] = order_key(__float_as_uint(top));
+  for (int k = 0; k < SM_STEPS * 16 / SM_THREADS; ++k) sh->tab[k * SM_THREADS + tid] = pow2[k];
   __syncthreads();
-  u64 best = 0ull;
-  for (int i = 0; i < SM_WARPS; ++i) best = sh->wred[i] > best ? sh->wred[i] : best;
+  mkey = __reduce_max_sync(0xffffffffu, (unsigned)sh->wred[lane & (SM_WARPS - 1)]);
   c.wait();
-  const int ph = c.exchange(Sel{best, 0ull});
-  for (int r = 0; r < c.S; ++r) best = sh->xch[ph][r].a > best ? sh->xch[ph][r].a : best;
-  const unsigned mkey = (unsigned)best;
+  const int ph = c.exchange(Sel{mkey, 0ull});
+  mkey = __reduce_max_sync(0xffffffffu, lane < c.S ? (unsigned)sh->xch[ph][lane].a : 0u);
   if (!is_candidate(mkey)) {   // nothing to choose from: an allowed id, as the greedy pick gives
     if (c.rank == 0 && tid == 0) {
       ids[row_i] = (stop_free ? 6 : 2) % lim;
@@ -840,11 +903,6 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     c.sync();                            // no CTA leaves while a peer may still write to it
     return;
   }
-  // ---- settings of the row
-  float T = opt.temperature ? opt.temperature[row_i] : opt.temperature_all;
-  const int top_k = opt.top_k ? opt.top_k[row_i] : opt.top_k_all;
-  const float top_p = opt.top_p ? opt.top_p[row_i] : opt.top_p_all;
-  const float min_p = opt.min_p ? opt.min_p[row_i] : opt.min_p_all;
   const bool greedy = !(T > SM_GREEDY_T) || top_k == 1;
   Weigher w;
   row.has_inf = mkey == kInfKey;
@@ -857,7 +915,6 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   w.cs = (float)(w.c / 128.0 / (double)w.scale);
   w.tab = sh->tab + (lane & 15);
   const double x_max = min_p > 0.f ? -128.0 * log2((double)fminf(min_p, 1.f)) : INFINITY;   // of 128 x
-  float uv = u[(size_t)row_i * u_ld + (u_index ? min(max(u_index[row_i], 0), u_len - 1) : 0)];
   uv = fminf(uv, 0.99999994f);           // the largest number below 1
   u64 cut = 0ull;
   if (greedy) {
@@ -926,26 +983,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   u64 mass = __double2ull_rn(sum);
   mass = warp_sum64(mass);
   count = __reduce_add_sync(0xffffffffu, count);
-  __syncthreads();
-  if (lane == 0) {
-    sh->wred[warp] = mass;
-    sh->wred2[warp] = count;
-  }
-  __syncthreads();
-  u64 all = 0ull, below = 0ull, cnt = 0ull;
-  for (int i = 0; i < SM_WARPS; ++i) {
-    if (i < warp) below += sh->wred[i];
-    all += sh->wred[i];
-    cnt += sh->wred2[i];
-  }
-  const int p2 = c.exchange(Sel{all, cnt});
-  u64 total = 0ull, n_kept = 0ull, all_below = 0ull;
-  for (int r = 0; r < c.S; ++r) {
-    if (r < c.rank) all_below += sh->xch[p2][r].a;
-    total += sh->xch[p2][r].a;
-    n_kept += sh->xch[p2][r].b;
-  }
-  below += all_below;
+  const Sums in = block_sums(sh, mass, count), over = c.sums(c.exchange(Sel{in.a, in.b}));
+  const u64 total = over.a, n_kept = over.b, all_below = over.a_below, all = in.a, below = all_below + in.a_below;
   const u64 target = part_of(uv, total);
   // The piece that holds the pick has at most SM_WARPS tiles of 32 vectors: each warp of its CTA weighs one again.
   if (below <= target && target < below + mass) {   // one warp of the cluster
@@ -963,6 +1002,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     const int v0 = min(end, c.rank * part + owner * per), v1 = min(end, v0 + per);
     row.v0 = min(v1, v0 + warp * 32);
     row.v1 = min(v1, row.v0 + 32);
+    row.kept = false;
     u64 wt[8], own = 0ull;
     int id0 = 0;
 #pragma unroll
@@ -983,10 +1023,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
       const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += t;
     }
-    if (lane == 31) sh->wred[warp] = inc;
-    __syncthreads();
-    u64 run = piece + inc - own;
-    for (int i = 0; i < warp; ++i) run += sh->wred[i];
+    u64 run = piece + inc - own + block_sums(sh, __shfl_sync(0xffffffffu, inc, 31), 0ull).a_below;
     if (run <= target && target < run + own) {       // one lane
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
