@@ -57,13 +57,27 @@ def test_settings(rows, V, dtype, settings):
     (200, 2048, torch.bfloat16, 2001, True),
     (2, 40001, torch.float32, 40000, False),
     (1, 262144, torch.bfloat16, None, False),    # the widest vocabulary: 32768 logits a CTA
-    (150, 36000, torch.float32, None, False),    # split only because a CTA's part would not fit
+    (150, 36000, torch.float32, None, False),
 ])
 @pytest.mark.parametrize("settings", [dict(temperature=0.9, top_p=0.92), dict(top_k=7, min_p=0.01), dict()])
 def test_sizes(rows, V, dtype, limit, stop_free, settings):
     x, u = _logits(rows, V, dtype, 2)
     _check(x, u, *sampling.sample(x, u, active_limit=limit, stop_free=stop_free, **settings), settings, limit,
            stop_free)
+
+
+@pytest.mark.parametrize("V", [131072, 131080, 262144])
+def test_the_most_that_one_cta_takes(V):
+    """Around the sizes that split a row whatever the batch; equal logits fill one bin with all of a CTA's weights."""
+    x, u = _logits(150, V, torch.bfloat16, 17)
+    x[0] = 0.0
+    x[1] = 0.0
+    x[1, 7] = 1.0
+    for st in (dict(top_p=0.7), dict(top_k=V - 100, top_p=0.999), dict()):
+        for rows in (2, 150):
+            got = sampling.sample(x[:rows], u[:rows], **st)
+            n = min(rows, 3)
+            _check(x[:n], u[:n], *(t[:n] for t in got), st)
 
 
 def test_settings_per_row():

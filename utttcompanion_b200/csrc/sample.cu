@@ -25,16 +25,24 @@
 // integers the half-rate integer pipe was 60 % busy and bound the kernel.
 //
 // Layout.  One cluster of S CTAs per row; each warp owns a contiguous piece of the
-// row and streams it in 16-byte loads, once per step (the row comes from HBM once
-// and stays in L1 / L2 for the others): (1) largest logit; (2) where top-k or top-p
-// ask for it, a histogram over 2048 bins of x, merged over the cluster in
-// distributed shared memory, and (3) the candidates of the bin that holds the cut,
-// ranked against each other; of too many equal logits the last kept one is counted
-// off in id order, and a bin with too many nearly equal ones is split again by the
-// bits of its (key, id) pairs; (4) kept mass per warp; the warp that holds the pick
-// walks its piece again.  Weights below 2^-24 (a billionth of a percent of the mass
-// each) get no bin: what top-p asks for nearly always ends before them, and if it
-// does not, they are one bin that is split by the same steps.
+// row and streams it in 16-byte loads, once per step (the row comes from HBM once;
+// a small piece then stays in shared memory, others come from L2 again):
+// (1) largest logit; (2) where top-k or top-p ask for it, a histogram over 2048 bins
+// of x, merged over the cluster in distributed shared memory; (3) where the
+// candidates down to the cut's bin are few, all of them in one list, from which the
+// row is finished; else those of the bin, ranked against each other (of too many
+// equal logits the last kept one is counted off in id order, and a bin with too many
+// nearly equal ones is split again by the bits of its (key, id) pairs); (4) kept mass
+// per warp; the CTA that holds the pick weighs that warp's piece again.  Weights below
+// 2^-24 (a billionth of a percent of the mass each) get no bin: what top-p asks for
+// nearly always ends before them, and if it does not, they are one bin that is split
+// by the same steps.
+//
+// What bounds it.  Large batches: instructions.  256 rows of 131072 BF16 logits at
+// top-p 0.95 take 224 us, 163 warp instructions per 32 logits over the four walks at
+// 0.75 a cycle and scheduler (FP64 20 %, ALU 42 %, DRAM 4 % busy); without cuts they
+// take 120 us, with top-k 50 and top-p 0.9 67 us.  Small ones: latency.  A row of
+// 32000 takes 16.7 us, 7 cluster barriers among them.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -52,8 +60,8 @@ constexpr int SM_CAP = SM_THREADS;        // candidates ranked against each othe
 constexpr int SM_RING = 4;               // 16-byte vectors on their way per lane
 constexpr int SM_TAIL = SM_BINS;          // the bin of everything beyond SM_RANGE
 constexpr int SM_MAX_CTAS = 8;
-constexpr int SM_MAX_V = 262144;         // 8 CTAs of 32768 keys
-constexpr int SM_MAX_PART = 65536;       // ids per CTA: sums of as many 16-bit limbs stay below 2^32
+constexpr int SM_MAX_V = 262144;
+constexpr int SM_MAX_PART = 131071;      // candidates per CTA: sums of as many limbs of up to 2^15 stay below 2^32
 constexpr float SM_RANGE = 24.f;         // x up to here has bins (64 to the unit) and exact weights
 constexpr int SM_STEPS = 128;            // table entries per octave
 constexpr float SM_GREEDY_T = 1e-5f;     // _sample_next_token's greedy border
@@ -75,7 +83,7 @@ struct SampleShared {
   u64 res_base, res_held, res_cut;
   int res_bin;
   u64 more[SM_MAX_CTAS * SM_WARPS];      // what every warp of the cluster has beyond the bins
-  alignas(16) unsigned hist[3][SM_BINS];  // count, or 16-bit limbs of the mass
+  alignas(16) unsigned hist[3][SM_BINS];  // count, or 15-bit limbs of the mass
   alignas(16) u64 merged[SM_BINS];       // the cluster's histogram
 };
 
@@ -467,7 +475,7 @@ __device__ __forceinline__ void merge_bins(Cluster& c, int mode) {
         h2[r] = p[r]->hist[2][bin];
       }
 #pragma unroll
-      for (int r = 0; r < S; ++r) v += ((u64)h1[r] << 16) + ((u64)h2[r] << 32);
+      for (int r = 0; r < S; ++r) v += ((u64)h1[r] << 15) + ((u64)h2[r] << 30);
     }
 #pragma unroll
     for (int r = 0; r < S; ++r) v += h0[r];
@@ -493,8 +501,8 @@ __device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, 
     val[0] = h0.x, val[1] = h0.y, val[2] = h0.z, val[3] = h0.w;
     if (mode == FIND_MASS) {
       const uint4 h1 = reinterpret_cast<const uint4*>(sh->hist[1])[tid], h2 = reinterpret_cast<const uint4*>(sh->hist[2])[tid];
-      val[0] += ((u64)h1.x << 16) + ((u64)h2.x << 32), val[1] += ((u64)h1.y << 16) + ((u64)h2.y << 32);
-      val[2] += ((u64)h1.z << 16) + ((u64)h2.z << 32), val[3] += ((u64)h1.w << 16) + ((u64)h2.w << 32);
+      val[0] += ((u64)h1.x << 15) + ((u64)h2.x << 30), val[1] += ((u64)h1.y << 15) + ((u64)h2.y << 30);
+      val[2] += ((u64)h1.z << 15) + ((u64)h2.z << 30), val[3] += ((u64)h1.w << 15) + ((u64)h2.w << 30);
     }
   } else {
     if (c.S == 2) merge_bins<2>(c, mode);
@@ -543,7 +551,7 @@ __device__ int locate(Cluster& c, int mode, float top_p, u64 more, u64& target, 
 }
 
 __device__ __forceinline__ void add_mass(SampleShared* sh, int bin, u64 wt) {
-  const unsigned l0 = (unsigned)wt & 0xffffu, l1 = (unsigned)wt >> 16, l2 = (unsigned)(wt >> 32);
+  const unsigned l0 = (unsigned)wt & 0x7fffu, l1 = (unsigned)(wt >> 15) & 0x7fffu, l2 = (unsigned)(wt >> 30);   // <= 2^15
   atomicAdd(&sh->hist[0][bin], l0);
   atomicAdd(&sh->hist[1][bin], l1);
   if (l2) atomicAdd(&sh->hist[2][bin], l2);
@@ -967,7 +975,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     wt = (double)w.tail_weight(y);
     return true;
   };
-  double sum = 0.0;                      // at most 2^7 weights of 2^45: exact
+  double sum = 0.0;                      // at most 2^8 weights of 2^45: exact
   unsigned count = 0u;
   row.each([&](const unsigned (&x)[8], int id) {
 #pragma unroll
@@ -986,7 +994,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   const Sums in = block_sums(sh, mass, count), over = c.sums(c.exchange(Sel{in.a, in.b}));
   const u64 total = over.a, n_kept = over.b, all_below = over.a_below, all = in.a, below = all_below + in.a_below;
   const u64 target = part_of(uv, total);
-  // The piece that holds the pick has at most SM_WARPS tiles of 32 vectors: each warp of its CTA weighs one again.
+  // The CTA that holds the pick weighs that warp's piece again, each warp a tile of 32 vectors at a time.
   if (below <= target && target < below + mass) {   // one warp of the cluster
     if (lane == 0) {
       sh->res_bin = warp;
@@ -997,12 +1005,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   }
   __syncthreads();
   const int owner = sh->res_bin;
-  if (owner >= 0) {                      // the same for the whole CTA
-    const u64 piece = sh->res_base;
-    const int v0 = min(end, c.rank * part + owner * per), v1 = min(end, v0 + per);
-    row.v0 = min(v1, v0 + warp * 32);
-    row.v1 = min(v1, row.v0 + 32);
-    row.kept = false;
+  const int p0 = min(end, c.rank * part + max(owner, 0) * per), p1 = owner >= 0 ? min(end, p0 + per) : p0;
+  u64 piece = sh->res_base;              // mass before the tiles
+  row.kept = false;
+  for (int v0 = p0; v0 < p1 && piece <= target; v0 += SM_THREADS) {   // the same for the whole CTA
+    row.v0 = min(p1, v0 + warp * 32);
+    row.v1 = min(p1, row.v0 + 32);
     u64 wt[8], own = 0ull;
     int id0 = 0;
 #pragma unroll
@@ -1023,7 +1031,9 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
       const u64 t = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += t;
     }
-    u64 run = piece + inc - own + block_sums(sh, __shfl_sync(0xffffffffu, inc, 31), 0ull).a_below;
+    const Sums tiles = block_sums(sh, __shfl_sync(0xffffffffu, inc, 31), 0ull);
+    u64 run = piece + inc - own + tiles.a_below;
+    piece += tiles.a;
     if (run <= target && target < run + own) {       // one lane
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -1053,12 +1063,14 @@ extern "C" int uttt_sample(int rows, int V, const void* logits, int logits_f32, 
   cudaStream_t st = (cudaStream_t)stream;
   ProfScope ps(UTTT_PROF_ARGMAX, st);
   const int lim = active_limit < V ? active_limit : V;
-  // a row is split over a cluster while the rows alone leave SMs idle (two CTAs fit an SM; at least 2048 logits per
-  // CTA), and where a CTA's part would be too large for the histogram's limbs
+  // A row is split over a cluster of S while the rows alone leave SMs idle (two CTAs fit an SM; at least 2048 logits per
+  // CTA), and where a CTA's part would be too large for the histogram's limbs (ids 0, 1 and 3 are no candidates).
+  // At top-p 0.95, S = 1 / 2 / 4 / 8, launches one by one: one row of 32000 48 / 41 / 35 / 32 us, 64 rows 56 / 45 / 43 /
+  // 63, 333 rows of 8003 53 / 74 / 123 / 251, 256 rows of 131072 225 / 243 / 284 / 379.
   const int nvec = (lim + 7) / 8;
   int S = 1;
-  while (S < SM_MAX_CTAS &&
-         ((lim + S - 1) / S > SM_MAX_PART || ((long long)rows * 2 * S <= 2 * num_sms() && lim / (2 * S) >= 2048)))
+  while (S < SM_MAX_CTAS && ((S == 1 ? lim - 3 : (nvec + S - 1) / S * 8) > SM_MAX_PART ||
+                             ((long long)rows * 2 * S <= 2 * num_sms() && lim / (2 * S) >= 2048)))
     S *= 2;
   const int part = (nvec + S - 1) / S;
   auto kernel = logits_f32 ? sample_kernel<true> : sample_kernel<false>;
