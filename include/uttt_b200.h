@@ -376,7 +376,8 @@ int uttt_kv_ring_fill(int B, int L, int end_pos, int n_kv, int hd, int W, const 
  * reaches it, whatever its bits (a NaN or an infinity that it does see makes its
  * output NaN or infinite).  hd in {32, 64, 128}, n_heads / n_kv <= 8, N <= 64;
  * rings, k_tree and v_tree 16-byte aligned (UTTT_ERR_UNSUPPORTED otherwise), qkv,
- * out and the tables at any address and row stride.  No workspace.
+ * out and the tables at any address and row stride.  No workspace; a device wait
+ * that expires makes its rows of out NaN.
  */
 int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos, const void* qkv,
                    int qkv_ld, const int* parents, const int* n_nodes, const int* pos, const int* slot,

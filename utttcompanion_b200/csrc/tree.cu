@@ -26,6 +26,13 @@
 // The probabilities enter the second product as two BF16 parts, P_hi = bf16(P) and
 // P_lo = bf16(P - P_hi) (about 16 significant bits, as the prefill kernel does);
 // scores, statistics and sums are FP32.
+//
+// What bounds it (1.58B heads unless said).  64 rows of 1 to 16 nodes over window
+// 512: 28.7 us; of a full wave's 22 us 3 are the nodes' paths and RoPE and 2 the
+// output, between them the rings stream at the HBM rate (77 MB).  8 rows of 31 nodes
+// over window 8192, one KV head: 32.5 us, 16 tiles a CTA at 1350 cycles (the softmax
+// between two products on the tensor cores; its powers alone are 512) and 6000 cycles
+// for the cluster's join.  One row of 5 nodes: 13 us, the host's side of the call.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -340,7 +347,8 @@ constexpr int tree_smem() {
 }
 
 // CTAs that share a row's keys.  A CTA takes about as long as `head` tiles before and after its own tiles (node
-// paths, RoPE, output), a cluster `join` more; S minimises the waves of CTAs times that.
+// paths, RoPE, output), a cluster `join` more; S minimises the waves of CTAs times that.  (Clusters of 16, for long
+// windows: 44.5 us against 32.5 for 8 rows of 31 nodes and window 8192; the GPU does not hold 16 of them at a time.)
 inline int tree_split(long long ctas, int tiles, int per_sm, int head, int join) {
   const long long slots = (long long)num_sms() * per_sm;
   int best = 1;
@@ -821,6 +829,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   __shared__ float ml_s[128][2];         // of the rows that the cluster sends
   __shared__ u64 bad_mask[8];            // ring tiles with non-finite values: their keys ...
   __shared__ int bad_tile[8], n_bad;     // ... and numbers
+  __shared__ int expired;                // whether a wait has given up: the rows become NaN then
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sQ = base, *sK = base + LY::K0, *sV = base + LY::V0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -858,7 +867,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
     }
     mbar_init(&ready, 128);
     fence_mbarrier_init();
-    n_bad = 0;
+    n_bad = expired = 0;
     bad_tree = 0ull;
     deepest = 0;
   }
@@ -892,6 +901,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         if (ik < cnt && free_slot(k_empty, ik)) load(&tmK, sK, k_full, ik++);
         if (iv < cnt && free_slot(v_empty, iv)) load(&tmV, sV, v_full, iv++);
       }
+      if (ik < cnt || iv < cnt) set_status(&expired, UTTT_ERR_TIMEOUT);
     }
   } else if (warp == 1) {
     if (cnt > 0) {
@@ -904,12 +914,12 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
                      vd = sdesc_sw128(smem_u32(sV), 8192, 1024);
       const uint32_t tS = __shfl_sync(0xffffffffu, tmem, 0);
       const bool leader = elect_one();
-      mbar_wait(&ready, 0, nullptr);
+      mbar_wait(&ready, 0, &expired);
       auto issue_s = [&](int i) {
         const int s = i & 1;
-        if (!(has_tree && i == 0)) mbar_wait(&k_full[s], tma_fills(i) & 1, nullptr);
+        if (!(has_tree && i == 0)) mbar_wait(&k_full[s], tma_fills(i) & 1, &expired);
         // P of sequence i - 2 has left this buffer
-        if (i >= 2) mbar_wait(&v_empty[s], ((i >> 1) - 1) & 1, nullptr);
+        if (i >= 2) mbar_wait(&v_empty[s], ((i >> 1) - 1) & 1, &expired);
         tc_fence_after();
         const uint64_t ks = kd + (uint64_t)(s * (LY::TILE >> 4));
         if (leader) {
@@ -925,8 +935,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       for (int i = 0; i < cnt; ++i) {
         if (i + 1 < cnt) issue_s(i + 1);
         const int s = i & 1;
-        if (!(has_tree && i == 0)) mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
-        mbar_wait(&p_full[s], (i >> 1) & 1, nullptr);
+        if (!(has_tree && i == 0)) mbar_wait(&v_full[s], tma_fills(i) & 1, &expired);
+        mbar_wait(&p_full[s], (i >> 1) & 1, &expired);
         tc_fence_after();
         const uint64_t vs = vd + (uint64_t)(s * (LY::TILE >> 4));
         const uint32_t pa = tS + s * 64;
@@ -999,12 +1009,12 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
                                      j0 <= next - W + max_dep);
       u64 seen = is_tree ? anc : ~0ull;
       // scores i are issued once values i - 2 have been used: after this wait v_full's phase can be told
-      mbar_wait(&s_full[s], (i >> 1) & 1, nullptr);
+      mbar_wait(&s_full[s], (i >> 1) & 1, &expired);
       tc_fence_after();
       if (edge) {
         const u64 valid_keys = bit_range(0, nvalid - j0), some = hidden_places(j0, next, W, max_dep) & valid_keys;
         seen = valid_keys & ~hidden_places(j0, next, W, dep);
-        mbar_wait(&v_full[s], tma_fills(i) & 1, nullptr);
+        mbar_wait(&v_full[s], tma_fills(i) & 1, &expired);
         auto at = [&](int r, int c) {
           return reinterpret_cast<uint4*>(sV + s * LY::TILE + (c >> 3) * 8192 + sw128_offset(r, (c & 7) * 16));
         };
@@ -1039,7 +1049,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       const bool grow = mt > m + TT_GROWTH || m == -INFINITY;
       if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
         // O of this warp's rows holds sequences .. i - 1: their MMAs end first
-        if (i > 0) mbar_wait(&v_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, nullptr);
+        if (i > 0) mbar_wait(&v_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, &expired);
         tc_fence_after();
         const float c = grow && m != -INFINITY ? exp2f(m - mt) : 1.f;
         l *= c;
@@ -1092,9 +1102,10 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
     }
 
     // ---- O -> BF16 rows of out, or partials for the cluster
-    if (active && cnt > 0) mbar_wait(&v_empty[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1, nullptr);
+    if (active && cnt > 0) mbar_wait(&v_empty[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1, &expired);
     tc_fence_after();
     named_bar(1, 128);                   // bad_* is complete, no tile is in use any more
+    if (status_set(&expired)) m = 0.f, l = __int_as_float(0x7fffffff);
     if (S > 1) cg::this_cluster().sync();   // every CTA has read its tiles: rows may be sent over them
     const Joiner jn{reinterpret_cast<float*>(base), ml_s, S, 128 / S, LY::OLD};
     cg::cluster_group cl = cg::this_cluster();
