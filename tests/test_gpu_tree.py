@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from drafting_refs import accept_row, tree_row
-from utttcompanion_b200 import kv_cache, tree
+from utttcompanion_b200 import kv_cache, sampling, tree
 from utttcompanion_b200.model import rope_tables
 
 pytestmark = pytest.mark.gpu
@@ -191,6 +191,66 @@ def test_captured_and_replayed_with_other_rows():
     graph.replay()
     torch.cuda.synchronize()
     _check(c, 12, out, kt, vt)
+
+
+def _wave(seed):
+    """320 CTAs where the GPU holds 296: a full wave and a second launch for the rest of the rows."""
+    return _case(64, 16, 20, 5, 128, 512, [32 + 64 * i for i in range(64)], "random", [1 + i % 16 for i in range(64)],
+                 seed=seed)
+
+
+def test_a_second_launch_is_captured_and_replayed():
+    c, d = _wave(11), _wave(12)
+    want = [[t.clone() for t in _run(x, 20)] for x in (c, d)]
+    got = [torch.zeros_like(t) for t in want[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        _run(c, 20, out=got[0], k_tree=got[1], v_tree=got[2])
+    for x, w in ((c, want[0]), (d, want[1])):
+        for name in c:
+            c[name].copy_(x[name])
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, w))
+
+
+def test_what_follows_waits_for_both_launches():
+    """The next kernel starts early (its grid is launched while the last one runs): it must not read early."""
+    cases = [_wave(13 + i) for i in range(3)]
+    u = torch.zeros(1024, device=DEV)
+    outs = [_run(c, 20)[0].clone() for c in cases]
+    want = [sampling.sample(o, u, temperature=0.0).ids for o in outs]
+    out = torch.zeros_like(outs[0])
+    for i in range(30):
+        out.zero_()
+        _run(cases[i % 3], 20, out=out)
+        ids = sampling.sample(out, u, temperature=0.0).ids
+        assert torch.equal(ids, want[i % 3])
+
+
+def test_two_streams_at_once():
+    a, b = _wave(16), _case(5, 64, 12, 4, 64, 300, [10, 200, 299, 300, 9000], seed=17)
+    g = torch.Generator(device=DEV).manual_seed(18)
+    x = (torch.randn(40, 32000, device=DEV, generator=g) * 3).to(torch.bfloat16)
+    u = torch.rand(40, device=DEV, generator=g)
+
+    def both():
+        return _run(a, 20) + _run(b, 12) + tuple(sampling.sample(x, u, top_p=0.9, temperature=0.8))
+    want = [t.clone() for t in both()]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for s, r in zip(streams, got):
+            with torch.cuda.stream(s):
+                r.append(both())
+    torch.cuda.synchronize()
+    for r in got[0] + got[1]:
+        assert all(torch.equal(p, q) for p, q in zip(r, want))
 
 
 def test_attention_refusals():
