@@ -955,14 +955,19 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
   const float y_hi = fminf(any_cut ? yc * 1.000001f + 1e-5f : INFINITY,
                            any_min ? (float)(x_max / 128.0) * 1.000001f + 1e-5f : INFINITY);
   const float y_lo = any_cut ? fminf(yc * 0.999999f - 1e-5f, 64.f) : 64.f;
-  // whether an element is kept, and its weight (a whole number, as a double)
-  auto weigh = [&](unsigned bits, int id, double& wt) -> bool {
+  // whether an element is above the cut (and perhaps within min-p)
+  auto in_cut = [&](unsigned bits, int id) -> bool {
     const float y = w.rough(bits);
     if (!(y <= y_hi)) return false;
     if (y > y_lo) {
       const unsigned key = order_key(bits);
       if (!is_candidate(key) || pair_of(key, id) < cut) return false;
     }
+    return true;
+  };
+  // whether such an element is kept, and its weight (a whole number, as a double)
+  auto weigh = [&](unsigned bits, double& wt) -> bool {
+    const float y = w.rough(bits);
     if (y <= SM_RANGE) {
       const double d = w.below(bits);
       if (any_min && d * w.c > x_max) return false;
@@ -975,19 +980,54 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     wt = (double)w.tail_weight(y);
     return true;
   };
-  double sum = 0.0;                      // at most 2^8 weights of 2^45: exact
+  double sum = 0.0;                      // at most 2^8 weights of 2^45 (a warp's candidates by 32): exact
   unsigned count = 0u;
-  row.each([&](const unsigned (&x)[8], int id) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      double wt;
-      if (weigh(x[e], id + e, wt)) {
-        sum += wt;
-        ++count;
-      }
+  auto add = [&](unsigned bits) {
+    double wt;
+    if (weigh(bits, wt)) {
+      sum += wt;
+      ++count;
     }
-    return true;
-  });
+  };
+  if (any_cut || any_min) {
+    // What is above the cut goes through a list of the warp's own, so that 32 at a time are weighed whichever lanes
+    // they came from (the histogram's place is free by now).
+    unsigned* const list = &sh->hist[0][0] + warp * (3 * SM_BINS / SM_WARPS);
+    static_assert(3 * SM_BINS / SM_WARPS >= 31 + 8 * 32);
+    int n = 0;
+    row.each([&](const unsigned (&x)[8], int id) {
+      unsigned mask = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mask |= in_cut(x[e], id + e) ? 1u << e : 0u;
+      const int own = __popc(mask);
+      int inc = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += t;
+      }
+      unsigned* to = list + n + inc - own;
+      n += __shfl_sync(0xffffffffu, inc, 31);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (mask >> e & 1u) *to++ = x[e];
+      __syncwarp();
+      while (n >= 32) {
+        n -= 32;
+        add(list[n + lane]);
+      }
+      __syncwarp();
+      return true;
+    });
+    if (lane < n) add(list[lane]);
+  } else {
+    row.each([&](const unsigned (&x)[8], int id) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (in_cut(x[e], id + e)) add(x[e]);
+      return true;
+    });
+  }
   u64 mass = __double2ull_rn(sum);
   mass = warp_sum64(mass);
   count = __reduce_add_sync(0xffffffffu, count);
@@ -1020,7 +1060,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         double v;
-        wt[e] = weigh(x[e], id + e, v) ? mantissa(v + 4503599627370496.0) : 0ull;
+        wt[e] = in_cut(x[e], id + e) && weigh(x[e], v) ? mantissa(v + 4503599627370496.0) : 0ull;
         own += wt[e];
       }
       return true;
