@@ -156,6 +156,13 @@ struct Weigher {
   // x in FP32; NaN or infinite for NaN and -inf.  Scaled, so that m - s does not overflow: by 1/2, and by 2^-100 at
   // temperatures above 10^30, which would flush log2(e) / T to zero
   __device__ __forceinline__ float rough(unsigned bits) const { return fmaf(__uint_as_float(bits), -scale, ms) * cs; }
+  // logits for quick tests: none whose x is at most y is smaller, or at least y larger
+  __device__ __forceinline__ float no_less(float y) const {
+    return __double2float_rd(m - ((double)y * 1.000001 + 1e-5) / ((double)cs * (double)scale));
+  }
+  __device__ __forceinline__ float no_more(float y) const {
+    return __double2float_ru(m - ((double)y * 0.999999 - 1e-5) / ((double)cs * (double)scale));
+  }
   // m - s >= 0, exact but for one rounding to 53 bits
   __device__ __forceinline__ double below(unsigned bits) const { return m - (double)__uint_as_float(bits); }
   // k, the whole number next to 128 x, and the rest r
@@ -671,9 +678,9 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64& 
     // an upper bound of the candidates down to this bin's end: each weighs at least 2^-x there
     const u64 least = MODE == FIND_COUNT ? 1ull : (u64)exp2(45.0 - ((double)bin + 0.8) / 64.0);
     if (base + held <= (u64)SM_CAP * least) {
-      const float y2 = ((float)bin + 0.75f) * (1.f / 64.f) + 1e-5f;
+      const float s2 = w.no_less(((float)bin + 0.75f) * (1.f / 64.f));
       listed = gather(
-          c, row, [&](unsigned bits) { return w.rough(bits) <= y2; },
+          c, row, [&](unsigned bits) { return __uint_as_float(bits) >= s2; },
           [&](unsigned bits, int) {
             double r;
             return w.rough(bits) <= SM_RANGE && w.bin(w.split(w.below(bits), r)) <= bin;
@@ -682,10 +689,10 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64& 
     }
   }
   target -= base;
-  // FP32's x is off by less than 2^-18 up to SM_RANGE: most elements are told apart from the bin by it
-  // (bin b has the x that round to 2 b / 128 or (2 b + 1) / 128)
-  const float y0 = bin == SM_TAIL ? SM_RANGE : ((float)bin - 0.25f) * (1.f / 64.f) - 1e-5f;
-  const float y1 = bin == SM_TAIL ? INFINITY : ((float)bin + 0.75f) * (1.f / 64.f) + 1e-5f;
+  // bin b has the x that round to 2 b / 128 or (2 b + 1) / 128; beyond SM_RANGE are those that FP32 says so of, off by
+  // less than 2^-18
+  const float s0 = bin == SM_TAIL ? -INFINITY : w.no_less(((float)bin + 0.75f) * (1.f / 64.f));
+  const float s1 = w.no_more(bin == SM_TAIL ? SM_RANGE : ((float)bin - 0.25f) * (1.f / 64.f));
   u64 mn = ~0ull, mx = 0ull, lo = 0ull, hi = ~0ull;
   auto take = [&](unsigned bits, int id, u64& pr) {   // a candidate within the cut and [lo, hi]
     const unsigned key = order_key(bits);
@@ -699,10 +706,7 @@ __device__ u64 find_cut(Cluster& c, const Row<F32>& row, const Weigher& w, u64& 
   };
   unsigned n = gather(
       c, row,
-      [&](unsigned bits) {
-        const float y = w.rough(bits);
-        return y >= y0 && y <= y1;
-      },
+      [&](unsigned bits) { return __uint_as_float(bits) >= s0 && __uint_as_float(bits) <= s1; },
       [&](unsigned bits, int id) {
         const bool tail = !(w.rough(bits) <= SM_RANGE);
         u64 pr;
