@@ -952,22 +952,18 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     }
   }
   // ---- kept mass per warp
-  // FP32's x (good to 2^-22 of itself) tells all but the elements next to the cut apart from it; the keys decide there
-  // and beyond 64, where an overflow could stand for anything
+  // The cut is told by the logits themselves, and among equal ones by id; min-p by x, after a quick test.  (A compare
+  // takes subnormal numbers for zero: they come out equal at most, and the keys decide.)
   const bool any_cut = cut != 0ull, any_min = x_max != INFINITY;
-  const float yc = w.rough(__float_as_uint(key_value((unsigned)(cut >> 32))));
-  const float y_hi = fminf(any_cut ? yc * 1.000001f + 1e-5f : INFINITY,
-                           any_min ? (float)(x_max / 128.0) * 1.000001f + 1e-5f : INFINITY);
-  const float y_lo = any_cut ? fminf(yc * 0.999999f - 1e-5f, 64.f) : 64.f;
+  const float s_cut = any_cut ? key_value((unsigned)(cut >> 32)) : -INFINITY;
+  const float s_low = any_min ? max_exact(s_cut, w.no_less((float)(x_max / 128.0)), -INFINITY) : s_cut;
   // whether an element is above the cut (and perhaps within min-p)
   auto in_cut = [&](unsigned bits, int id) -> bool {
-    const float y = w.rough(bits);
-    if (!(y <= y_hi)) return false;
-    if (y > y_lo) {
-      const unsigned key = order_key(bits);
-      if (!is_candidate(key) || pair_of(key, id) < cut) return false;
-    }
-    return true;
+    const float s = __uint_as_float(bits);
+    if (s > s_low) return true;
+    if (s != s_low) return false;
+    const unsigned key = order_key(bits);
+    return is_candidate(key) && pair_of(key, id) >= cut;
   };
   // whether such an element is kept, and its weight (a whole number, as a double)
   auto weigh = [&](unsigned bits, double& wt) -> bool {
