@@ -39,9 +39,10 @@
 // by the same steps.
 //
 // What bounds it.  Large batches: instructions.  256 rows of 131072 BF16 logits at
-// top-p 0.95 take 224 us, 163 warp instructions per 32 logits over the four walks at
-// 0.75 a cycle and scheduler (FP64 20 %, ALU 42 %, DRAM 4 % busy); without cuts they
-// take 120 us, with top-k 50 and top-p 0.9 67 us.  Small ones: latency.  A row of
+// top-p 0.95 take 196 us, 140 warp instructions per 32 logits over the four walks at
+// 0.73 a cycle and scheduler (FP64 14 %, ALU 44 %, DRAM 4 % busy): 8 % of the time for
+// the largest logit, 42 % for the histogram, 13 % for the gather, 31 % for the kept
+// mass.  Without cuts they take 100 us.  Small ones: latency.  A row of
 // 32000 takes 16.7 us, 7 cluster barriers among them.
 #include <cooperative_groups.h>
 
@@ -1105,8 +1106,8 @@ extern "C" int uttt_sample(int rows, int V, const void* logits, int logits_f32, 
   const int lim = active_limit < V ? active_limit : V;
   // A row is split over a cluster of S while the rows alone leave SMs idle (two CTAs fit an SM; at least 2048 logits per
   // CTA), and where a CTA's part would be too large for the histogram's limbs (ids 0, 1 and 3 are no candidates).
-  // At top-p 0.95, S = 1 / 2 / 4 / 8, launches one by one: one row of 32000 48 / 41 / 35 / 32 us, 64 rows 56 / 45 / 43 /
-  // 63, 333 rows of 8003 53 / 74 / 123 / 251, 256 rows of 131072 225 / 243 / 284 / 379.
+  // At top-p 0.95, S = 1 / 2 / 4 / 8, launches one by one: one row of 32000 46 / 40 / 34 / 32 us, 64 rows 53 / 42 / 42 /
+  // 63, 333 rows of 8003 53 / 73 / 124 / 250, 256 rows of 131072 199 / 222 / 266 / 362.
   const int nvec = (lim + 7) / 8;
   int S = 1;
   while (S < SM_MAX_CTAS && ((S == 1 ? lim - 3 : (nvec + S - 1) / S * 8) > SM_MAX_PART ||
