@@ -839,7 +839,6 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   // A launch that joins the one before it starts as soon as that one's CTAs have: they waited for what came before
   // both.  It ends after that one instead, so that what comes next waits for both.
   if (!a.joins) pdl_wait();
-  pdl_trigger();
   const int ti = tid - 64;               // warps 2-5: 0 .. 127
   const int par_i = ti >= 0 && ti < N ? a.parents[(size_t)b * N + ti] : -1;
   const int n = a.n_nodes ? min(a.n_nodes[b], N) : N;
@@ -876,6 +875,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Not before this CTA has its TMEM: a matrix product that starts early takes its own and keeps it until this grid ends.
+  pdl_trigger();
   const uint32_t tmem = tmem_slot, tO = tmem + 128;   // S / P: two buffers of 64 columns, O: HD columns
 
   if (warp == 0) {
