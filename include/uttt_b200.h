@@ -293,8 +293,7 @@ int uttt_split_exchange_finish(int rows, int d, const float* z_partial, const vo
  * residual projection can emit the next block's normalised input
  * (uTTTBlock.forward, :1544-1554).  Segments of a row run in order.
  * Requires K % 64 == 0.  out may alias a RESID segment's aux (in place).
- * The workspace must be zero on entry (a fresh uttt_linear_workspace buffer
- * is); every call leaves it zero again.
+ * Equal calls give equal bits: split-K partial sums are added in K order.
  */
 #define UTTT_SEG_STORE 0
 #define UTTT_SEG_RESID 1

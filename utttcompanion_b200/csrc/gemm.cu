@@ -7,9 +7,11 @@
 // weights as the 128-row M side and the tokens as N (16..256): decode batches
 // have few tokens, prefill many.  A CTA owns 128 output features x one token
 // tile x one K range; with several K ranges (split-K, used when the output is
-// too narrow to fill the GPU) the partials are red.add-ed into Y32.  The
-// row-wise finishing kernel then applies the reference's epilogue of each
-// projection (residual add, RMSNorm, sigmoid gates) and writes BF16.
+// too narrow to fill the GPU) each writes its partial sums into a Y32 of its own.
+// The row-wise finishing kernel then adds those up in the order of the ranges (so a
+// call repeats itself bit for bit; added with atomics, a BF16 rounding turned now and
+// then), applies the reference's epilogue of each projection (residual add, RMSNorm,
+// sigmoid gates) and writes BF16.
 #include <string.h>
 
 #include <cooperative_groups.h>
@@ -28,8 +30,7 @@ constexpr int G_STAGES = 4;
 struct GemmParams {
   int M, N, K, TN;
   int kb_per_split;
-  int atomic;  // red.add (split-K) instead of stores
-  float* y;    // (M, N) FP32
+  float* y;    // (K ranges, M, N) FP32
   int* status;
 };
 
@@ -109,6 +110,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
     tc_fence_after();
     const int q = warp & 3;
     const int n = n0 + q * 32 + lane;
+    float* y = p.y + (size_t)blockIdx.z * p.M * p.N;
     for (int c0 = 0; c0 < p.TN; c0 += 16) {
       float v[16];
       tmem_ld16(tmem_addr(tmem, q * 32, c0), v);
@@ -117,13 +119,7 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int m = m0 + c0 + i;
-          if (m < p.M) {
-            float* dst = p.y + (size_t)m * p.N + n;
-            if (p.atomic)
-              red_add_f32(dst, v[i]);
-            else
-              *dst = v[i];
-          }
+          if (m < p.M) y[(size_t)m * p.N + n] = v[i];
         }
       }
     }
@@ -163,6 +159,20 @@ struct SegPack {
   UtttSegment s[6];
 };
 
+// The sums of columns i, i + stride, ... (below len) of a row over the K ranges, whose rows lie `plane` apart.
+__device__ __forceinline__ void row_sums(float (&v)[F_UNROLL], const float* ys, int i, int stride, int len, int ranges,
+                                         size_t plane) {
+#pragma unroll
+  for (int u = 0; u < F_UNROLL; ++u) v[u] = i + u * stride < len ? ys[i + u * stride] : 0.f;
+#pragma unroll 4
+  for (int k = 1; k < ranges; ++k) {
+    const float* yk = ys + k * plane;
+#pragma unroll
+    for (int u = 0; u < F_UNROLL; ++u)
+      if (i + u * stride < len) v[u] += yk[i + u * stride];
+  }
+}
+
 __device__ __forceinline__ float seg_value(const UtttSegment& sg, float v, int r, int i, float rinv) {
   switch (sg.op) {
     case UTTT_SEG_RESID:
@@ -201,7 +211,8 @@ __device__ __forceinline__ void row_sync(int CF) {
     cg::this_cluster().sync();
 }
 
-__global__ void __launch_bounds__(F_THREADS) finish_kernel(float* __restrict__ y, int N, int nseg,
+__global__ void __launch_bounds__(F_THREADS) finish_kernel(const float* __restrict__ y, int N, int ranges,
+                                                           size_t plane, int nseg,
                                                            const __grid_constant__ SegPack sp, float eps) {
   __shared__ float red[F_THREADS / 32];
   __shared__ float cred[6];
@@ -209,7 +220,7 @@ __global__ void __launch_bounds__(F_THREADS) finish_kernel(float* __restrict__ y
   const int first = blockIdx.y * F_THREADS + tid, stride = CF * F_THREADS;   // this CTA's stripe of the row
   pdl_wait();
   pdl_trigger();
-  float* yrow = y + (size_t)r * N;
+  const float* yrow = y + (size_t)r * N;
   for (int si = 0; si < nseg; ++si) {
     const UtttSegment& sg = sp.s[si];
     __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(sg.out) + (size_t)r * sg.out_ld;
@@ -239,19 +250,20 @@ __global__ void __launch_bounds__(F_THREADS) finish_kernel(float* __restrict__ y
     float rinv = 1.f;
     if (sg.op == UTTT_SEG_RMSNORM) {
       float ss = 0.f;
-      for (int i = first; i < sg.len; i += stride) {
-        const float v = bf16r(ys[i]);
-        ss += v * v;
+      for (int i0 = first; i0 < sg.len; i0 += stride * F_UNROLL) {
+        float v[F_UNROLL];
+        row_sums(v, ys, i0, stride, sg.len, ranges, plane);
+#pragma unroll
+        for (int u = 0; u < F_UNROLL; ++u) {
+          const float x = bf16r(v[u]);
+          ss += x * x;
+        }
       }
       rinv = rsqrtf(cluster_row_sum(fblock_sum(ss, red), cred, si, CF) / (float)sg.len + eps);
     }
     for (int i0 = first; i0 < sg.len; i0 += stride * F_UNROLL) {
       float v[F_UNROLL];
-#pragma unroll
-      for (int u = 0; u < F_UNROLL; ++u) {
-        const int i = i0 + u * stride;
-        v[u] = i < sg.len ? ys[i] : 0.f;
-      }
+      row_sums(v, ys, i0, stride, sg.len, ranges, plane);
 #pragma unroll
       for (int u = 0; u < F_UNROLL; ++u) {
         const int i = i0 + u * stride;
@@ -265,9 +277,22 @@ __global__ void __launch_bounds__(F_THREADS) finish_kernel(float* __restrict__ y
       }
     }
   }
-  // every segment of every CTA has read this row (and its partial sums) before it is cleared
-  row_sync(CF);
-  for (int i = first; i < N; i += stride) yrow[i] = 0.f;   // leave the accumulator zero for the next call
+  if (CF > 1) cg::this_cluster().sync();   // no CTA leaves while another may still read its row statistics
+}
+
+// token tile: the whole batch when it fits one MMA (decode), else 128
+int token_tile(int M) {
+  if (M > 128 && M <= 256) return ((M + 15) / 16) * 16;
+  return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
+}
+// K ranges: split until the grid covers the GPU, with at least one k-block of 64 each.  Without nkb: the most that any
+// K takes.
+int k_ranges(int M, int N, int nkb = 1 << 30) {
+  const int tn = token_tile(M);
+  const long long tiles = (long long)((N + 127) / 128) * ((M + tn - 1) / tn);
+  int splits = 1;
+  while (tiles * splits < 148 && splits * 2 <= nkb) splits *= 2;
+  return splits;
 }
 
 }  // namespace
@@ -277,7 +302,7 @@ using namespace uttt;
 
 extern "C" size_t uttt_linear_workspace(int M, int N) {
   if (M <= 0 || N <= 0) return 0;
-  return 256 + ws_round((size_t)M * N * sizeof(float));
+  return 256 + ws_round((size_t)k_ranges(M, N) * M * N * sizeof(float));
 }
 
 extern "C" int uttt_linear(int M, int N, int K, const void* x, const void* w, int nseg, const UtttSegment* segs,
@@ -295,23 +320,18 @@ extern "C" int uttt_linear(int M, int N, int K, const void* x, const void* w, in
   }
   cudaStream_t st = (cudaStream_t)stream;
   WsCursor ws(workspace, workspace_bytes);
-  float* y = ws.take<float>((size_t)M * N);
-  if (!ws.ok()) return UTTT_ERR_WORKSPACE;
-
-  // token tile: the whole batch when it fits one MMA (decode), else 128
-  int TN = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
-  if (M > 128 && M <= 256) TN = ((M + 15) / 16) * 16;
+  const int TN = token_tile(M);
   const int mtiles = (M + TN - 1) / TN;
   const int ntiles = (N + 127) / 128;
   const int nkb = K / 64;
-  // split K until the grid covers the GPU (at least 1 k-block of 64 per split)
-  int splits = 1;
-  while (ntiles * mtiles * splits < 148 && splits * 2 <= nkb) splits *= 2;
-  const int kbps = (nkb + splits - 1) / splits;
-  splits = (nkb + kbps - 1) / kbps;
+  const int most = k_ranges(M, N, nkb);
+  const int kbps = (nkb + most - 1) / most;
+  const int splits = (nkb + kbps - 1) / kbps;
+  float* y = ws.take<float>((size_t)splits * M * N);
+  if (!ws.ok()) return UTTT_ERR_WORKSPACE;
 
   GemmParams p;
-  p.M = M; p.N = N; p.K = K; p.TN = TN; p.kb_per_split = kbps; p.atomic = splits > 1; p.y = y;
+  p.M = M; p.N = N; p.K = K; p.TN = TN; p.kb_per_split = kbps; p.y = y;
   p.status = ws_status(workspace);
   CUtensorMap tmW, tmX;
   {
@@ -362,7 +382,7 @@ extern "C" int uttt_linear(int M, int N, int K, const void* x, const void* w, in
   cfg.numAttrs = 2;
   {
     ProfScope ps(UTTT_PROF_FINISH, st);
-    if (cudaLaunchKernelEx(&cfg, finish_kernel, y, N, nseg, sp, eps) != cudaSuccess) return launch_status();
+    if (cudaLaunchKernelEx(&cfg, finish_kernel, (const float*)y, N, splits, (size_t)M * N, nseg, sp, eps) != cudaSuccess) return launch_status();
   }
   return launch_status();
 }
