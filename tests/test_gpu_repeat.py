@@ -1,7 +1,8 @@
 """GPU: equal calls give equal bits, whatever order their CTAs finish in.
 
-Sums that several CTAs add to are taken in a fixed order (split-K projections).  A repeated call therefore has nothing to
-differ by, so the outputs are compared bit for bit; a second stream keeps the CTAs from arriving in the same order every time.
+Sums that several CTAs add to are taken in a fixed order (split-K projections) or in 64 bits, where FP32 numbers no more
+than 2^23 apart add up exactly (the hidden tiles of a readout).  A repeated call therefore has nothing to differ by,
+so the outputs are compared bit for bit; a second stream keeps the CTAs from arriving in the same order every time.
 """
 
 import pytest
@@ -9,6 +10,9 @@ import torch
 
 from utttcompanion_b200 import _lib
 from utttcompanion_b200 import fastweight as fw
+from utttcompanion_b200.model import UtttB200
+from utttcompanion_b200.readout import fast_readout
+from utttcompanion_b200.workloads import ModelConfig, reference_init_state_dict
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -87,3 +91,59 @@ def test_linear_epilogues_over_several_k_ranges(op, M, N, K):
         bound = (off + (mag.amax(1, keepdim=True) / y.square().mean(1, keepdim=True).sqrt() + 2.0 ** -7) + 2.0 ** -7) \
             * big * 1.02
     assert bool(((a - b).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("B,T,d,h", [(1, 1, 256, 384), (3, 1, 2560, 6912), (1, 1, 768, 2048), (70, 1, 256, 640)])
+def test_decode_readout_repeats_itself(B, T, d, h):
+    _readouts(B, T, d, h)
+
+
+@pytest.mark.parametrize("B,T,d,h", [(1, 33, 256, 384), (1, 12, 2560, 6912), (2, 70, 768, 2048), (5, 64, 256, 640)])
+def test_tiled_readout_repeats_itself(B, T, d, h):
+    _readouts(B, T, d, h)
+
+
+def _readouts(B, T, d, h):
+    g = torch.Generator(device=DEV).manual_seed(B + T + h)
+    x = torch.randn(B, T, d, device=DEV, generator=g).to(torch.bfloat16)
+    packed = (torch.randn(B, d, 2 * h, device=DEV, generator=g) * d ** -0.5).to(torch.bfloat16)
+    down = (torch.randn(B, h, d, device=DEV, generator=g) * h ** -0.5).to(torch.bfloat16)
+    lw, lb = torch.rand(d, device=DEV, generator=g) + 0.5, torch.randn(d, device=DEV, generator=g)
+    got = _repeat(lambda: fast_readout(x, packed, None, down, lw, lb, out_dtype=torch.float32, packed=True))
+    assert all(torch.equal(got[0], y) for y in got[1:])
+
+
+def _tiny(personas):
+    cfg = ModelConfig(vocab_size=512, d_model=256, n_layers=2, n_heads=4, n_kv_heads=2, d_ff_fast=384,
+                      sliding_window_size=24, chunk_size=64, max_seq_len=512)
+    sd = reference_init_state_dict(cfg, seed=3)
+    sd = {k: (v * 6.0 if k in ("tok_embeddings.weight", "lm_head.weight") else v) for k, v in sd.items()}
+    return UtttB200(sd, cfg, max_personas=personas)
+
+
+def test_sampled_replies_repeat_themselves():
+    """Prefill, packed decode steps and picks: one turned rounding in any of them would change some reply sooner or
+    later (at temperature 1.2 the picks' borders lie close)."""
+    eng = _tiny(6)
+    st = eng.init_fast_state(1)
+    for n in (33, 200):
+        prompt = torch.randint(6, 512, (n,), generator=torch.Generator().manual_seed(n))
+        first = eng.generate_replies(prompt, st, 40, 5, temperature=1.2, top_p=None, seed=7)
+        for _ in range(12):
+            assert eng.generate_replies(prompt, st, 40, 5, temperature=1.2, top_p=None, seed=7) == first
+
+
+def test_logits_repeat_themselves():
+    eng = _tiny(6)
+    st = eng.init_fast_state(1)
+    packed, down = eng.read_copies(st.w_up, st.w_gate, st.w_down)
+    prompt = torch.randint(6, 512, (90,), generator=torch.Generator().manual_seed(4))
+    ids, pos = (torch.tensor(v, dtype=torch.int32, device=DEV) for v in ([7, 8, 9], [90, 90, 90]))
+    slots, zero = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    want = None
+    for _ in range(25):
+        lg = eng.prefill(prompt, 0, packed, down, 0)
+        eng.fork_kv([0, 0], [1, 2], [90, 90])
+        got = [lg, eng.decode_step(ids, pos, slots, packed, down, zero), eng.rings[:, :, :3].clone()]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -77,6 +77,7 @@ struct ChunkParams {
   int tok0_next, Cc_next;  // the fused forward's chunk (bwd kernel with kFuse)
   int hp;             // hidden padded to 128
   int z_rows;         // rows of zacc per state (0: 64, the chunk tile)
+  double* zacc64;     // fwd readout: where z is summed instead of zacc (null: zacc)
   int tiles;          // fwd readout over all token tiles in one launch: grid (T/64, h/128, B)
   float beta, clip, eps, inv_scale;
   int* status;
@@ -453,9 +454,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk_fwd_kernel(const __grid_con
         tc_fence_before();
         mbar_arrive(&zfree[zb]);
       }
-      float* za = p.zacc + zrow0 * p.d + (mt0 + pm) * 128 + row;
-      for (int i = 0; i < 32; ++i)
-        if (c0 + i < Cc) red_add_f32(za + (size_t)(c0 + i) * p.d, z[i]);
+      const size_t z0 = zrow0 * p.d + (mt0 + pm) * 128 + row;
+      if (p.zacc64) {
+        double* za = p.zacc64 + z0;
+        for (int i = 0; i < 32; ++i)
+          if (c0 + i < Cc) red_add_f64(za + (size_t)(c0 + i) * p.d, (double)z[i]);
+      } else {
+        float* za = p.zacc + z0;
+        for (int i = 0; i < 32; ++i)
+          if (c0 + i < Cc) red_add_f32(za + (size_t)(c0 + i) * p.d, z[i]);
+      }
     };
     if constexpr (kAsync) {
       for (int mt = 0; mt < nmt; ++mt) {
@@ -719,9 +727,9 @@ LnKernel chunk_ln_for(int d) {
 
 // ============================================================================
 // readout epilogue: out = x + LN(z) * gamma + beta  (swiglu_fast_forward's
-// last line, model/uttt_layer.py:243-247).  Consumes and re-zeroes z.
+// last line, model/uttt_layer.py:243-247).
 // ============================================================================
-__global__ void __launch_bounds__(LN_THREADS) readout_ln_kernel(const float* __restrict__ zbase, int zrows,
+__global__ void __launch_bounds__(LN_THREADS) readout_ln_kernel(const double* __restrict__ zbase, int zrows,
                                                                 const __nv_bfloat16* __restrict__ x, int T,
                                                                 int tok0, int Cc, int d, const float* ln_w,
                                                                 const float* ln_b, float eps, void* out,
@@ -729,7 +737,7 @@ __global__ void __launch_bounds__(LN_THREADS) readout_ln_kernel(const float* __r
   __shared__ float red[LN_THREADS / 32];
   const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   if (c >= Cc) return;
-  float* zrow = const_cast<float*>(zbase) + ((size_t)b * zrows + c) * d;
+  const double* zrow = zbase + ((size_t)b * zrows + c) * d;
   const size_t tok = (size_t)b * T + tok0 + c;
   float z[LN_MAXV];
   float sum = 0.f;
@@ -738,8 +746,7 @@ __global__ void __launch_bounds__(LN_THREADS) readout_ln_kernel(const float* __r
     const int i = tid + j * LN_THREADS;
     z[j] = 0.f;
     if (i < d) {
-      z[j] = zrow[i];
-      zrow[i] = 0.f;
+      z[j] = (float)zrow[i];
       sum += z[j];
     }
   }
@@ -1979,7 +1986,7 @@ int chunk_write_impl(int B, int T, int C, int d, int h, int chunk_begin, int n_c
 namespace uttt {
 int launch_readout_decode(int B, int d, int h, const __nv_bfloat16* x, const __nv_bfloat16* wp,
                           const __nv_bfloat16* wd, const int* state_index, const float* ln_w, const float* ln_b,
-                          float eps, float* zacc, unsigned* done, void* out, int out_bf16, cudaStream_t st);
+                          float eps, void* zacc, unsigned* done, void* out, int out_bf16, cudaStream_t st);
 int launch_readout_finish(int B, int d, const float* z, const __nv_bfloat16* x, const float* ln_w, const float* ln_b,
                           float eps, void* out, int out_bf16, int z_bf16, cudaStream_t st);
 }
@@ -2038,9 +2045,16 @@ extern "C" int uttt_readout_finish(int B, int d, const float* z, const void* x, 
                                out_dtype == UTTT_DTYPE_BF16, z_bf16 != 0, st);
 }
 
+namespace {
+// z of a readout, FP64 (and behind it, for T == 1, the rows' completion counters)
+size_t readout_z_bytes(int B, int T, int d) {
+  return (size_t)B * (T > CT / 2 ? (size_t)T : CT / 2) * d * sizeof(double);
+}
+}  // namespace
+
 extern "C" size_t uttt_fast_readout_workspace(int B, int T, int d, int h) {
   if (B <= 0 || T <= 0 || d <= 0 || h <= 0) return 0;
-  size_t bytes = 256 + ws_round((size_t)B * (T > CT ? T : CT) * d * sizeof(float));
+  size_t bytes = 256 + ws_round(readout_z_bytes(B, T, d));
   // one token tile of a few rows: room for the d-split exchange of the tensor-core readout
   if (T > 1 && T <= CT && B <= READOUT_DSPLIT_MAX_B) bytes += dsplit_xch_bytes(B, h) + dsplit_flag_bytes(B, h);
   return bytes;
@@ -2061,7 +2075,7 @@ extern "C" int uttt_fast_readout(int B, int T, int d, int h, const void* x, int 
   UTTT_REQUIRE(workspace_bytes >= uttt_fast_readout_workspace(B, T, d, h), UTTT_ERR_WORKSPACE);
   cudaStream_t st = (cudaStream_t)stream;
   WsCursor ws(workspace, workspace_bytes);
-  float* zacc = ws.take<float>((size_t)B * (T > CT ? T : CT) * d);
+  double* zacc = reinterpret_cast<double*>(ws.take<uint8_t>(readout_z_bytes(B, T, d)));
   if (!ws.ok()) return UTTT_ERR_WORKSPACE;
   const int ob = out_dtype == UTTT_DTYPE_BF16;
   if (T == 1 && w_dtype == UTTT_DTYPE_BF16) {
@@ -2069,19 +2083,19 @@ extern "C" int uttt_fast_readout(int B, int T, int d, int h, const void* x, int 
     // with the LayerNorm + residual in its last CTA per state; z (B, d) and the
     // per-state completion counters (B) sit at the front of the z buffer
     unsigned* done = reinterpret_cast<unsigned*>(zacc + (size_t)B * d);
-    UTTT_TRY(cuda_status(cudaMemsetAsync(zacc, 0, (size_t)B * d * sizeof(float) + (size_t)B * sizeof(unsigned), st)));
+    UTTT_TRY(cuda_status(cudaMemsetAsync(zacc, 0, (size_t)B * d * sizeof(double) + (size_t)B * sizeof(unsigned), st)));
     ProfScope ps(UTTT_PROF_READOUT, st);
     return launch_readout_decode(B, d, h, (const __nv_bfloat16*)x, (const __nv_bfloat16*)w_up,
                                  (const __nv_bfloat16*)w_down, state_index, ln_weight, ln_bias, eps, zacc, done, out,
                                  ob, st);
   }
-  UTTT_TRY(cuda_status(cudaMemsetAsync(zacc, 0, (size_t)B * T * d * sizeof(float), st)));
+  UTTT_TRY(cuda_status(cudaMemsetAsync(zacc, 0, (size_t)B * T * d * sizeof(double), st)));
   static DeviceOnce attr_done;
   UTTT_TRY(run_once_per_device(attr_done, [] { return set_fwd_attributes(); }));
   ChunkParams p;
   memset(&p, 0, sizeof(p));
   p.B = B; p.T = T; p.C = CT; p.d = d; p.h = h; p.hp = (h + 127) / 128 * 128;
-  p.zacc = zacc;
+  p.zacc64 = zacc;
   p.status = ws_status(workspace);
   p.k = (const __nv_bfloat16*)x;
   if (w_dtype == UTTT_DTYPE_BF16) {

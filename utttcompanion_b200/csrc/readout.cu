@@ -11,7 +11,10 @@
 // instruction covers a row of both: lanes 0-15 read u, lanes 16-31 read g; the
 // warps split the slice), h = silu(g) * u, then the partial z = h W_down[tile, :]
 // over its slice of d columns (the warps split the tile's rows), reduced in
-// shared memory and added into z (FP32) with one red.add per column.  With
+// shared memory and added into z with one red.add per column.  z is FP64: a sum of
+// FP32 numbers is exact in it unless they lie further apart than 2^23, so the order in
+// which the CTAs arrive does not show and a call repeats itself (in FP32 the last bit
+// depended on it, and a BF16 rounding of z turned now and then).  With
 // KS > 1 the KS CTAs of a tile form one thread-block cluster: their partial u, g
 // meet in distributed shared memory, summed in rank order by every CTA, so all
 // of them hold the same h.  KS grows when B * tiles would leave SMs idle (one
@@ -64,9 +67,9 @@ template <int MD, int MINB>
 __global__ void __launch_bounds__(GTHREADS, MINB) readout_decode_kernel(
     const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ wp, const __nv_bfloat16* __restrict__ wd,
     const int* __restrict__ state_index, int d, int h, const float* __restrict__ ln_w,
-    const float* __restrict__ ln_b, float eps, float* __restrict__ zacc, unsigned* __restrict__ done, void* out,
+    const float* __restrict__ ln_b, float eps, void* __restrict__ zacc, unsigned* __restrict__ done, void* out,
     int out_bf16) {
-  // done == nullptr: partial mode (a slice of the hidden units): z only, no LayerNorm
+  // done == nullptr: partial mode (a slice of the hidden units): z only, in FP32, no LayerNorm
   __shared__ __align__(16) float xs[MD];
   __shared__ __align__(16) float part[8][ZG];
   __shared__ float ug[2 * GT];
@@ -149,7 +152,8 @@ __global__ void __launch_bounds__(GTHREADS, MINB) readout_decode_kernel(
 
   // ---- partial z: warp w takes the tile's rows 16w..16w+15, lane 8 columns of a 256-column chunk
   const __nv_bfloat16* drow = wd + (size_t)state * h * d + (size_t)j0 * d;
-  float* zrow = zacc + (size_t)b * d;
+  float* zpart = reinterpret_cast<float*>(zacc) + (size_t)b * d;    // partial mode
+  double* zrow = reinterpret_cast<double*>(zacc) + (size_t)b * d;   // otherwise
   for (int c0 = kb; c0 < ke; c0 += ZG) {
     const int ncol = min(ZG, ke - c0);
     float acc[2][8];
@@ -188,7 +192,10 @@ __global__ void __launch_bounds__(GTHREADS, MINB) readout_decode_kernel(
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) s += part[w][t];
-      red_add_f32(zrow + c0 + t, s);
+      if (done == nullptr)
+        red_add_f32(zpart + c0 + t, s);
+      else
+        red_add_f64(zrow + c0 + t, (double)s);
     }
     __syncthreads();
   }
@@ -209,7 +216,7 @@ __global__ void __launch_bounds__(GTHREADS, MINB) readout_decode_kernel(
     const int c = tid + i * GTHREADS;
     zv[i] = 0.f;
     if (c < d) {
-      zv[i] = round_bf16(__ldcg(zrow + c));
+      zv[i] = round_bf16((float)__ldcg(zrow + c));
       sum += zv[i];
     }
   }
@@ -289,11 +296,11 @@ int launch_readout_finish(int B, int d, const float* z, const __nv_bfloat16* x, 
   return launch_status();
 }
 
-// zacc: (B, d) FP32 zero on entry; done: (B) zero counters, or nullptr for a
-// partial readout (z only).
+// zacc: (B, d) FP64, zero on entry; done: (B) zero counters, or nullptr for a
+// partial readout (z only, FP32).
 int launch_readout_decode(int B, int d, int h, const __nv_bfloat16* x, const __nv_bfloat16* wp,
                           const __nv_bfloat16* wd, const int* state_index, const float* ln_w, const float* ln_b,
-                          float eps, float* zacc, unsigned* done, void* out, int out_bf16, cudaStream_t st) {
+                          float eps, void* zacc, unsigned* done, void* out, int out_bf16, cudaStream_t st) {
   if (d % 128 != 0 || d > MAXD || h % 8 != 0) return UTTT_ERR_UNSUPPORTED;
   const int tiles = (h + GT - 1) / GT;
   const bool small = d <= 1024;
