@@ -916,6 +916,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       const uint32_t tS = __shfl_sync(0xffffffffu, tmem, 0);
       const bool leader = elect_one();
       mbar_wait(&ready, 0, &expired);
+      __syncwarp();
       auto issue_s = [&](int i) {
         const int s = i & 1;
         if (!(has_tree && i == 0)) mbar_wait(&k_full[s], tma_fills(i) & 1, &expired);
@@ -1012,6 +1013,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       // scores i are issued once values i - 2 have been used: after this wait v_full's phase can be told
       mbar_wait(&s_full[s], (i >> 1) & 1, &expired);
       tc_fence_after();
+      // (tcgen05's loads and stores need the warp's lanes together: after every part that lanes may leave one by one)
       if (edge) {
         const u64 valid_keys = bit_range(0, nvalid - j0), some = hidden_places(j0, next, W, max_dep) & valid_keys;
         seen = valid_keys & ~hidden_places(j0, next, W, dep);
@@ -1033,6 +1035,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         }
         fence_proxy_async_smem();
       }
+      __syncwarp();
       float sv[64];
 #pragma unroll
       for (int c = 0; c < 64; c += 16)
@@ -1052,6 +1055,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
         // O of this warp's rows holds sequences .. i - 1: their MMAs end first
         if (i > 0) mbar_wait(&v_empty[(i - 1) & 1], ((i - 1) >> 1) & 1, &expired);
         tc_fence_after();
+        __syncwarp();
         const float c = grow && m != -INFINITY ? exp2f(m - mt) : 1.f;
         l *= c;
 #pragma unroll
@@ -1115,6 +1119,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       const bool any_bad = bad_tree != 0ull || n_bad > 0;
       if (S > 1 && valid) jn.send_ml(cl, z, i_row, m, l);
       float4* far = jn.row(cl, z, i_row);
+      __syncwarp();
       __nv_bfloat16* dst = a.out + ((size_t)b * N + node) * a.out_ld + (size_t)(g * rep + row % rep) * HD;
 #pragma unroll 1
       for (int k = 0; k < HD; k += 32) {
@@ -1143,8 +1148,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
               }
             }
           }
-        if (!valid) continue;
-        if (S > 1) {
+        if (!valid) {                    // a row of padding: it only takes part in the warp's loads
+        } else if (S > 1) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4) far[(k + e) / 4] = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
         } else if (a.vec_out) {
@@ -1157,6 +1162,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
 #pragma unroll
           for (int e = 0; e < 32; ++e) dst[k + e] = __float2bfloat16(ov[e] * inv);
         }
+        __syncwarp();                    // the lanes part above; a load from tensor memory needs them together
       }
     }
   }
