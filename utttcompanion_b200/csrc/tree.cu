@@ -110,6 +110,12 @@ __device__ __forceinline__ u64 hidden_places(int j0, int next, int W, int depth)
   return bit_range(next - j0, depth + 1) | bit_range(next - W - j0, depth + 1);
 }
 
+// what other SMs' completed writes hold is seen by the loads and the asynchronous copies that follow
+__device__ __forceinline__ void fence_device() {
+  asm volatile("fence.acq_rel.gpu;" ::: "memory");
+  asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // 8 elements of a row of qkv
@@ -837,8 +843,13 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   const int g = blockIdx.y % a.n_kv, row0 = blockIdx.y / a.n_kv * 128;
   const int N = a.N, rep = a.rep, W = a.W;
   // A launch that joins the one before it starts as soon as that one's CTAs have: they waited for what came before
-  // both.  It ends after that one instead, so that what comes next waits for both.
-  if (!a.joins) pdl_wait();
+  // both, so all of it is complete.  Only a wait of its own would let this grid see it; instead every thread takes a
+  // fence at device scope, which drops what this SM may hold of older values, for its own loads and for its tile
+  // copies, before it reads anything.  The launch ends after the one before it, so that what comes next waits for both.
+  if (a.joins)
+    fence_device();
+  else
+    pdl_wait();
   const int ti = tid - 64;               // warps 2-5: 0 .. 127
   const int par_i = ti >= 0 && ti < N ? a.parents[(size_t)b * N + ti] : -1;
   const int n = a.n_nodes ? min(a.n_nodes[b], N) : N;
