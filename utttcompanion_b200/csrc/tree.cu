@@ -735,9 +735,14 @@ int launch_tree(const TreeArgs& a, int B, cudaStream_t st) {
 // 2^8 lose nothing: P_hi / P_lo and the FP32 sums are relative).  Warp 0 issues the
 // TMA loads, warp 1 the MMAs, warps 2-5 own a row per thread; they also rotate Q
 // and, in one CTA of the cluster, the drafted keys, which are its first tile.
-// Two CTAs of 96 KB and 256 TMEM columns share an SM.
+// Two CTAs share an SM, each with 256 of its 512 TMEM columns.  A third would wait for
+// columns while its cluster's other CTAs hold theirs at a barrier, and two clusters could
+// wait for each other for good, so a CTA never asks for less than a third of an SM's shared
+// memory (97 KB at head dim 128; 64 needs 49 KB and takes 77).
 // ---------------------------------------------------------------------------
 constexpr int TT_THREADS = 192;
+constexpr int TT_SM_SMEM = 228 * 1024;   // shared memory of an SM, of which every CTA takes 1 KB more than it asks for
+constexpr int TT_STATIC_SMEM = 4096;     // no less than the kernel's own shared variables
 constexpr float TT_GROWTH = 8.f;         // log2 of the growth that a rescaling waits for
 
 template <int HD>
@@ -748,7 +753,9 @@ struct TtLayout {
   static constexpr int K0 = Q_BYTES, V0 = Q_BYTES + 2 * TILE;   // two slots each
   static constexpr int OLD = HD + 4;              // row stride of the partial outputs (floats)
   static constexpr int USED = Q_BYTES + 4 * TILE > 128 * OLD * 4 ? Q_BYTES + 4 * TILE : 128 * OLD * 4;
-  static constexpr int SMEM = 1024 + USED;
+  static constexpr int SMEM = 1024 + USED > TT_SM_SMEM / 3 ? 1024 + USED : TT_SM_SMEM / 3;
+  static_assert(3 * (SMEM + 1024) > TT_SM_SMEM, "a third CTA must not fit an SM");
+  static_assert(2 * (SMEM + 1024 + TT_STATIC_SMEM) <= TT_SM_SMEM, "two CTAs must fit an SM");
 };
 
 // D[tmem] (+)= A[tmem] * B[smem]^T (kind::f16): A is 128 lanes of packed BF16 pairs
