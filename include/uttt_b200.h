@@ -377,11 +377,21 @@ int uttt_kv_ring_fill(int B, int L, int end_pos, int n_kv, int hd, int W, const 
  * rings, k_tree and v_tree 16-byte aligned (UTTT_ERR_UNSUPPORTED otherwise), qkv,
  * out and the tables at any address and row stride.  No workspace; a device wait
  * that expires makes its rows of out NaN.
+ *
+ * uttt_attn_tree_status is the same call and says so: a wait that expires puts
+ * UTTT_ERR_TIMEOUT into the device word `status` (may be NULL), which nothing else
+ * changes.  max_polls: how often a CTA looks for a free tile slot before it gives
+ * up (0: the default, far beyond any launch).
  */
 int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos, const void* qkv,
                    int qkv_ld, const int* parents, const int* n_nodes, const int* pos, const int* slot,
                    const void* k_ring, const void* v_ring, const float* rope_cos, const float* rope_sin, void* k_tree,
                    void* v_tree, void* out, int out_ld, void* stream);
+int uttt_attn_tree_status(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos, const void* qkv,
+                          int qkv_ld, const int* parents, const int* n_nodes, const int* pos, const int* slot,
+                          const void* k_ring, const void* v_ring, const float* rope_cos, const float* rope_sin,
+                          void* k_tree, void* v_tree, void* out, int out_ld, int* status, unsigned max_polls,
+                          void* stream);
 /*
  * The accepted path of each row's tree: node 0 (the token that was pending), then
  * from every node on its lowest later child whose token is the pick after that

@@ -75,6 +75,8 @@ SIGNATURES: Dict[str, tuple] = {
     "uttt_kv_ring_fill": (i32, [i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
     "uttt_attn_tree": (i32, [i32, i32, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                              vp, i32, vp]),
+    "uttt_attn_tree_status": (i32, [i32, i32, i32, i32, i32, i32, i32, i32, vp, i32, vp, vp, vp, vp, vp, vp, vp, vp,
+                                    vp, vp, vp, i32, vp, C.c_uint, vp]),
     "uttt_tree_accept": (i32, [i32, i32, vp, vp, vp, vp, vp, vp, vp, vp]),
     "uttt_kv_ring_commit": (i32, [i32, i32, i32, i32, i32, i32, i32, vp, vp, C.c_longlong, vp, vp, C.c_longlong, vp,
                                   vp, vp, vp, vp]),

@@ -97,6 +97,8 @@ struct TreeArgs {
   int vec_in, vec_out;                   // whether rows of qkv (with the tables) and of out start on 16 bytes
   int b0;                                // the first row of the launch
   int joins;                             // whether the launch is the rest of the one before it
+  int* status;                           // receives UTTT_ERR_TIMEOUT if a wait expires (or null)
+  uint32_t max_polls;                    // of a CTA's loads for a free slot
 };
 
 // bits lo .. lo + len - 1, as far as they lie in 0 .. 63
@@ -842,6 +844,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   __shared__ float ml_s[128][2];         // of the rows that the cluster sends
   __shared__ u64 bad_mask[8];            // ring tiles with non-finite values: their keys ...
   __shared__ int bad_tile[8], n_bad;     // ... and numbers
+  __shared__ uint64_t drained;
   __shared__ int expired;                // whether a wait has given up: the rows become NaN then
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sQ = base, *sK = base + LY::K0, *sV = base + LY::V0;
@@ -883,6 +886,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       mbar_init(&p_full[i], act);
     }
     mbar_init(&ready, 128);
+    mbar_init(&drained, 1);
     fence_mbarrier_init();
     n_bad = expired = 0;
     bad_tree = 0ull;
@@ -896,6 +900,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   // Not before this CTA has its TMEM: a matrix product that starts early takes its own and keeps it until this grid ends.
   pdl_trigger();
   const uint32_t tmem = tmem_slot, tO = tmem + 128;   // S / P: two buffers of 64 columns, O: HD columns
+  int ik = 0, iv = 0;                    // key and value tiles that this thread has asked for
+  bool leader = false;                   // whether it issues the MMAs
 
   if (warp == 0) {
     if (lane == 0) {
@@ -915,8 +921,8 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       auto free_slot = [&](uint64_t* empty, int i) {
         return i < 2 || mbar_test(smem_u32(&empty[i & 1]), ((i >> 1) - 1) & 1);
       };
-      int ik = 0, iv = 0;
-      for (uint32_t polls = 0; (ik < cnt || iv < cnt) && polls < kMaxLoadPolls; ++polls) {
+      for (uint32_t polls = 0; (ik < cnt || iv < cnt) && polls < a.max_polls; ++polls) {
+        if ((polls & 1023u) == 1023u && status_set(&expired)) break;
         if (ik < cnt && free_slot(k_empty, ik)) load(&tmK, sK, k_full, ik++);
         if (iv < cnt && free_slot(v_empty, iv)) load(&tmV, sV, v_full, iv++);
       }
@@ -932,7 +938,7 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
       const uint64_t qd = sdesc_sw128(smem_u32(sQ), 16, 1024), kd = sdesc_sw128(smem_u32(sK), 16, 1024),
                      vd = sdesc_sw128(smem_u32(sV), 8192, 1024);
       const uint32_t tS = __shfl_sync(0xffffffffu, tmem, 0);
-      const bool leader = elect_one();
+      leader = elect_one();
       mbar_wait(&ready, 0, &expired);
       __syncwarp();
       auto issue_s = [&](int i) {
@@ -1188,6 +1194,19 @@ __global__ void __launch_bounds__(TT_THREADS, 2) attn_tree_tc_kernel(const __gri
   if (S > 1 && warp < 2) cg::this_cluster().sync();   // the same barrier, for the warps that issued
   tc_fence_before();
   __syncthreads();
+  if (expired != 0) {                    // the same for the whole CTA
+    // After a wait that expired copies and MMAs may still be under way: they end before their memory is given back.
+    for (int i = max(0, ik - 2); i < ik; ++i)
+      if (!(has_tree && i == 0)) mbar_wait_limit(&k_full[i & 1], tma_fills(i) & 1, nullptr, kMaxPolls);
+    for (int i = max(0, iv - 2); i < iv; ++i)
+      if (!(has_tree && i == 0)) mbar_wait_limit(&v_full[i & 1], tma_fills(i) & 1, nullptr, kMaxPolls);
+    if (leader) {
+      mma_commit(&drained);
+      mbar_wait_limit(&drained, 0, nullptr, kMaxPolls);
+    }
+    if (tid == 0) set_status(a.status, UTTT_ERR_TIMEOUT);
+    __syncthreads();
+  }
   if (warp == 1) tmem_dealloc(tmem, 256);
   if (S == 1) {
     if (a.joins) pdl_wait();
@@ -1295,11 +1314,11 @@ __global__ void tree_accept_kernel(int B, int N, const int* __restrict__ tokens,
 
 using namespace uttt;
 
-extern "C" int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos,
-                              const void* qkv, int qkv_ld, const int* parents, const int* n_nodes, const int* pos,
-                              const int* slot, const void* k_ring, const void* v_ring, const float* rope_cos,
-                              const float* rope_sin, void* k_tree, void* v_tree, void* out, int out_ld,
-                              void* stream) {
+extern "C" int uttt_attn_tree_status(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos,
+                                     const void* qkv, int qkv_ld, const int* parents, const int* n_nodes, const int* pos,
+                                     const int* slot, const void* k_ring, const void* v_ring, const float* rope_cos,
+                                     const float* rope_sin, void* k_tree, void* v_tree, void* out, int out_ld,
+                                     int* status, unsigned max_polls, void* stream) {
   UTTT_REQUIRE(B > 0 && N > 0 && n_heads > 0 && n_kv > 0 && hd > 0 && W > 0 && n_slots > 0 && n_pos > 0,
                UTTT_ERR_INVALID);
   UTTT_REQUIRE(qkv && parents && pos && slot && k_ring && v_ring && rope_cos && rope_sin && k_tree && v_tree && out,
@@ -1337,6 +1356,8 @@ extern "C" int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W
   a.vec_in = at16(qkv) && qkv_ld % 8 == 0 && at16(rope_cos) && at16(rope_sin);
   a.vec_out = at16(out) && out_ld % 8 == 0;
   a.b0 = a.joins = 0;
+  a.status = status;
+  a.max_polls = max_polls ? max_polls : kMaxLoadPolls;
   if (hd == 128) return launch_tree_tc<128>(a, B, st);
   if (hd == 64) return launch_tree_tc<64>(a, B, st);
   const int rows = N * a.rep;
@@ -1344,6 +1365,15 @@ extern "C" int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W
   if (rows <= 32) return launch_tree<2>(a, B, st);
   if (rows <= 64) return launch_tree<4>(a, B, st);
   return launch_tree<8>(a, B, st);
+}
+
+extern "C" int uttt_attn_tree(int B, int N, int n_heads, int n_kv, int hd, int W, int n_slots, int n_pos,
+                              const void* qkv, int qkv_ld, const int* parents, const int* n_nodes, const int* pos,
+                              const int* slot, const void* k_ring, const void* v_ring, const float* rope_cos,
+                              const float* rope_sin, void* k_tree, void* v_tree, void* out, int out_ld,
+                              void* stream) {
+  return uttt_attn_tree_status(B, N, n_heads, n_kv, hd, W, n_slots, n_pos, qkv, qkv_ld, parents, n_nodes, pos, slot,
+                               k_ring, v_ring, rope_cos, rope_sin, k_tree, v_tree, out, out_ld, nullptr, 0, stream);
 }
 
 extern "C" int uttt_tree_accept(int B, int N, const int* tokens, const int* parents, const int* n_nodes,

@@ -167,6 +167,7 @@ class UtttB200:
         self.rings = torch.zeros(2, cfg.n_layers, max_personas, cfg.n_kv_heads, cfg.sliding_window_size, hd,
                                  dtype=torch.bfloat16, device=dev)
         self.k_ring, self.v_ring = (list(r.unbind(0)) for r in self.rings)
+        self.tree_status = torch.zeros(1, dtype=torch.int32, device=dev)   # nonzero: a wait in a tree step expired
 
     # ------------------------------------------------------------------ launch helpers
     def _st(self) -> int:
@@ -508,7 +509,8 @@ class UtttB200:
         for i, lay in enumerate(self.layers):
             self._linear(x, lay.wqkv, [_seg(0, self.qkv_dim, _lib.SEG_STORE, qkv, self.qkv_dim)])
             tree.tree_attention(qkv, parents, pos, slots, self.k_ring[i], self.v_ring[i], self.rope_cos,
-                                self.rope_sin, nh, n_nodes=n_nodes, out=att, k_tree=kv[0, i], v_tree=kv[1, i])
+                                self.rope_sin, nh, n_nodes=n_nodes, out=att, k_tree=kv[0, i], v_tree=kv[1, i],
+                                status=self.tree_status)
             x2 = self._resid_linear(h, att, lay.wo, lay.uttt_norm)
             q = self._q_proj(lay, x2)
             r = self._readout(q.reshape(B, N, d), read_packed, read_down, sidx)
@@ -520,10 +522,19 @@ class UtttB200:
                     ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Accept each row's path (``tree.tree_accept`` of int32 (B, N) device tensors) and put its keys and values
         into the rings; returns (path, n_path, next pending token).  The row's ring then holds ``pos + n_path``
-        positions."""
+        positions.  After a tree step in which a device wait expired nothing is accepted or copied (``n_path`` is 0)
+        until ``check_tree_step`` has raised it."""
         path, n_path, following = tree.tree_accept(tokens, parents, picks, n_nodes)
+        n_path.masked_fill_(self.tree_status != 0, 0)
         kv_cache.ring_commit(self.rings, kv, pos, slots, path, n_path)
         return path, n_path, following
+
+    def check_tree_step(self) -> None:
+        """Wait for the tree steps so far; ``RuntimeError`` if a device wait of one of them expired (cleared by it)."""
+        st = int(self.tree_status.item())
+        if st:
+            self.tree_status.zero_()
+            _lib.check(st, "tree_step")
 
     def generate_drafted(self, prompt: torch.Tensor, state: FastState, n_tokens: int,
                          draft: Callable[[List[int]], Tuple[Sequence[int], Sequence[int]]], slot: int = 0,
@@ -589,6 +600,8 @@ class UtttB200:
             path, n_path, following = self.tree_commit(tok_t, par_t, picks, kv, pos_t, slot_t)
             steps += 1
             taken = path[0, :int(n_path.item())].tolist()
+            if not taken:
+                self.check_tree_step()
             pos += len(taken)
             for tok in [tokens[i] for i in taken[1:]] + [int(following.item())]:
                 done = ended(tok)

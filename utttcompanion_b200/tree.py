@@ -91,16 +91,17 @@ def _int_rows(name: str, t: Optional[torch.Tensor], shape, index: int) -> Option
 def tree_attention(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
                    k_ring: torch.Tensor, v_ring: torch.Tensor, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
                    n_heads: int, n_nodes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                   k_tree: Optional[torch.Tensor] = None, v_tree: Optional[torch.Tensor] = None
-                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Attention of B trees of N nodes (``uttt_attn_tree``); returns ``(out, k_tree, v_tree)``.
+                   k_tree: Optional[torch.Tensor] = None, v_tree: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Attention of B trees of N nodes (``uttt_attn_tree_status``); returns ``(out, k_tree, v_tree)``.
 
     ``qkv`` BF16 (B * N, [q | k | v] heads), rows any stride; ``parents`` int32 (B, N); ``pos`` and ``slots``
     int32 (B,): positions cached so far and ring slot of each row; ``k_ring`` / ``v_ring`` BF16
     (slots, n_kv, W, hd) of one layer, only read; ``rope_cos`` / ``rope_sin`` FP32 (positions, hd);
     ``n_nodes`` int32 (B,): nodes of each row (default N).  ``out`` BF16 (B * N, n_heads * hd), rows any stride,
     ``k_tree`` / ``v_tree`` BF16 (B, n_kv, N, hd): taken if given, else new (zeros); what lies behind a row's last
-    node is left as it was."""
+    node is left as it was.  ``status`` int32 (1,): becomes nonzero if a device wait expires (the wait's rows of
+    ``out`` are NaN then)."""
     _require_cuda(qkv, parents)
     dev, bf, index = qkv.device, torch.bfloat16, qkv.get_device()
     if parents.dim() != 2 or k_ring.dim() != 4:
@@ -140,17 +141,18 @@ def tree_attention(qkv: torch.Tensor, parents: torch.Tensor, pos: torch.Tensor, 
     rows = (B,)
     args = (_int_rows("parents", parents, (B, N), index), _int_rows("n_nodes", n_nodes, rows, index),
             _int_rows("pos", pos, rows, index), _int_rows("slots", slots, rows, index))
+    word = _int_rows("status", status, (1,), index)
     if B == 0:
         return out, k_tree, v_tree
     on, stream = _launch(dev)
     with on:
-        st = _lib.load().uttt_attn_tree(B, N, n_heads, n_kv, hd, W, n_slots, table[0], qkv.data_ptr(),
-                                        qkv_ld if R > 1 else qkv.shape[1], *args, k_ring.data_ptr(),
-                                        v_ring.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
-                                        k_tree.data_ptr(), v_tree.data_ptr(), out.data_ptr(),
-                                        out_ld if R > 1 else q_dim, stream)
+        st = _lib.load().uttt_attn_tree_status(B, N, n_heads, n_kv, hd, W, n_slots, table[0], qkv.data_ptr(),
+                                               qkv_ld if R > 1 else qkv.shape[1], *args, k_ring.data_ptr(),
+                                               v_ring.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(),
+                                               k_tree.data_ptr(), v_tree.data_ptr(), out.data_ptr(),
+                                               out_ld if R > 1 else q_dim, word, 0, stream)
     if st:
-        _lib.check(st, "uttt_attn_tree")
+        _lib.check(st, "uttt_attn_tree_status")
     return out, k_tree, v_tree
 
 
