@@ -63,6 +63,7 @@ constexpr int SM_TAIL = SM_BINS;          // the bin of everything beyond SM_RAN
 constexpr int SM_MAX_CTAS = 8;
 constexpr int SM_MAX_V = 262144;
 constexpr int SM_MAX_PART = 131071;      // candidates per CTA: sums of as many limbs of up to 2^15 stay below 2^32
+constexpr int SM_MAX_VECS = 16384;       // 8-logit vectors per CTA: 1024 a warp, so a lane adds at most 256 weights
 constexpr float SM_RANGE = 24.f;         // x up to here has bins (64 to the unit) and exact weights
 constexpr int SM_STEPS = 128;            // table entries per octave
 constexpr float SM_GREEDY_T = 1e-5f;     // _sample_next_token's greedy border
@@ -981,7 +982,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
     wt = (double)w.tail_weight(y);
     return true;
   };
-  double sum = 0.0;                      // at most 2^8 weights of 2^45 (a warp's candidates by 32): exact
+  double sum = 0.0;                      // at most 2^8 weights of 2^45 (SM_MAX_VECS): exact
   unsigned count = 0u;
   auto add = [&](unsigned bits) {
     double wt;
@@ -1105,12 +1106,14 @@ extern "C" int uttt_sample(int rows, int V, const void* logits, int logits_f32, 
   ProfScope ps(UTTT_PROF_ARGMAX, st);
   const int lim = active_limit < V ? active_limit : V;
   // A row is split over a cluster of S while the rows alone leave SMs idle (two CTAs fit an SM; at least 2048 logits per
-  // CTA), and where a CTA's part would be too large for the histogram's limbs (ids 0, 1 and 3 are no candidates).
+  // CTA), and where a CTA's part would be too large for the histogram's limbs (ids 0, 1 and 3 are no candidates) or for
+  // the lanes' sums.
   // At top-p 0.95, S = 1 / 2 / 4 / 8, launches one by one: one row of 32000 46 / 40 / 34 / 32 us, 64 rows 53 / 42 / 42 /
   // 63, 333 rows of 8003 53 / 73 / 124 / 250, 256 rows of 131072 199 / 222 / 266 / 362.
   const int nvec = (lim + 7) / 8;
   int S = 1;
   while (S < SM_MAX_CTAS && ((S == 1 ? lim - 3 : (nvec + S - 1) / S * 8) > SM_MAX_PART ||
+                             (nvec + S - 1) / S > SM_MAX_VECS ||
                              ((long long)rows * 2 * S <= 2 * num_sms() && lim / (2 * S) >= 2048)))
     S *= 2;
   const int part = (nvec + S - 1) / S;
