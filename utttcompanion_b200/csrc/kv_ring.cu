@@ -72,6 +72,7 @@ extern "C" int uttt_kv_ring_commit(int n_layers, int B, int N, int n_kv, int hd,
                    aligned16(v_tree) && aligned16(k_ring) && aligned16(v_ring),
                UTTT_ERR_UNSUPPORTED);
   UTTT_REQUIRE(N <= 64 && B <= 65535 && n_layers <= 1 << 20 && n_kv <= 1 << 16, UTTT_ERR_UNSUPPORTED);
+  UTTT_REQUIRE((long long)N * n_kv * (hd / 8) <= 1 << 30, UTTT_ERR_UNSUPPORTED);   // pieces of a row, counted in an int
   cudaStream_t st = (cudaStream_t)stream;
   ring_commit_kernel<<<dim3(2 * n_layers, B), 256, 0, st>>>(
       n_layers, N, n_kv, hd / 8, W, n_slots, (const uint4*)k_tree, (const uint4*)v_tree, tree_stride / 8,
@@ -86,14 +87,15 @@ extern "C" int uttt_kv_ring_fork(int n_layers, int n_pairs, int n_kv, int hd, in
   UTTT_REQUIRE(k_ring && v_ring && src && dst && ring_stride >= (long long)n_slots * n_kv * W * hd,
                UTTT_ERR_INVALID);
   UTTT_REQUIRE(hd % 8 == 0 && ring_stride % 8 == 0 && aligned16(k_ring) && aligned16(v_ring), UTTT_ERR_UNSUPPORTED);
-  UTTT_REQUIRE((long long)n_layers * 2 * n_kv <= 65535 && (long long)W * (hd / 8) <= 0x7fffffff,
+  // the kernel counts a head's 16-byte pieces in an int, a grid's stride past the last one
+  UTTT_REQUIRE((long long)n_layers * 2 * n_kv <= 65535 && (long long)W * (hd / 8) <= 1 << 30 && n_slots <= 1 << 30,
                UTTT_ERR_UNSUPPORTED);
   // Pairs run in rounds: one goes once no other waiting pair still reads its destination, so chains (5 -> 3,
   // 7 -> 5) read what was there before the call.  Everything is checked before the first launch.
   int* buf = new (std::nothrow) int[(size_t)2 * n_slots + n_pairs];
   UTTT_REQUIRE(buf, UTTT_ERR_INVALID);
   int *reads = buf, *written = buf + n_slots, *round = written + n_slots, rounds = 0;
-  for (int i = 0; i < 2 * n_slots; ++i) buf[i] = 0;
+  for (size_t i = 0; i < (size_t)2 * n_slots; ++i) buf[i] = 0;
   int status = UTTT_OK, left = 0;
   for (int i = 0; i < n_pairs && status == UTTT_OK; ++i) {
     round[i] = -1;
