@@ -366,7 +366,7 @@ int uttt_kv_ring_fill(int B, int L, int end_pos, int n_kv, int hd, int W, const 
  * ancestors less than W above it: what uttt_attn_decode gives along its path.
  *   qkv, k_ring, v_ring, rope_cos / rope_sin   as uttt_attn_decode; the rings
  *           have n_slots slots, the tables n_pos rows (positions past them take
- *           the last row); any W.  The rings are only read.
+ *           the last row); W <= 2^30.  The rings are only read.
  *   n_nodes nodes of each row (NULL: N); 0 leaves a row out.
  *   k_tree, v_tree  BF16 (B, n_kv, N, hd): the nodes' RoPE'd keys and values
  *   out     BF16 rows (B * N, out_ld), heads concatenated

@@ -28,3 +28,11 @@ def test_commit_counts_a_rows_pieces_in_an_int():
     n_kv, hd = 1 << 16, 1 << 16
     stride = 64 * n_kv * hd
     assert lib.uttt_kv_ring_commit(1, 1, 64, n_kv, hd, 1, 1, p, p, stride, p, p, stride, p, p, p, p, None) == SIZE
+
+
+def test_tree_attention_tells_places_by_ints():
+    lib = _lib.load()
+    keep, p = _buf()
+    for W in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert lib.uttt_attn_tree(1, 4, 4, 2, 64, W, 1, 16, p, 512, p, None, p, p, p, p, p, p, p, p, p, 256,
+                                  None) == SIZE

@@ -1325,7 +1325,8 @@ extern "C" int uttt_attn_tree_status(int B, int N, int n_heads, int n_kv, int hd
                UTTT_ERR_INVALID);
   UTTT_REQUIRE(n_heads % n_kv == 0 && n_heads / n_kv <= TR_MAX_REP && N <= TR_MAX_N, UTTT_ERR_UNSUPPORTED);
   UTTT_REQUIRE(hd == 32 || hd == 64 || hd == 128, UTTT_ERR_UNSUPPORTED);
-  UTTT_REQUIRE(B <= 65535 && n_kv <= 65535, UTTT_ERR_UNSUPPORTED);
+  // places of a ring are told by differences of up to twice the window, in ints
+  UTTT_REQUIRE(B <= 65535 && n_kv <= 65535 && W <= 1 << 30, UTTT_ERR_UNSUPPORTED);
   UTTT_REQUIRE(qkv_ld >= (n_heads + 2 * n_kv) * hd && out_ld >= n_heads * hd, UTTT_ERR_INVALID);
   cudaStream_t st = (cudaStream_t)stream;
   ProfScope ps(UTTT_PROF_ATTN, st);
