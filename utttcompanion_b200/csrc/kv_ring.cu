@@ -18,7 +18,7 @@ namespace uttt {
 namespace {
 
 // grid (layers * 2, B): tensor blockIdx.x of row blockIdx.y; V = hd / 8 pieces of 16 bytes per head vector
-__global__ void ring_commit_kernel(int L, int N, int n_kv, int V, int W, int n_slots, const uint4* __restrict__ ktree,
+__global__ void ring_commit_kernel(int N, int n_kv, int V, int W, int n_slots, const uint4* __restrict__ ktree,
                                    const uint4* __restrict__ vtree, long long tree_stride, uint4* __restrict__ kring,
                                    uint4* __restrict__ vring, long long ring_stride, const int* __restrict__ pos,
                                    const int* __restrict__ slot, const int* __restrict__ path,
@@ -75,7 +75,7 @@ extern "C" int uttt_kv_ring_commit(int n_layers, int B, int N, int n_kv, int hd,
   UTTT_REQUIRE((long long)N * n_kv * (hd / 8) <= 1 << 30, UTTT_ERR_UNSUPPORTED);   // pieces of a row, counted in an int
   cudaStream_t st = (cudaStream_t)stream;
   ring_commit_kernel<<<dim3(2 * n_layers, B), 256, 0, st>>>(
-      n_layers, N, n_kv, hd / 8, W, n_slots, (const uint4*)k_tree, (const uint4*)v_tree, tree_stride / 8,
+      N, n_kv, hd / 8, W, n_slots, (const uint4*)k_tree, (const uint4*)v_tree, tree_stride / 8,
       (uint4*)k_ring, (uint4*)v_ring, ring_stride / 8, pos, slot, path, n_path);
   return launch_status();
 }
