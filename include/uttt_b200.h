@@ -447,7 +447,8 @@ int uttt_greedy_argmax(int rows, int V, const void* logits, int logits_f32, long
 
 /*
  * Sampling of one token per row (_sample_next_token, model/uttt_model.py:1181-1235,
- * with top-k and min-p) from given uniform numbers, for packed decode batches.
+ * with top-k and min-p; its repetition penalty, if any, is the caller's to apply to
+ * the logits) from given uniform numbers, for packed decode batches.
  * The candidates are those of uttt_greedy_argmax (without its BF16 rounding);
  * a NaN or -inf logit is none.  With m the largest logit, w_i = exp((s_i - m) / T);
  * in the order (logit descending, id ascending) top_k keeps the first k, top_p

@@ -1,6 +1,6 @@
 // Sampling of one token per row from logits, with temperature, top-k, top-p and
 // min-p, from one given uniform number per row (the rules of _sample_next_token,
-// model/uttt_model.py:1181-1235, plus top-k and min-p; the random number is an
+// model/uttt_model.py:1181-1235, without its repetition penalty, plus top-k and min-p; the random number is an
 // input, so a pick is repeatable whatever else is in the batch).
 //
 // Mathematics.  A row's candidates are its ids below active_limit that are not

@@ -135,6 +135,15 @@ class uTTTModelB200:
         self._graph: Optional[DecodeGraph] = None
         self._graph_key = None
 
+    @property
+    def repetition_penalty(self) -> float:
+        """Of ``stream_generate`` (1: none); kept on the engine, whose packed sampled paths refuse one above 1."""
+        return self.engine.repetition_penalty
+
+    @repetition_penalty.setter
+    def repetition_penalty(self, value: float) -> None:
+        self.engine.repetition_penalty = float(value)
+
     @classmethod
     def from_reference(cls, model, device=None, max_personas: int = 1) -> "uTTTModelB200":
         """Build from a reference ``uTTTModel`` instance (its weights, config and vocabulary limit)."""

@@ -15,8 +15,8 @@ the GPU and runs the hot path with this package's kernels only:
 * ``generate_greedy`` -- ``stream_generate`` at temperature 0.
 * ``tree_step`` / ``tree_commit`` / ``generate_drafted`` -- a tree of drafted tokens verified in one
   packed step (the reference drafts along one line, ``model/uttt_model.py:1052-1179``).
-* ``sample`` / ``generate_replies`` -- sampled tokens (``_sample_next_token``, ``:1181-1235``) from given
-  random numbers; several replies of one prompt from forked KV rings.
+* ``sample`` / ``generate_replies`` -- sampled tokens (``_sample_next_token``, ``:1181-1235``, without its
+  repetition penalty, which these paths refuse) from given random numbers; several replies of one prompt from forked KV rings.
 * ``test_time_update`` -- ``uTTTModel.test_time_update`` with the chunk-first
   shared schedule (``model/uttt_model.py:453-608``): all layers of a chunk read
   the chunk-start snapshot; their writes advance one cursor.
@@ -161,6 +161,8 @@ class UtttB200:
         self.rope_cos, self.rope_sin = cos.to(dev).contiguous(), sin.to(dev).contiguous()
         self.n_pos = n_pos
         self.active_limit = SIMPLE_ACTIVE_VOCAB_LIMIT if cfg.vocab_size >= 24000 else cfg.vocab_size
+        # of stream_generate; the packed sampled paths do not know it and refuse one above 1 (sampling.check_penalty)
+        self.repetition_penalty = float(getattr(cfg, "repetition_penalty", 1.0))
         self.qkv_dim = (cfg.n_heads + 2 * cfg.n_kv_heads) * hd
         self.max_personas = max_personas
         # keys, then values, of every layer: one tensor, so that one launch can copy all of a persona's rings
@@ -549,6 +551,7 @@ class UtttB200:
         ring also holds the path's tokens behind it."""
         sampling.check_settings(temperature, top_k, top_p, min_p)
         sampled = temperature > 1e-5
+        sampling.check_penalty(self, temperature)
         if sampled and (u is None or u.numel() < n_tokens):
             raise ValueError("sampled generation needs one number per token")
         if n_tokens < 1:
@@ -617,6 +620,7 @@ class UtttB200:
         forked to one slot per reply (``slots``; default 0 .. n_replies - 1), and the replies decode as one packed
         batch, each from its own random numbers (``sampling.reply_uniforms(n_tokens, seed + reply)``)."""
         sampling.check_settings(temperature, top_k, top_p, min_p)
+        sampling.check_penalty(self, temperature)
         slots = list(range(n_replies)) if slots is None else [int(s) for s in slots]
         if n_replies < 1 or len(slots) != n_replies or len(set(slots)) != n_replies or n_tokens < 1 \
                 or min(slots) < 0 or max(slots) >= self.max_personas:

@@ -1,8 +1,8 @@
 """Sampling of one token per row from given random numbers (``uttt_sample``).
 
 ``UtttB200.greedy``'s counterpart at temperature > 0: the rules of
-``uTTTModel._sample_next_token`` (``model/uttt_model.py:1181-1235``) with top-k
-and min-p beside top-p, for every row of a packed batch in one launch, each row
+``uTTTModel._sample_next_token`` (``model/uttt_model.py:1181-1235``) without its
+repetition penalty (``check_penalty``), with top-k and min-p beside top-p, for every row of a packed batch in one launch, each row
 with its own settings.  The uniform numbers are inputs, so a pick depends on
 its row's logits, settings and number alone.
 """
@@ -41,6 +41,15 @@ def check_settings(temperature: float = 1.0, top_k: Optional[int] = None, top_p:
         raise ValueError("top_p must be finite and in (0, 1]")
     if min_p is not None and (not math.isfinite(min_p) or not 0 <= min_p <= 1):
         raise ValueError("min_p must be finite and in [0, 1]")
+
+
+def check_penalty(engine, temperature: float) -> None:
+    """The ``ValueError`` of sampled generation on an engine whose model asks for a repetition penalty (``:1181-1235``:
+    the scores of the last 48 ids).  The packed paths keep no ids beside the logits; ``dropin.uTTTModelB200``'s
+    ``stream_generate`` applies it."""
+    if temperature > 1e-5 and getattr(engine, "repetition_penalty", 1.0) > 1.0:
+        raise ValueError("packed sampling applies no repetition penalty: set repetition_penalty to 1, or use "
+                         "uTTTModelB200.stream_generate")
 
 
 def reply_uniforms(n: int, seed: int) -> torch.Tensor:

@@ -310,6 +310,7 @@ class ServingEngine:
         if type(max_new_tokens) is not int or max_new_tokens < 1:
             raise ValueError("max_new_tokens must be a positive integer")
         sampling.check_settings(temperature, top_k, top_p, min_p)
+        sampling.check_penalty(self.engine, temperature)
         if temperature > 1e-5:
             if max_new_tokens > self.max_sampled_tokens:
                 raise ValueError(f"this engine samples replies of up to {self.max_sampled_tokens} tokens "
