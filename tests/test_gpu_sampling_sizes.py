@@ -45,3 +45,11 @@ def test_limits_inside_a_wider_row():
         assert all(torch.equal(a[:2], b) for a, b in zip(whole, two))
         want = sample_row(x[0].float().cpu().numpy(), float(u[0]), temperature=1e3, limit=limit)
         assert (int(whole.ids[0]), int(whole.kept[0])) == want[:2]
+
+
+def test_numbers_of_no_row_are_refused():
+    x = torch.randn(1, 100, device=DEV)
+    for u in (torch.tensor(0.5, device=DEV), torch.rand(1, 1, 1, device=DEV)):
+        with pytest.raises(ValueError):
+            sampling.sample(x, u)
+    assert sampling.sample(x, torch.rand(1, 1, device=DEV)).ids.shape == (1,)

@@ -33,3 +33,9 @@ def test_the_model_and_its_engine_have_one_penalty():
     m.engine = SimpleNamespace(repetition_penalty=1.0)
     m.repetition_penalty = 1.3
     assert m.engine.repetition_penalty == 1.3 and m.repetition_penalty == 1.3
+
+
+@pytest.mark.parametrize("top_k", [float("inf"), float("nan"), -float("inf")])
+def test_a_top_k_that_is_no_number_of_ids(top_k):
+    with pytest.raises(ValueError):
+        sampling.check_settings(top_k=top_k)

@@ -35,7 +35,7 @@ def check_settings(temperature: float = 1.0, top_k: Optional[int] = None, top_p:
     """The ``ValueError`` of settings that no call takes (the reference's checks, ``:1190-1197``)."""
     if not math.isfinite(temperature) or temperature < 0:
         raise ValueError("temperature must be finite and nonnegative")
-    if top_k is not None and (int(top_k) != top_k or not 0 <= top_k < 2 ** 31):
+    if top_k is not None and (not math.isfinite(top_k) or int(top_k) != top_k or not 0 <= top_k < 2 ** 31):
         raise ValueError("top_k must be a nonnegative integer")
     if top_p is not None and (not math.isfinite(top_p) or not 0 < top_p <= 1):
         raise ValueError("top_p must be finite and in (0, 1]")
@@ -124,9 +124,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Setting = 1.0, to
     rows, V = logits.shape
     if not 6 < V <= MAX_VOCAB:
         raise ValueError(f"logits must be FP32 or BF16 (rows, V) with 6 < V <= {MAX_VOCAB}")
-    n_u = 1 if u.dim() == 1 else u.shape[-1]
-    if u.get_device() != index or u.dtype is not f or u.dim() > 2 or u.shape[0] != rows or not u.is_contiguous():
+    if u.get_device() != index or u.dtype is not f or u.dim() not in (1, 2) or u.shape[0] != rows \
+            or not u.is_contiguous():
         raise ValueError("u must be a contiguous FP32 (rows,) or (rows, n) tensor beside the logits")
+    n_u = 1 if u.dim() == 1 else u.shape[1]
     if rows == 0:
         return Sampled(*(torch.empty(0, dtype=t, device=logits.device) for t in (torch.int32, torch.int32, f)))
     ld, step = logits.stride()
