@@ -147,3 +147,18 @@ def test_logits_repeat_themselves():
         got = [lg, eng.decode_step(ids, pos, slots, packed, down, zero), eng.rings[:, :, :3].clone()]
         want = want or got
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_replies_may_use_every_position_of_the_table():
+    """The last reply token is picked but never decoded from: T prompt ids and n tokens use T + n - 1 positions."""
+    cfg = ModelConfig(vocab_size=512, d_model=256, n_layers=2, n_heads=4, n_kv_heads=2, d_ff_fast=384,
+                      sliding_window_size=24, chunk_size=64, max_seq_len=512)
+    sd = reference_init_state_dict(cfg, seed=3)
+    small, large = UtttB200(sd, cfg, max_personas=2, max_positions=64), UtttB200(sd, cfg, max_personas=2)
+    prompt = torch.randint(6, 512, (30,), generator=torch.Generator().manual_seed(4))
+    for n in (33, 34, 35):
+        got = small.generate_replies(prompt, small.init_fast_state(1), n, 2, seed=1)
+        assert got == large.generate_replies(prompt, large.init_fast_state(1), n, 2, seed=1)
+        assert [len(r) for r in got] == [n, n]
+    with pytest.raises(ValueError):
+        small.generate_replies(prompt, small.init_fast_state(1), 36, 2, seed=1)

@@ -626,7 +626,7 @@ class UtttB200:
                 or min(slots) < 0 or max(slots) >= self.max_personas:
             raise ValueError("one KV slot of the engine per reply")
         T = prompt.numel()
-        if T < 1 or T + n_tokens >= self.n_pos:
+        if T < 1 or T + n_tokens - 2 >= self.n_pos:          # the last token but one is the last that is decoded from
             raise ValueError("empty prompt, or a reply longer than the RoPE table")
         packed, down = self.read_copies(state.w_up, state.w_gate, state.w_down)
         dev = self.device
