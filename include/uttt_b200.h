@@ -395,8 +395,8 @@ int uttt_attn_tree_status(int B, int N, int n_heads, int n_kv, int hd, int W, in
 /*
  * The accepted path of each row's tree: node 0 (the token that was pending), then
  * from every node on its lowest later child whose token is the pick after that
- * node, until there is none (the rule that keeps a drafted reply equal to the
- * undrafted one).  tokens, parents, picks: (B, N); path (B, N): the nodes, -1
+ * node, until there is none (so a drafted reply differs from the undrafted one
+ * only where their logits' roundings pick differently).  tokens, parents, picks: (B, N); path (B, N): the nodes, -1
  * behind the last; n_path (B); next (B): the pick after the path's last node.
  * A row without nodes gets n_path 0 and next -1.  N <= 64.
  */

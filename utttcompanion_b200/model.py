@@ -546,8 +546,9 @@ class UtttB200:
         """``generate_greedy`` (or, at temperature > 0, sampled generation from the numbers ``u`` (n_tokens,)) with
         drafted tokens: ``draft(ids)`` proposes, after the prompt and the reply so far, a tree of tokens
         (``tokens[i]`` at node i + 1, ``parents[i]`` < i + 1; node 0 is the last id), e.g. ``tree.PromptLookup()``.
-        Token t of the reply is the pick from its own logits with ``u[t]``, as without a draft, so drafts change how
-        many steps the reply takes, not the reply.  Returns (ids, steps).  After a stop inside an accepted path the
+        Token t of the reply is the pick from its own logits with ``u[t]``, as without a draft.  A draft changes how
+        many steps the reply takes, and the reply itself only at near-ties: a step over a tree rounds its logits (BF16)
+        elsewhere than a decode step does.  Equal calls give equal replies.  Returns (ids, steps).  After a stop inside an accepted path the
         ring also holds the path's tokens behind it."""
         sampling.check_settings(temperature, top_k, top_p, min_p)
         sampled = temperature > 1e-5

@@ -2,9 +2,10 @@
 
 ``UtttB200.greedy``'s counterpart at temperature > 0: the rules of
 ``uTTTModel._sample_next_token`` (``model/uttt_model.py:1181-1235``) without its
-repetition penalty (``check_penalty``), with top-k and min-p beside top-p, for every row of a packed batch in one launch, each row
-with its own settings.  The uniform numbers are inputs, so a pick depends on
-its row's logits, settings and number alone.
+repetition penalty (``check_penalty``), with top-k and min-p beside top-p, for
+every row of a packed batch in one launch, each row with its own settings.  The
+uniform numbers are inputs, so a pick depends on its row's logits, settings and
+number alone (the logits' own last bits may depend on how many rows a step has).
 """
 
 from __future__ import annotations
