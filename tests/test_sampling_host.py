@@ -39,3 +39,13 @@ def test_the_model_and_its_engine_have_one_penalty():
 def test_a_top_k_that_is_no_number_of_ids(top_k):
     with pytest.raises(ValueError):
         sampling.check_settings(top_k=top_k)
+
+
+def test_a_sampled_row_is_not_left_with_another_turns_numbers():
+    rows = sampling.SamplingRows(torch.device("cpu"), 2, 4)
+    rows.set(0, 0.7, u=torch.tensor([0.25, 0.5]))
+    for u in (None, torch.zeros(0)):
+        with pytest.raises(ValueError):
+            rows.set(0, 0.9, u=u)
+    assert rows.temperature.tolist() == [pytest.approx(0.7), 0.0]
+    rows.set(0)                                                  # greedy again: none needed

@@ -77,6 +77,8 @@ class SamplingRows:
         check_settings(temperature, top_k, top_p, min_p)
         if not 0 <= row < self.temperature.shape[0]:
             raise ValueError("row outside the table")
+        if temperature > 1e-5 and (u is None or u.numel() == 0):
+            raise ValueError("a sampled row needs its random numbers")
         if u is not None and u.numel() > self.uniforms:
             raise ValueError(f"a row holds {self.uniforms} random numbers")
 
