@@ -133,13 +133,17 @@ __global__ void __launch_bounds__(G_THREADS, 1) gemm_kernel(const __grid_constan
 // Row-wise finishing of a projection: up to 6 column segments per row.  A row
 // is striped over a cluster of CF CTAs (grid (M, CF); CF grows while the rows
 // alone would leave SMs idle, so a decode batch of one row still spreads over
-// 8 SMs), 4 independent loads per thread in flight; a row statistic (the
-// RMSNorm sums of squares) is summed over the cluster's CTAs in distributed
-// shared memory, in rank order.  The FP32 accumulator row is zeroed after use,
-// so the next projection can accumulate into it without a memset.
+// 8 SMs), four columns a thread; a row statistic (the RMSNorm sums of squares) is
+// summed over the cluster's CTAs in distributed shared memory, in rank order.
+//
+// What bounds it: latency for few rows, then reading the K ranges' sums from L2.  They
+// come as 16-byte vectors, two ranges in flight: the projections of 1024 rows of 2560
+// take 41.6 us and of one row 9.7 (residual and norm); a column a load 47.8 and 9.9.
+// With one range in flight a row takes 10.3 us, with four or eight 9.9 and 10.6: the
+// registers, and a longer loop that every launch fetches anew, cost more than they hide.
 // ---------------------------------------------------------------------------
 constexpr int F_THREADS = 256;
-constexpr int F_UNROLL = 4;
+constexpr int F_COLS = 4;
 
 __device__ __forceinline__ float bf16r(float x) { return __bfloat162float(__float2bfloat16(x)); }
 
@@ -159,35 +163,87 @@ struct SegPack {
   UtttSegment s[6];
 };
 
-// The sums of columns i, i + stride, ... (below len) of a row over the K ranges, whose rows lie `plane` apart.
-__device__ __forceinline__ void row_sums(float (&v)[F_UNROLL], const float* ys, int i, int stride, int len, int ranges,
-                                         size_t plane) {
+// Columns i .. i + 3 (below len) of a row.  VEC: the row starts on a vector of four; what is left at its end, and every
+// column of other rows, is read and written one by one.
+template <class T, class V>
+__device__ __forceinline__ bool as_vector(const T* row, int i, int len) {
+  return (reinterpret_cast<uintptr_t>(row) & (sizeof(V) - 1)) == 0 && i + F_COLS <= len;
+}
+__device__ __forceinline__ void load4(float (&v)[F_COLS], const float* row, int i, int len) {
+  if (as_vector<float, float4>(row, i, len)) {
+    const float4 x = *reinterpret_cast<const float4*>(row + i);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+  } else {
 #pragma unroll
-  for (int u = 0; u < F_UNROLL; ++u) v[u] = i + u * stride < len ? ys[i + u * stride] : 0.f;
-#pragma unroll 4
+    for (int u = 0; u < F_COLS; ++u) v[u] = i + u < len ? row[i + u] : 0.f;
+  }
+}
+__device__ __forceinline__ void load4(float (&v)[F_COLS], const __nv_bfloat16* row, int i, int len) {
+  if (as_vector<__nv_bfloat16, uint2>(row, i, len)) {
+    const uint2 x = *reinterpret_cast<const uint2*>(row + i);
+    v[0] = bf16_lo(x.x), v[1] = bf16_hi(x.x), v[2] = bf16_lo(x.y), v[3] = bf16_hi(x.y);
+  } else {
+#pragma unroll
+    for (int u = 0; u < F_COLS; ++u) v[u] = i + u < len ? __bfloat162float(row[i + u]) : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(const UtttSegment& sg, int r, int i, const float (&v)[F_COLS]) {
+  if (sg.out_f32) {
+    float* row = reinterpret_cast<float*>(sg.out) + (size_t)r * sg.out_ld;
+    if (as_vector<float, float4>(row, i, sg.len)) {
+      *reinterpret_cast<float4*>(row + i) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < F_COLS; ++u)
+        if (i + u < sg.len) row[i + u] = v[u];
+    }
+  } else {
+    __nv_bfloat16* row = reinterpret_cast<__nv_bfloat16*>(sg.out) + (size_t)r * sg.out_ld;
+    if (as_vector<__nv_bfloat16, uint2>(row, i, sg.len)) {
+      *reinterpret_cast<uint2*>(row + i) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < F_COLS; ++u)
+        if (i + u < sg.len) row[i + u] = __float2bfloat16(v[u]);
+    }
+  }
+}
+// The sums of four columns over the K ranges, whose rows lie `plane` apart (a multiple of four where rows are vectors).
+__device__ __forceinline__ void row_sums(float (&v)[F_COLS], const float* ys, int i, int len, int ranges, size_t plane) {
+  load4(v, ys, i, len);
+#pragma unroll 2
   for (int k = 1; k < ranges; ++k) {
-    const float* yk = ys + k * plane;
+    float x[F_COLS];
+    load4(x, ys + k * plane, i, len);
 #pragma unroll
-    for (int u = 0; u < F_UNROLL; ++u)
-      if (i + u * stride < len) v[u] += yk[i + u * stride];
+    for (int u = 0; u < F_COLS; ++u) v[u] += x[u];
   }
 }
 
-__device__ __forceinline__ float seg_value(const UtttSegment& sg, float v, int r, int i, float rinv) {
+// What a segment's op takes beside y: the residual, or gamma or the bias (1 or 0 where there is none).
+__device__ __forceinline__ void load_aux(float (&v)[F_COLS], const UtttSegment& sg, int r, int i) {
+  if (sg.op == UTTT_SEG_RESID) {
+    load4(v, reinterpret_cast<const __nv_bfloat16*>(sg.aux) + (size_t)r * sg.aux_ld, i, sg.len);
+  } else if (sg.aux && sg.op != UTTT_SEG_STORE) {
+    load4(v, reinterpret_cast<const float*>(sg.aux), i, sg.len);
+    if (sg.op == UTTT_SEG_RMSNORM)
+#pragma unroll
+      for (int u = 0; u < F_COLS; ++u) v[u] = bf16r(v[u]);
+  } else {
+#pragma unroll
+    for (int u = 0; u < F_COLS; ++u) v[u] = sg.op == UTTT_SEG_RMSNORM ? 1.f : 0.f;
+  }
+}
+__device__ __forceinline__ float seg_value(const UtttSegment& sg, float v, float aux, float rinv) {
   switch (sg.op) {
     case UTTT_SEG_RESID:
-      return __bfloat162float((reinterpret_cast<const __nv_bfloat16*>(sg.aux) + (size_t)r * sg.aux_ld)[i]) + bf16r(v);
-    case UTTT_SEG_RMSNORM: {
+      return aux + bf16r(v);
+    case UTTT_SEG_RMSNORM:
       // F.rms_norm of the BF16 projection: FP32 statistics, weight applied in FP32
-      float o = bf16r(v) * rinv;
-      if (sg.aux) o *= bf16r(reinterpret_cast<const float*>(sg.aux)[i]);
-      return o;
-    }
-    case UTTT_SEG_SIGMOID: {
+      return bf16r(v) * rinv * aux;
+    case UTTT_SEG_SIGMOID:
       // scale * sigmoid(linear + bias) with the BF16 roundings of F.linear, sigmoid and the product
-      const float lin = bf16r(v + (sg.aux ? reinterpret_cast<const float*>(sg.aux)[i] : 0.f));
-      return bf16r(sg.scale * bf16r(sigmoidf_(lin)));
-    }
+      return bf16r(sg.scale * bf16r(sigmoidf_(bf16r(v + aux))));
     default:
       return v;
   }
@@ -217,64 +273,57 @@ __global__ void __launch_bounds__(F_THREADS) finish_kernel(const float* __restri
   __shared__ float red[F_THREADS / 32];
   __shared__ float cred[6];
   const int CF = gridDim.y, r = blockIdx.x, tid = threadIdx.x;
-  const int first = blockIdx.y * F_THREADS + tid, stride = CF * F_THREADS;   // this CTA's stripe of the row
+  const int first = (blockIdx.y * F_THREADS + tid) * F_COLS, stride = CF * F_THREADS * F_COLS;   // of the row's columns
   pdl_wait();
   pdl_trigger();
   const float* yrow = y + (size_t)r * N;
   for (int si = 0; si < nseg; ++si) {
     const UtttSegment& sg = sp.s[si];
-    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(sg.out) + (size_t)r * sg.out_ld;
-    float* outf = reinterpret_cast<float*>(sg.out) + (size_t)r * sg.out_ld;
+    float v[F_COLS], aux[F_COLS], ss = 0.f;
     if (sg.op == UTTT_SEG_NORM) {
       // rms_norm of a BF16 row an earlier segment of this row has just written (every CTA of the cluster)
       row_sync(CF);
       const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(sg.aux) + (size_t)r * sg.aux_ld;
       const float* gamma = reinterpret_cast<const float*>(sg.aux2);
-      float ss = 0.f;
       for (int i = first; i < sg.len; i += stride) {
-        const float v = __bfloat162float(src[i]);
-        ss += v * v;
+        load4(v, src, i, sg.len);
+#pragma unroll
+        for (int u = 0; u < F_COLS; ++u) ss += v[u] * v[u];
       }
       const float rinv = rsqrtf(cluster_row_sum(fblock_sum(ss, red), cred, si, CF) / (float)sg.len + eps);
       for (int i = first; i < sg.len; i += stride) {
-        float v = __bfloat162float(src[i]) * rinv;
-        if (gamma) v *= bf16r(gamma[i]);
-        if (sg.out_f32)
-          outf[i] = v;
-        else
-          out[i] = __float2bfloat16(v);
+        load4(v, src, i, sg.len);
+        if (gamma) load4(aux, gamma, i, sg.len);
+#pragma unroll
+        for (int u = 0; u < F_COLS; ++u) {
+          v[u] *= rinv;
+          if (gamma) v[u] *= bf16r(aux[u]);
+        }
+        store4(sg, r, i, v);
       }
       continue;
     }
     const float* ys = yrow + sg.start;
+    int held = -1;                       // the columns whose sums are in v
     float rinv = 1.f;
     if (sg.op == UTTT_SEG_RMSNORM) {
-      float ss = 0.f;
-      for (int i0 = first; i0 < sg.len; i0 += stride * F_UNROLL) {
-        float v[F_UNROLL];
-        row_sums(v, ys, i0, stride, sg.len, ranges, plane);
+      for (int i = first; i < sg.len; i += stride) {
+        row_sums(v, ys, held = i, sg.len, ranges, plane);
 #pragma unroll
-        for (int u = 0; u < F_UNROLL; ++u) {
+        for (int u = 0; u < F_COLS; ++u) {
           const float x = bf16r(v[u]);
           ss += x * x;
         }
       }
       rinv = rsqrtf(cluster_row_sum(fblock_sum(ss, red), cred, si, CF) / (float)sg.len + eps);
     }
-    for (int i0 = first; i0 < sg.len; i0 += stride * F_UNROLL) {
-      float v[F_UNROLL];
-      row_sums(v, ys, i0, stride, sg.len, ranges, plane);
+    for (int i = first; i < sg.len; i += stride) {
+      load_aux(aux, sg, r, i);
+      if (i != held) row_sums(v, ys, held = i, sg.len, ranges, plane);   // (a short row's are still there)
 #pragma unroll
-      for (int u = 0; u < F_UNROLL; ++u) {
-        const int i = i0 + u * stride;
-        if (i < sg.len) {
-          const float o = seg_value(sg, v[u], r, i, rinv);
-          if (sg.out_f32)
-            outf[i] = o;
-          else
-            out[i] = __float2bfloat16(o);
-        }
-      }
+      for (int u = 0; u < F_COLS; ++u) v[u] = seg_value(sg, v[u], aux[u], rinv);
+      held = -1;
+      store4(sg, r, i, v);
     }
   }
   if (CF > 1) cg::this_cluster().sync();   // no CTA leaves while another may still read its row statistics
@@ -367,7 +416,7 @@ extern "C" int uttt_linear(int M, int N, int K, const void* x, const void* w, in
   memset(&sp, 0, sizeof(sp));
   for (int i = 0; i < nseg; ++i) sp.s[i] = segs[i];
   int CF = 1;   // CTAs per row (a cluster): spread narrow batches over the SMs
-  while (CF < 8 && (long long)M * CF < 2LL * num_sms() && N > CF * F_THREADS * F_UNROLL) CF *= 2;
+  while (CF < 8 && (long long)M * CF < 2LL * num_sms() && N > CF * F_THREADS * F_COLS) CF *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(M, CF);
   cfg.blockDim = dim3(F_THREADS);
