@@ -739,35 +739,40 @@ __global__ void __launch_bounds__(LN_THREADS) readout_ln_kernel(const double* __
   if (c >= Cc) return;
   const double* zrow = zbase + ((size_t)b * zrows + c) * d;
   const size_t tok = (size_t)b * T + tok0 + c;
-  float z[LN_MAXV];
+  // two columns a load, all of a thread's loads in flight
+  constexpr int NZ = LN_MAXV / 2;
+  double2 zd[NZ];
+#pragma unroll
+  for (int j = 0; j < NZ; ++j) {
+    const int i = 2 * (tid + j * LN_THREADS);
+    zd[j] = i < d ? *reinterpret_cast<const double2*>(zrow + i) : make_double2(0.0, 0.0);
+  }
+  float z[2 * NZ];
   float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < LN_MAXV; ++j) {
-    const int i = tid + j * LN_THREADS;
-    z[j] = 0.f;
-    if (i < d) {
-      z[j] = (float)zrow[i];
-      sum += z[j];
-    }
+  for (int j = 0; j < NZ; ++j) {
+    z[2 * j] = (float)zd[j].x;
+    z[2 * j + 1] = (float)zd[j].y;
+    sum += z[2 * j] + z[2 * j + 1];
   }
   const float dinv = 1.f / (float)d;
   const float mean = block_sum(sum, red) * dinv;
   float sq = 0.f;
 #pragma unroll
-  for (int j = 0; j < LN_MAXV; ++j) {
-    const int i = tid + j * LN_THREADS;
-    if (i < d) sq += (z[j] - mean) * (z[j] - mean);
-  }
+  for (int j = 0; j < 2 * NZ; ++j)
+    if (2 * (tid + (j >> 1) * LN_THREADS) < d) sq += (z[j] - mean) * (z[j] - mean);
   const float rstd = rsqrtf(block_sum(sq, red) * dinv + eps);
 #pragma unroll
-  for (int j = 0; j < LN_MAXV; ++j) {
-    const int i = tid + j * LN_THREADS;
+  for (int j = 0; j < NZ; ++j) {
+    const int i = 2 * (tid + j * LN_THREADS);
     if (i < d) {
-      const float y = __bfloat162float(x[tok * d + i]) + ((z[j] - mean) * rstd * ln_w[i] + ln_b[i]);
+      const uint32_t xx = *reinterpret_cast<const uint32_t*>(x + tok * d + i);
+      const float y0 = bf16_lo(xx) + ((z[2 * j] - mean) * rstd * ln_w[i] + ln_b[i]);
+      const float y1 = bf16_hi(xx) + ((z[2 * j + 1] - mean) * rstd * ln_w[i + 1] + ln_b[i + 1]);
       if (out_bf16)
-        reinterpret_cast<__nv_bfloat16*>(out)[tok * d + i] = __float2bfloat16(y);
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(out) + tok * d + i) = pack_bf16x2(y0, y1);
       else
-        reinterpret_cast<float*>(out)[tok * d + i] = y;
+        *reinterpret_cast<float2*>(reinterpret_cast<float*>(out) + tok * d + i) = make_float2(y0, y1);
     }
   }
 }
