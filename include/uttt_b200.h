@@ -462,7 +462,9 @@ int uttt_greedy_argmax(int rows, int V, const void* logits, int logits_f32, long
  * u[r * u_ld + u_index[r]] (u_index NULL: 0; clamped to [0, u_len)).
  *   logits  rows of V (ld elements apart), FP32 or BF16, any alignment
  *   ids     the picks; kept (optional) the number of kept ids; prob (optional)
- *           the pick's share of the kept mass.  A row without candidates gets
+ *           the pick's share of the kept mass (both from the whole-number weights:
+ *           an id 2^40 times less likely than the first weighs a few units, one
+ *           2^46 times less likely none).  A min_p below 2^-126 counts as 0.  A row without candidates gets
  *           the id that uttt_greedy_argmax gives it, kept 0 and prob 0.
  * V <= 262144, rows <= 65535.  No workspace.
  */

@@ -42,8 +42,11 @@
 // top-p 0.95 take 196 us, 140 warp instructions per 32 logits over the four walks at
 // 0.73 a cycle and scheduler (FP64 14 %, ALU 44 %, DRAM 4 % busy): 8 % of the time for
 // the largest logit, 42 % for the histogram, 13 % for the gather, 31 % for the kept
-// mass.  Without cuts they take 100 us.  Small ones: latency.  A row of
-// 32000 takes 16.7 us, 7 cluster barriers among them.
+// mass.  Without cuts they take 100 us.  Small ones: latency, 7 cluster barriers and
+// more walks the more is kept.  In a row of calls a row of 32000 FP32 logits takes 17 us
+// at T 0.7, top-p 0.9 (5 ids kept, finished in the list) and 21 at T 1, top-p 0.95
+// (6200 kept; 32 alone); 64 rows 17 us at top-k 50 and 30 at top-p 0.95; 333 rows of
+// 8003 24 and 43 (38 for rows of 8000, which all start on 16 bytes).
 #include <cooperative_groups.h>
 
 #include "common.cuh"

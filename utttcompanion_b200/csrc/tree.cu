@@ -28,11 +28,16 @@
 // scores, statistics and sums are FP32.
 //
 // What bounds it (1.58B heads unless said).  64 rows of 1 to 16 nodes over window
-// 512: 28.7 us; of a full wave's 22 us 3 are the nodes' paths and RoPE and 2 the
-// output, between them the rings stream at the HBM rate (77 MB).  8 rows of 31 nodes
-// over window 8192, one KV head: 32.5 us, 16 tiles a CTA at 1350 cycles (the softmax
-// between two products on the tensor cores; its powers alone are 512) and 6000 cycles
-// for the cluster's join.  One row of 5 nodes: 13 us, the host's side of the call.
+// 512: 30.4 us, of which 59 rows in one wave take 22.5; of a CTA's 28000 cycles 8500
+// are the nodes' paths, loads and RoPE before the first tile and 2400 the output,
+// between them the rings stream at the HBM rate (77 MB).  8 rows of 31 nodes over
+// window 8192, one KV head: 32.6 us.  One of its CTAs ends after 43900 cycles (22 us):
+// 9300 before the first tile, 24000 in 16 tiles (1500 each: the softmax between two
+// products on the tensor cores, its powers alone 512) and 9700 for the cluster's join;
+// the rest is SMs that hold two such CTAs while others hold none (the tensor pipe is
+// busy 57 % on the busiest SM, 25 % on average).  One row of 5 nodes: 13 us, the
+// host's side of the call (9 in a captured graph).  Head dim 32: 28 us for the 64
+// rows, 46 for the 8 over window 8192.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
