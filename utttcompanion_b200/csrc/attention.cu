@@ -66,10 +66,9 @@ __host__ __device__ constexpr size_t dec_smem_floats(int hd, int rep, int span) 
 // sum [REP][2] (read by the cluster).
 template <int HD, int REP>
 __global__ void __launch_bounds__(DEC_THREADS) attn_decode_kernel(
-    const __nv_bfloat16* __restrict__ qkv, int qkv_ld, const int* __restrict__ pos, const int* __restrict__ slot,
-    __nv_bfloat16* __restrict__ kring, __nv_bfloat16* __restrict__ vring, int n_kv, int W,
-    const float* __restrict__ cos_t, const float* __restrict__ sin_t, float scale, __nv_bfloat16* __restrict__ out,
-    int out_ld) {
+    const __nv_bfloat16* qkv, int qkv_ld, const int* pos, const int* slot, __nv_bfloat16* kring, __nv_bfloat16* vring,
+    int n_kv, int W, const float* __restrict__ cos_t, const float* __restrict__ sin_t, float scale,
+    __nv_bfloat16* __restrict__ out, int out_ld) {
   const int S = gridDim.z, span = W / S, s_lo = blockIdx.z * span, sp = dec_span_pad(span);
   extern __shared__ float dsm[];
   float* qs = dsm;                                    // [REP][HD]

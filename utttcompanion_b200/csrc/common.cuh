@@ -36,6 +36,9 @@ __device__ __forceinline__ void set_status(int* status, int code) {
 // pdl_wait: returns once every grid this launch depends on has completed and its
 // writes are visible (at once for a launch without the programmatic attribute).
 // pdl_trigger: lets the next launch in the stream start its prologue now.
+// A kernel launched so reads what earlier launches wrote through pointers that are neither __restrict__ nor given to
+// __ldg: the read-only path is for memory that nothing writes while the kernel lives, and this one may have started
+// before the writer ended.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -163,8 +163,7 @@ struct SegPack {
   UtttSegment s[6];
 };
 
-// Columns i .. i + 3 (below len) of a row.  VEC: the row starts on a vector of four; what is left at its end, and every
-// column of other rows, is read and written one by one.
+// Columns i .. i + 3 (below len) of a row: as one vector if the row starts on one, else, and at the row's end, one by one.
 template <class T, class V>
 __device__ __forceinline__ bool as_vector(const T* row, int i, int len) {
   return (reinterpret_cast<uintptr_t>(row) & (sizeof(V) - 1)) == 0 && i + F_COLS <= len;
@@ -267,7 +266,7 @@ __device__ __forceinline__ void row_sync(int CF) {
     cg::this_cluster().sync();
 }
 
-__global__ void __launch_bounds__(F_THREADS) finish_kernel(const float* __restrict__ y, int N, int ranges,
+__global__ void __launch_bounds__(F_THREADS) finish_kernel(const float* y, int N, int ranges,
                                                            size_t plane, int nseg,
                                                            const __grid_constant__ SegPack sp, float eps) {
   __shared__ float red[F_THREADS / 32];

@@ -309,8 +309,8 @@ __device__ __noinline__ Eight load_scalar(const char* src, int i, int V) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const int k = min(i + e, V - 1);     // what lies behind the row is masked by the caller
-    r.x[e] = F32 ? __ldg(reinterpret_cast<const unsigned*>(src) + k)
-                 : (unsigned)__ldg(reinterpret_cast<const unsigned short*>(src) + k) << 16;
+    r.x[e] = F32 ? reinterpret_cast<const unsigned*>(src)[k]
+                 : (unsigned)reinterpret_cast<const unsigned short*>(src)[k] << 16;
   }
   return r;
 }
@@ -863,9 +863,8 @@ __device__ __noinline__ void finish_list(Cluster c, const Weigher w, unsigned n,
 
 template <bool F32>
 __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(
-    const void* __restrict__ logits, long long ld, int V, int lim, int part, int stop_free, UtttSampling opt,
-    const float* __restrict__ u, long long u_ld, const int* __restrict__ u_index, int u_len, int* __restrict__ ids,
-    int* __restrict__ kept, float* __restrict__ prob) {
+    const void* logits, long long ld, int V, int lim, int part, int stop_free, UtttSampling opt, const float* u,
+    long long u_ld, const int* u_index, int u_len, int* ids, int* kept, float* prob) {
   extern __shared__ __align__(16) uint8_t smem[];
   SampleShared* sh = reinterpret_cast<SampleShared*>(smem);
   Cluster c{cg::this_cluster(), sh, (int)blockIdx.x, (int)gridDim.x, 0, 0};
